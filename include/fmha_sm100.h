@@ -21,6 +21,7 @@
  *   fmha_sm100_philox_*  — no counterpart: the reference takes a dense dropout mask
  *                          tensor (fmha/fmha_manual.cpp:433-449); these regenerate that
  *                          mask from (seed, offset) so that it never has to be stored.
+ *   fmha_sm100_causal_*  — no counterpart: the reference has no causal mask and one key head per query head.
  */
 #ifndef FMHA_SM100_H_
 #define FMHA_SM100_H_
@@ -162,6 +163,42 @@ typedef struct {
   const int64_t* philox_offset_dev; /* optional device int64 added to philox_offset, see fmha_fwd_params */
 } fmha_bwd_params;
 
+/* Causal attention of a packed variable-length batch with grouped heads: row i of a sequence sees its rows 0 to i, and query head h
+   reads key head h / (H / H_kv).  q, o (and d_o, dq) are [total_rows, H, D] views, k, v (and dk, dv) [total_rows, H_kv, D]; sequence b
+   owns rows [cu_seqlens[b], cu_seqlens[b+1]) of all of them (stride_b is not used), as with FMHA_MASK_CU_SEQLENS; one that is longer than
+   max_seqlen is cut there.  Rows outside the sequences are neither read into a result nor, without FMHA_FLAG_ZERO_UNCOVERED, written: what
+   they hold, an infinity or NaN included, does not matter.  Within a sequence an infinite or NaN value in V of a LATER row can reach rows
+   of the same 128 (a zero probability times it). */
+typedef struct {
+  int32_t struct_bytes; /* sizeof(fmha_causal_fwd_params) */
+  int32_t dtype;        /* FMHA_DTYPE_* */
+  int32_t B, H, H_kv, max_seqlen, D; /* H a multiple of H_kv; D in {64, 128} */
+  float scale;
+  fmha_tensor4 q, k, v; /* inputs */
+  fmha_tensor4 o;       /* output */
+  float* lse;           /* optional [H, total_rows] natural-log logsumexp */
+  const int32_t* cu_seqlens; /* device int32 [B+1] */
+  int32_t total_rows;
+  int32_t flags;        /* FMHA_FLAG_ZERO_UNCOVERED */
+  int32_t* status;      /* optional device int32[4] */
+} fmha_causal_fwd_params;
+
+typedef struct {
+  int32_t struct_bytes; /* sizeof(fmha_causal_bwd_params) */
+  int32_t dtype;
+  int32_t B, H, H_kv, max_seqlen, D;
+  float scale;
+  fmha_tensor4 q, k, v, o, d_o; /* inputs */
+  const float* lse;             /* from the forward call */
+  fmha_tensor4 dq, dk, dv;      /* outputs; dk and dv are summed over the query heads of a key head */
+  const int32_t* cu_seqlens;
+  int32_t total_rows;
+  void* workspace;              /* device scratch, 256-byte aligned, of fmha_sm100_causal_bwd_workspace_bytes() bytes */
+  size_t workspace_bytes;
+  int32_t flags;
+  int32_t* status;
+} fmha_causal_bwd_params;
+
 /* ---- entry points --------------------------------------------------------------- */
 
 /* Forward: O = dropout(softmax(scale * Q K^T + mask)) V, plus the row logsumexp.
@@ -196,6 +233,11 @@ int fmha_sm100_bwd_workspace_bytes(const fmha_bwd_params* p, size_t* bytes);
    Inputs, outputs, status codes and numerics are those of fmha_sm100_bwd. */
 #define FMHA_STATIC_SCRATCH_BYTES (32u << 20)
 int fmha_sm100_bwd_static_scratch(const fmha_bwd_params* p, void* stream);
+
+/* Causal attention of packed sequences with grouped heads, and its gradients. */
+int fmha_sm100_causal_fwd(const fmha_causal_fwd_params* p, void* stream);
+int fmha_sm100_causal_bwd(const fmha_causal_bwd_params* p, void* stream);
+int fmha_sm100_causal_bwd_workspace_bytes(const fmha_causal_bwd_params* p, size_t* bytes);
 
 /* 7-bit dropout threshold T for a drop probability: T = round(128 p) clamped to [0,127]. */
 int32_t fmha_sm100_dropout_threshold(float p_drop);

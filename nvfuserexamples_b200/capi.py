@@ -36,6 +36,7 @@ EXPORTS = [
     "fmha_sm100_philox_mask_host", "fmha_sm100_philox_mask_device", "fmha_sm100_check_status",
     "fmha_sm100_strerror", "fmha_sm100_last_cuda_error", "fmha_sm100_abi_version",
     "fmha_sm100_selftest_wait_timeout", "fmha_sm100_bwd_static_scratch",
+    "fmha_sm100_causal_fwd", "fmha_sm100_causal_bwd", "fmha_sm100_causal_bwd_workspace_bytes",
 ]
 
 
@@ -80,6 +81,31 @@ class BwdParams(C.Structure):
     ]
 
 
+class CausalFwdParams(C.Structure):
+    _fields_ = [
+        ("struct_bytes", C.c_int32), ("dtype", C.c_int32),
+        ("B", C.c_int32), ("H", C.c_int32), ("H_kv", C.c_int32), ("max_seqlen", C.c_int32), ("D", C.c_int32),
+        ("scale", C.c_float),
+        ("q", Tensor4), ("k", Tensor4), ("v", Tensor4), ("o", Tensor4),
+        ("lse", C.c_void_p), ("cu_seqlens", C.c_void_p), ("total_rows", C.c_int32),
+        ("flags", C.c_int32), ("status", C.c_void_p),
+    ]
+
+
+class CausalBwdParams(C.Structure):
+    _fields_ = [
+        ("struct_bytes", C.c_int32), ("dtype", C.c_int32),
+        ("B", C.c_int32), ("H", C.c_int32), ("H_kv", C.c_int32), ("max_seqlen", C.c_int32), ("D", C.c_int32),
+        ("scale", C.c_float),
+        ("q", Tensor4), ("k", Tensor4), ("v", Tensor4), ("o", Tensor4), ("d_o", Tensor4),
+        ("lse", C.c_void_p),
+        ("dq", Tensor4), ("dk", Tensor4), ("dv", Tensor4),
+        ("cu_seqlens", C.c_void_p), ("total_rows", C.c_int32),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+        ("flags", C.c_int32), ("status", C.c_void_p),
+    ]
+
+
 class FmhaError(RuntimeError):
     def __init__(self, code: int, what: str, detail: str = ""):
         self.code = code
@@ -107,6 +133,12 @@ def load() -> C.CDLL:
     lib.fmha_sm100_bwd_static_scratch.restype = C.c_int
     lib.fmha_sm100_bwd_workspace_bytes.argtypes = [C.POINTER(BwdParams), C.POINTER(C.c_size_t)]
     lib.fmha_sm100_bwd_workspace_bytes.restype = C.c_int
+    lib.fmha_sm100_causal_fwd.argtypes = [C.POINTER(CausalFwdParams), C.c_void_p]
+    lib.fmha_sm100_causal_fwd.restype = C.c_int
+    lib.fmha_sm100_causal_bwd.argtypes = [C.POINTER(CausalBwdParams), C.c_void_p]
+    lib.fmha_sm100_causal_bwd.restype = C.c_int
+    lib.fmha_sm100_causal_bwd_workspace_bytes.argtypes = [C.POINTER(CausalBwdParams), C.POINTER(C.c_size_t)]
+    lib.fmha_sm100_causal_bwd_workspace_bytes.restype = C.c_int
     lib.fmha_sm100_dropout_threshold.argtypes = [C.c_float]
     lib.fmha_sm100_dropout_threshold.restype = C.c_int32
     lib.fmha_sm100_philox_mask_host.argtypes = [C.c_uint64, C.c_uint64, C.c_int32, C.c_int32, C.c_int32, C.c_int32,

@@ -90,7 +90,9 @@ struct DqItem {
 
 }  // namespace
 
-template <bool BF16, bool KEYADD, bool DROP, bool PACKED>
+// CAUSAL: a packed batch whose rows see the keys up to their own position, with a.kv_group query heads to a key head.  An item's key tiles end
+// at its diagonal; the grid counts heads, sequences and, longest first, query tiles.
+template <bool BF16, bool KEYADD, bool DROP, bool PACKED, bool CAUSAL>
 __global__ void __launch_bounds__(kDqThreads, 1) fmha_bwd_dq_kernel(const __grid_constant__ BwdArgs a) {
   griddep_wait();
   using L = DqSmem;
@@ -143,8 +145,15 @@ __global__ void __launch_bounds__(kDqThreads, 1) fmha_bwd_dq_kernel(const __grid
   constexpr bool packed = PACKED;
   const bool persist = a.persist != 0;   // the grid is larger than the number of SMs
 
+  static_assert(!CAUSAL || (PACKED && !KEYADD && !DROP), "causal: packed batches without dropout");
   auto decode = [&](int x, int y, int z) {
     DqItem it;
+    if constexpr (CAUSAL) {
+      const int heads_at = x;
+      x = gridDim.z - 1 - z;
+      z = y;
+      y = heads_at;
+    }
     it.h = y;
     it.b = z;
     it.bh = z * a.H + y;
@@ -162,7 +171,7 @@ __global__ void __launch_bounds__(kDqThreads, 1) fmha_bwd_dq_kernel(const __grid
       it.k_limit = it.q_limit = packed_rows(it.row_base, cu[z + 1], a.S_q, a.total_rows);
       it.tb = 0;
     }
-    it.n_kv = (it.k_limit + kTileN - 1) / kTileN;
+    it.n_kv = ((CAUSAL ? min(it.k_limit, it.q0 + kTileM) : it.k_limit) + kTileN - 1) / kTileN;
     it.state = it.q0 < it.q_limit ? kDqWork : kDqEmpty;
     return it;
   };
@@ -258,6 +267,7 @@ __global__ void __launch_bounds__(kDqThreads, 1) fmha_bwd_dq_kernel(const __grid
     // ============================ TMA producer ======================================
     int n = 0, w = 0, g = 0;   // item number, items with work and key tiles so far
     for (DqItem it = first_work(n, true); it.state == kDqWork; it = next_work(n, true), ++w) {
+      const int hk = CAUSAL ? it.h / a.kv_group : it.h;
       for (int j = 0; j < it.n_kv; ++j, ++g) {
         const int s = g % KS;
         if (lane == 0) {
@@ -269,7 +279,7 @@ __global__ void __launch_bounds__(kDqThreads, 1) fmha_bwd_dq_kernel(const __grid
           if (g >= KS) mbar_wait(k_empty + s, (g / KS - 1) & 1, wctx, kDqsKEmpty);
           mbar_arrive_expect_tx(k_full + s, L::kTile);
           for (int c = 0; c < 2; ++c)
-            tma_load_4d(sK + s * L::kTile + c * 16384, &a.tm_k, k_full + s, c * 64, it.row_base + j * kTileN, it.h, it.tb);
+            tma_load_4d(sK + s * L::kTile + c * 16384, &a.tm_k, k_full + s, c * 64, it.row_base + j * kTileN, hk, it.tb);
           if (j == 0) {
             if (w > 0) mbar_wait(do_empty, (w - 1) & 1, wctx, kDqsDoEmpty);
             mbar_arrive_expect_tx(do_full, L::kTile);
@@ -277,7 +287,7 @@ __global__ void __launch_bounds__(kDqThreads, 1) fmha_bwd_dq_kernel(const __grid
           }
           if (g >= 1) mbar_wait(v_empty, (g - 1) & 1, wctx, kDqsVEmpty);
           mbar_arrive_expect_tx(v_full, L::kTile);
-          for (int c = 0; c < 2; ++c) tma_load_4d(sV + c * 16384, &a.tm_v, v_full, c * 64, it.row_base + j * kTileN, it.h, it.tb);
+          for (int c = 0; c < 2; ++c) tma_load_4d(sV + c * 16384, &a.tm_v, v_full, c * 64, it.row_base + j * kTileN, hk, it.tb);
           // Early, for the statistics warps need the next item's rows in time; but the first time not at once: on a chip
           // that is still filling up, the CTA asked for may be about to start on an idle SM.
           if (persist && j == (w == 0 ? min(2, it.n_kv - 1) : 0)) request_item(n + 1);
@@ -327,16 +337,23 @@ __global__ void __launch_bounds__(kDqThreads, 1) fmha_bwd_dq_kernel(const __grid
       }
     };
     // S and dP of key tile number t of this CTA; `first` of its item number w (with work)
-    auto issue_s = [&](int t, int w, bool first) {
+    // (`keys`: how many of its keys exist, where that is known; the rows of K and V behind the last are zeroed)
+    auto issue_s = [&](int t, int w, bool first, [[maybe_unused]] int keys) {
       if (first) copy_a(tQ, sQ, q_full, q_empty, w, kDqsQ);
       mbar_wait(k_full + t % KS, (t / KS) & 1, wctx, kDqsK);
+      if constexpr (CAUSAL) {
+        if (keys < kTileN) zero_tile_rows<2>(sK + (t % KS) * L::kTile, keys, kTileN, 16384);
+      }
       tc_fence_after_sync();
       issue_kk(tS, tQ, sK + (t % KS) * L::kTile);
       umma_commit_elect(s_full);
     };
-    auto issue_dp = [&](int t, int w, bool first) {
+    auto issue_dp = [&](int t, int w, bool first, [[maybe_unused]] int keys) {
       if (first) copy_a(tdO, sdO, do_full, do_empty, w, kDqsDo);
       mbar_wait(v_full, t & 1, wctx, kDqsV);
+      if constexpr (CAUSAL) {
+        if (keys < kTileN) zero_tile_rows<2>(sV, keys, kTileN, 16384);
+      }
       tc_fence_after_sync();
       issue_kk(tdP, tdO, sV);
       umma_commit_elect(dp_full);
@@ -345,8 +362,8 @@ __global__ void __launch_bounds__(kDqThreads, 1) fmha_bwd_dq_kernel(const __grid
     int n = 0, w = 0, t = 0;
     DqItem it = first_work(n, false);
     if (it.state == kDqWork) {
-      issue_s(0, 0, true);
-      issue_dp(0, 0, true);
+      issue_s(0, 0, true, it.k_limit);
+      issue_dp(0, 0, true, it.k_limit);
     }
     while (it.state == kDqWork) {
       DqItem nxt = it;
@@ -354,9 +371,10 @@ __global__ void __launch_bounds__(kDqThreads, 1) fmha_bwd_dq_kernel(const __grid
         const bool last = j + 1 == it.n_kv;
         if (last) nxt = next_work(n, false);
         const bool more = !last || nxt.state == kDqWork;
+        const int keys = last ? nxt.k_limit : it.k_limit - (j + 1) * kTileN;   // of tile t + 1, from its first on
         if (more) {
           mbar_wait(s_free, t & 1, wctx, kDqsSFree);
-          issue_s(t + 1, w + 1, last);
+          issue_s(t + 1, w + 1, last, keys);
         }
         mbar_wait(ds_full, t & 1, wctx, kDqsDs);
         tc_fence_after_sync();
@@ -370,7 +388,7 @@ __global__ void __launch_bounds__(kDqThreads, 1) fmha_bwd_dq_kernel(const __grid
         }
         umma_commit_elect(k_empty + t % KS);
         if (last) umma_commit_elect(dq_full);
-        if (more) issue_dp(t + 1, w + 1, last);
+        if (more) issue_dp(t + 1, w + 1, last, keys);
       }
       ++w;
       it = nxt;
@@ -386,6 +404,7 @@ __global__ void __launch_bounds__(kDqThreads, 1) fmha_bwd_dq_kernel(const __grid
       if (x.bh == 0 && x.q0 == 0 && half == 0 && lane == 0) *a.work_counter = 0;   // the dK / dV kernel draws its items from it
       if (packed && a.zero.grad[0].ptr != nullptr && (x.q0 + kTileM > x.q_limit || x.q_limit == a.S_q)) {
         for (int k = 0; k < 3; ++k)
+          if (!CAUSAL || k == 0 || x.h < a.H_kv)   // dk and dv have fewer heads
           zero_uncovered_rows(a.zero.grad[k].ptr, a.zero.grad[k].stride_s, a.zero.grad[k].stride_h, x.h, x.b, a.B,
                               reinterpret_cast<const int*>(a.mask), a.S_q, a.total_rows, D, x.q0, x.q0 + kTileM,
                               a.zero.mode == kUncoveredAll, half * 32 + lane, 64);
@@ -560,7 +579,8 @@ __global__ void __launch_bounds__(kDqThreads, 1) fmha_bwd_dq_kernel(const __grid
       __syncwarp();
       if (lane == 0) mbar_arrive(stat_empty + (w & 1));
       for (int j = 0; j < it.n_kv; ++j, ++t) {
-        const int n_cols = min(32, it.k_limit - j * kTileN - cq * 32);   // valid keys among this thread's 32
+        // valid keys among this thread's 32
+        const int n_cols = min(32, (CAUSAL ? min(it.k_limit, it.q0 + row + 1) : it.k_limit) - j * kTileN - cq * 32);
         [[maybe_unused]] uint32_t kw[8];
         if constexpr (DROP) {
           const uint32_t poff = *philox_off;
@@ -678,9 +698,9 @@ __global__ void __launch_bounds__(256) bwd_delta_kernel(const __grid_constant__ 
   }
 }
 
-template <bool BF16, bool KEYADD, bool DROP, bool PACKED>
+template <bool BF16, bool KEYADD, bool DROP, bool PACKED, bool CAUSAL = false>
 static int launch_dq_impl(const BwdArgs& a, cudaStream_t stream) {
-  auto kfn = fmha_bwd_dq_kernel<BF16, KEYADD, DROP, PACKED>;
+  auto kfn = fmha_bwd_dq_kernel<BF16, KEYADD, DROP, PACKED, CAUSAL>;
   static std::atomic<bool> configured[64] = {};   // per device; set after the attribute call succeeded
   int dev = 0;
   cudaGetDevice(&dev);
@@ -689,7 +709,8 @@ static int launch_dq_impl(const BwdArgs& a, cudaStream_t stream) {
     if (e != cudaSuccess) return static_cast<int>(e);
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
-  const dim3 grid((a.S_q + kTileM - 1) / kTileM, a.H, a.B);
+  const unsigned tiles = (a.S_q + kTileM - 1) / kTileM;
+  const dim3 grid = CAUSAL ? dim3(a.H, a.B, tiles) : dim3(tiles, a.H, a.B);
   BwdArgs args = a;
   // The two statistics warps need 12 000 cycles for an item's delta, five key tiles' worth: with fewer tiles the compute
   // warps wait (9 600 cycles per item at four), and a separate pass over O and dO is the cheaper way (B=16 H=16 S=512 with
@@ -712,6 +733,7 @@ int launch_bwd_dq(const BwdArgs& a, int dtype, cudaStream_t stream) {
   const bool keyadd = a.mask_kind == FMHA_MASK_KEY_ADDITIVE;
   const bool drop = a.dropout_kind == FMHA_DROPOUT_PHILOX;
   const bool packed = a.mask_kind == FMHA_MASK_CU_SEQLENS;
+  if (a.kv_group > 0) return bf ? launch_dq_impl<true, false, false, true, true>(a, stream) : launch_dq_impl<false, false, false, true, true>(a, stream);
 #define FMHA_DQ_CASE(BF, KA, DR, PK) \
   if (bf == BF && keyadd == KA && drop == DR && packed == PK) return launch_dq_impl<BF, KA, DR, PK>(a, stream);
 #define FMHA_DQ_CASES(BF, DR) FMHA_DQ_CASE(BF, false, DR, false) FMHA_DQ_CASE(BF, true, DR, false) FMHA_DQ_CASE(BF, false, DR, true)

@@ -182,6 +182,7 @@ __global__ void __launch_bounds__(256, PACKED ? 4 : 8) bwd_prepare_kernel(const 
     q_limit = packed_rows(base, cu[b + 1], m.S_q, m.total_rows);
     if (m.zero.grad[0].ptr != nullptr && (r0 + 32 * R > q_limit || len > q_limit)) {
       for (int t = 0; t < 3; ++t)
+        if (t == 0 || m.kv_group == 0 || h < m.H_kv)   // causal: dk and dv may have fewer heads
         zero_uncovered_rows(m.zero.grad[t].ptr, m.zero.grad[t].stride_s, m.zero.grad[t].stride_h, h, b, m.B, cu, m.S_q, m.total_rows, D,
                             r0, r0 + 32 * R, m.zero.mode == kUncoveredAll, threadIdx.x, blockDim.x);
     }
@@ -312,7 +313,11 @@ struct BwdItem {
 // counter.  A packed batch has the pass before it, to zero rows.  The accumulator, its clearing and conversion and the launches around
 // this one took 14 to 30 % of the time (whole backward, without / with dropout: B=2 H=4 S=128 10.6 -> 7.8 / 10.9 -> 8.4 us, B=13 H=12 S=100 15.1 -> 11.2 /
 // 16.6 -> 13.0, B=32 H=16 S=128 27.8 -> 19.5 / 29.1 -> 23.0, B=128 H=16 94.4 -> 68.3 / 97.8 -> 75.7; packed, B=32 H=16 of 64 to 128 rows 34.2 -> 27.7 / 36.1 -> 31.2).
-template <int D, bool BF16, bool KEYADD, bool DROP, bool PACKED = false, bool ONE_KV = false>
+// CAUSAL: a packed batch whose rows see the keys up to their own position, with a.kv_group query heads to a key head.  An item is a key tile of
+// a KEY head: its query tiles are those from the diagonal on of every query head of the group, one head after the other, so dK and dV are summed
+// over the group in tensor memory, always in the same order.  Items count heads and sequences first and key tiles, longest first, last.
+// Rows of Q, dO and K behind the end of the sequence are zeroed in shared memory: they are contracted over.
+template <int D, bool BF16, bool KEYADD, bool DROP, bool PACKED = false, bool ONE_KV = false, bool CAUSAL = false>
 __global__ void __launch_bounds__(kBwdThreads, 1) fmha_bwd_kernel(const __grid_constant__ BwdArgs a) {
   griddep_wait();
   using L = BwdSmem<D>;
@@ -369,7 +374,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1) fmha_bwd_kernel(const __grid_c
   const int lane = threadIdx.x & 31;
   const int kv_tiles = (a.S_k + kTileN - 1) / kTileN;
   const int n_q_all = (a.S_q + kTileM - 1) / kTileM;
-  const int num_items = kv_tiles * a.H * a.B;
+  static_assert(!CAUSAL || (PACKED && !KEYADD && !DROP && !ONE_KV), "causal: packed batches without dropout");
+  const int num_items = kv_tiles * (CAUSAL ? a.H_kv : a.H) * a.B;
   constexpr bool packed = PACKED;
 
   if (threadIdx.x == 0) {
@@ -431,10 +437,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1) fmha_bwd_kernel(const __grid_c
     it.q_limit = a.S_q;
     it.row_base = 0;
     if (id >= 0) {
-      const int kv_tile = id % kv_tiles;
-      const int bh = id / kv_tiles;
-      it.h = bh % a.H;
-      it.b = bh / a.H;
+      const int heads = CAUSAL ? a.H_kv : a.H;
+      const int kv_tile = CAUSAL ? id / (heads * a.B) : id % kv_tiles;
+      const int bh = CAUSAL ? id % (heads * a.B) : id / kv_tiles;
+      it.h = bh % heads;   // CAUSAL: the key head
+      it.b = bh / heads;
       it.k0 = kv_tile * kTileN;
       int k_limit = a.S_k;
       if (!packed && a.mask_kind == FMHA_MASK_SEQLEN) {
@@ -449,8 +456,20 @@ __global__ void __launch_bounds__(kBwdThreads, 1) fmha_bwd_kernel(const __grid_c
         it.n_q = (it.q_limit + kTileM - 1) / kTileM;
       }
       it.n_cols = min(kTileN, k_limit - it.k0);
+      if constexpr (CAUSAL) it.n_q = (it.n_q - kv_tile) * a.kv_group;
     }
     return it;
+  };
+  // Query tile and head of an item's i-th tile: i itself and the item's head, or, CAUSAL, from the diagonal on, head after head of the group.
+  struct QTile {
+    int tile, h;
+  };
+  auto first_q = [&](const BwdItem& it) { return CAUSAL ? QTile{it.k0 / kTileN, it.h * a.kv_group} : QTile{0, it.h}; };
+  auto next_q = [&](const BwdItem& it, QTile& x) {
+    ++x.tile;
+    if constexpr (CAUSAL) {
+      if (x.tile * kTileM >= it.q_limit) x = {it.k0 / kTileN, x.h + 1};
+    }
   };
   const uint32_t ring = smem_u32(smem + L::kOffRing);
   // Consumer side of the work-item ring (whole warp): item number `n` of this CTA.
@@ -498,13 +517,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1) fmha_bwd_kernel(const __grid_c
 #pragma unroll
         for (int c = 0; c < D / 64; ++c)
           tma_load_4d(sK + kvb * L::kTileBytes + c * 16384, &a.tm_k, k_full + kvb, c * 64, it.row_base + it.k0, it.h, tb);
-        for (int i = 0; i < it.n_q; ++i, ++g) {
+        QTile q = first_q(it);
+        for (int i = 0; i < it.n_q; ++i, ++g, next_q(it, q)) {
           const int qs = g % QS, os = g % OS;
           if (g >= QS) mbar_wait(q_empty + qs, ((g / QS) - 1) & 1, wctx, kSiteQEmpty);
           mbar_arrive_expect_tx(q_full + qs, L::kTileBytes);
 #pragma unroll
           for (int c = 0; c < D / 64; ++c)
-            tma_load_4d(sQ + qs * L::kTileBytes + c * 16384, &a.tm_q, q_full + qs, c * 64, it.row_base + i * kTileM, it.h, tb);
+            tma_load_4d(sQ + qs * L::kTileBytes + c * 16384, &a.tm_q, q_full + qs, c * 64, it.row_base + q.tile * kTileM, q.h, tb);
           if (i == 0) {   // V after the first Q: with one K/V buffer it comes free after K
             if (w >= KV) mbar_wait(v_empty + kvb, kvp, wctx, kSiteVEmpty);
             mbar_arrive_expect_tx(v_full + kvb, L::kTileBytes);
@@ -516,7 +536,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) fmha_bwd_kernel(const __grid_c
           mbar_arrive_expect_tx(do_full + os, L::kTileBytes);
 #pragma unroll
           for (int c = 0; c < D / 64; ++c)
-            tma_load_4d(sdO + os * L::kTileBytes + c * 16384, &a.tm_do, do_full + os, c * 64, it.row_base + i * kTileM, it.h, tb);
+            tma_load_4d(sdO + os * L::kTileBytes + c * 16384, &a.tm_do, do_full + os, c * 64, it.row_base + q.tile * kTileM, q.h, tb);
         }
         ++w;
       }
@@ -559,19 +579,28 @@ __global__ void __launch_bounds__(kBwdThreads, 1) fmha_bwd_kernel(const __grid_c
       umma_ts_x4(d, a_tmem, 8u, y, kIdescS, 0u);
     };
     // S^T and dP^T of tile tt, which belongs to item number wi (with work) and is its first / last one
-    auto issue_s = [&](int tt, int wi, bool first, bool last) {
+    // (`x`: tile tt's item and place, from which the CAUSAL variant knows which rows do not exist)
+    [[maybe_unused]] auto zero_q_rows = [&](uint8_t* tile, const BwdItem& it, const QTile& x) {
+      const int rows = it.q_limit - x.tile * kTileM;
+      if (rows < kTileM) zero_tile_rows<D / 64>(tile, rows, kTileM, 16384);
+    };
+    auto issue_s = [&](int tt, int wi, bool first, bool last, [[maybe_unused]] const BwdItem& it, [[maybe_unused]] const QTile& x) {
       if (first) {
         mbar_wait(k_full + wi % KV, (wi / KV) & 1, wctx, kSiteKFull);
+        if constexpr (CAUSAL) {
+          if (it.n_cols < kTileN) zero_tile_rows<D / 64>(sK + (wi % KV) * L::kTileBytes, it.n_cols, kTileN, 16384);
+        }
         if constexpr (D == 64) copy_a(tmem_base + kColK, sK + (wi % KV) * L::kTileBytes);
       }
       if (first) mbar_wait(q_full + tt % QS, (tt / QS) & 1, wctx, kSiteQFull);   // else waited for already
+      if constexpr (CAUSAL) zero_q_rows(sQ + (tt % QS) * L::kTileBytes, it, x);
       tc_fence_after_sync();
       if constexpr (D == 64) issue_tk(tS, tmem_base + kColK, sQ + (tt % QS) * L::kTileBytes);
       else issue_kk(tS, sK + (wi % KV) * L::kTileBytes, sQ + (tt % QS) * L::kTileBytes);
       umma_commit_elect(s_full);
       if (D == 128 && last) umma_commit_elect(k_empty + wi % KV);
     };
-    auto issue_dp = [&](int tt, int wi, bool first, bool last) {
+    auto issue_dp = [&](int tt, int wi, bool first, bool last, [[maybe_unused]] const BwdItem& it, [[maybe_unused]] const QTile& x) {
       if (first) {
         mbar_wait(v_full + wi % KV, (wi / KV) & 1, wctx, kSiteVFull);
         if constexpr (D == 64) {
@@ -580,6 +609,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) fmha_bwd_kernel(const __grid_c
         }
       }
       if (first) mbar_wait(do_full + tt % OS, (tt / OS) & 1, wctx, kSiteDoFull);
+      if constexpr (CAUSAL) zero_q_rows(sdO + (tt % OS) * L::kTileBytes, it, x);
       tc_fence_after_sync();
       if constexpr (D == 64) issue_tk(tdP, tmem_base + kColV, sdO + (tt % OS) * L::kTileBytes);
       else issue_kk(tdP, sV + (wi % KV) * L::kTileBytes, sdO + (tt % OS) * L::kTileBytes);
@@ -595,15 +625,17 @@ __global__ void __launch_bounds__(kBwdThreads, 1) fmha_bwd_kernel(const __grid_c
     };
     BwdItem cur = next_work();
     if (cur.id >= 0) {
-      issue_s(0, 0, true, cur.n_q == 1);
-      issue_dp(0, 0, true, cur.n_q == 1);
+      issue_s(0, 0, true, cur.n_q == 1, cur, first_q(cur));
+      issue_dp(0, 0, true, cur.n_q == 1, cur, first_q(cur));
     }
     while (cur.id >= 0) {
       const int kvb = w % KV;
       const int n_q = cur.n_q;
       BwdItem nxt = cur;
+      QTile qn = first_q(cur);   // of tile t + 1
       for (int i = 0; i < n_q; ++i, ++t) {
         const bool last = i + 1 == n_q;
+        next_q(cur, qn);
         const int qs = t % QS, os = t % OS;
         const uint32_t acc0 = (i > 0) ? 1u : 0u;
         // (the next tile's Q and, below, dO are usually there: polled here, the answer does not hold up S and dP)
@@ -628,7 +660,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1) fmha_bwd_kernel(const __grid_c
         const bool more = !last || nxt.id >= 0;
         const int wn = last ? w + 1 : w;                                  // item of tile t+1, and whether t+1 is its last tile
         const bool next_last = last ? nxt.n_q == 1 : i + 2 == n_q;
-        if (more) issue_s(t + 1, wn, last, next_last);
+        if (last) qn = first_q(nxt);
+        if (more) issue_s(t + 1, wn, last, next_last, last ? nxt : cur, qn);
         // ---- dK += dS^T Q (A from tensor memory), dP of the next tile over dS(t), dQ tile = dS K ------------------------------
         const uint64_t dQ_m = make_smem_desc_sw128(smem_u32(sQ + qs * L::kTileBytes), 16384, 1024);
         if (!last) mbar_wait(do_full + (t + 1) % OS, ((t + 1) / OS) & 1, wctx, kSiteDoFull);
@@ -646,7 +679,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) fmha_bwd_kernel(const __grid_c
         }
         umma_commit_elect(q_empty + qs);
         if (last) umma_commit_elect(acc_full);
-        if (more) issue_dp(t + 1, wn, last, next_last);
+        if (more) issue_dp(t + 1, wn, last, next_last, last ? nxt : cur, qn);
         if constexpr (D == 64) {
           const uint64_t ddS_m = make_smem_desc_sw128(smem_u32(sdS + (t % DS) * L::kDsBytes), 16384, 1024);   // MN-major A (queries x keys)
           const uint64_t dK_m = make_smem_desc_sw128(smem_u32(sK + kvb * L::kTileBytes), 16384, 1024);        // MN-major B
@@ -678,13 +711,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1) fmha_bwd_kernel(const __grid_c
       if (cur.id < 0) break;
       if (cur.n_cols <= 0) continue;
       // logsumexp rows: [B*H, S_q], or [H, total_rows] for a packed batch; delta is always [B*H, S_q]
-      const float* lse = a.lse + (packed ? static_cast<int64_t>(cur.h) * a.total_rows + cur.row_base : static_cast<int64_t>(cur.b * a.H + cur.h) * a.S_q);
-      const float* delta = a.delta + static_cast<int64_t>(cur.b * a.H + cur.h) * a.S_q;
+      QTile q = first_q(cur);
+      const float* lse = a.lse + (packed ? static_cast<int64_t>(q.h) * a.total_rows + cur.row_base : static_cast<int64_t>(cur.b * a.H + q.h) * a.S_q);
+      const float* delta = a.delta + static_cast<int64_t>(cur.b * a.H + q.h) * a.S_q;
       for (int i = 0; i < cur.n_q; ++i, ++t) {
         float x[4], d[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const int r = i * kTileM + k * 32 + lane;
+          const int r = q.tile * kTileM + k * 32 + lane;
           x[k] = INFINITY;   // rows past the end: their probabilities are zero
           d[k] = 0.f;
           if (r < cur.q_limit) {
@@ -702,6 +736,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1) fmha_bwd_kernel(const __grid_c
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(stat_full + slot);
+        const int h = q.h;
+        next_q(cur, q);
+        if (CAUSAL && q.h != h) {
+          lse += a.total_rows;
+          delta += a.S_q;
+        }
       }
     }
   } else {
@@ -854,7 +894,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1) fmha_bwd_kernel(const __grid_c
         if (c < a.S_k) key_add = reinterpret_cast<const float*>(a.mask)[static_cast<size_t>(cur.b) * a.S_k + c] * kLog2eB;
       }
 
-      for (int i = 0; i < n_q; ++i, ++t) {
+      QTile q = first_q(cur);
+      for (int i = 0; i < n_q; ++i, ++t, next_q(cur, q)) {
         // ONE_KV: O and dO for delta of rows [8 cw, +8) of the tile, eight lanes a row, four rows an instruction.  (Its place among the
         // statistics is free: every warp has passed the barriers of the tile before.)
         [[maybe_unused]] uint4 wo[2], wd[2];
@@ -899,6 +940,13 @@ __global__ void __launch_bounds__(kBwdThreads, 1) fmha_bwd_kernel(const __grid_c
         uint32_t p[32];
         tmem_ld32(tmem_base + lane_addr + kColS + cq * 32, p);
         tmem_wait_ld_dep(p);
+        if constexpr (CAUSAL) {   // on the diagonal a key is seen by the queries from its own position on
+          if (q.tile * kTileM == cur.k0) {
+#pragma unroll
+            for (int k = 0; k < 32; ++k)
+              if (cq * 32 + k < row) p[k] = __float_as_uint(-INFINITY);
+          }
+        }
         const float2 sl22 = make_float2(sl2, sl2);
         const float2 add2 = make_float2(key_add, key_add);
         uint32_t pk[16];
@@ -983,7 +1031,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) fmha_bwd_kernel(const __grid_c
         if constexpr (D == 64) {
           if (!dq_out) dq_readout(t - 1, prev_tile);
           dq_out = false;
-          prev_tile = ONE_KV ? 2 * i + (w & 1) : bh * n_q_all + i;
+          prev_tile = ONE_KV ? 2 * i + (w & 1) : CAUSAL ? (cur.b * a.H + q.h) * n_q_all + q.tile : bh * n_q_all + i;
         }
       }
       pending = true;
@@ -1023,10 +1071,10 @@ bool bwd_one_kv(int D, int64_t heads, int S_q, int S_k) {
   return D == 64 && S_k <= kTileN && (S_q <= 3 * kTileM || heads >= 12 * ((S_q + kTileM - 1) / kTileM));
 }
 
-template <int D, bool BF16, bool KEYADD, bool DROP, bool PACKED = false, bool ONE_KV = false>
+template <int D, bool BF16, bool KEYADD, bool DROP, bool PACKED = false, bool ONE_KV = false, bool CAUSAL = false>
 static int launch_bwd_impl(const BwdArgs& a, cudaStream_t stream) {
   using L = BwdSmem<D>;
-  auto kfn = fmha_bwd_kernel<D, BF16, KEYADD, DROP, PACKED, ONE_KV>;
+  auto kfn = fmha_bwd_kernel<D, BF16, KEYADD, DROP, PACKED, ONE_KV, CAUSAL>;
   static std::atomic<bool> configured[64] = {};   // per device; set after the attribute call succeeded
   int dev = 0;
   cudaGetDevice(&dev);
@@ -1035,7 +1083,7 @@ static int launch_bwd_impl(const BwdArgs& a, cudaStream_t stream) {
     if (e != cudaSuccess) return static_cast<int>(e);
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
-  const int64_t items = static_cast<int64_t>((a.S_k + kTileN - 1) / kTileN) * a.H * a.B;
+  const int64_t items = static_cast<int64_t>((a.S_k + kTileN - 1) / kTileN) * (CAUSAL ? a.H_kv : a.H) * a.B;
   const int grid = static_cast<int>(std::min<int64_t>(items, sm_count()));   // one persistent CTA per SM
   const cudaError_t e = launch_overlapped(kfn, dim3(grid), dim3(kBwdThreads), L::kDynBytes, stream, a);
   return static_cast<int>(e != cudaSuccess ? e : cudaGetLastError());
@@ -1045,6 +1093,10 @@ int launch_bwd(const BwdArgs& a, int D, int dtype, cudaStream_t stream) {
   const bool bf = dtype == FMHA_DTYPE_BF16;
   const bool keyadd = a.mask_kind == FMHA_MASK_KEY_ADDITIVE;
   const bool drop = a.dropout_kind == FMHA_DROPOUT_PHILOX;
+  if (a.kv_group > 0) {
+    if (D == 64) return bf ? launch_bwd_impl<64, true, false, false, true, false, true>(a, stream) : launch_bwd_impl<64, false, false, false, true, false, true>(a, stream);
+    return bf ? launch_bwd_impl<128, true, false, false, true, false, true>(a, stream) : launch_bwd_impl<128, false, false, false, true, false, true>(a, stream);
+  }
   const bool one_kv = bwd_one_kv(D, static_cast<int64_t>(a.B) * a.H, a.S_q, a.S_k);
   if (a.mask_kind == FMHA_MASK_CU_SEQLENS) {
 #define FMHA_BWD_ONE_PACKED(BF, DR) \

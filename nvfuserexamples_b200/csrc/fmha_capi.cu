@@ -447,6 +447,135 @@ int fmha_sm100_bwd(const fmha_bwd_params* p, void* stream_) {
   return FMHA_OK;
 }
 
+// ---- causal attention of packed sequences, grouped heads ------------------------------------------
+static int validate_causal(int struct_bytes, size_t expect, int dtype, int B, int H, int H_kv, int max_len, int D, float scale, int total_rows) {
+  const int rc = validate_common(struct_bytes, expect, dtype, B, H, max_len, max_len, D, scale);
+  if (rc != FMHA_OK) return rc;
+  if (H_kv < 0 || total_rows < 0 || (H > 0 && (H_kv == 0 || H % H_kv != 0))) return FMHA_ERR_BAD_ARG;
+  // work items and grid axes: heads along x, sequences along y, tiles along z
+  if (static_cast<int64_t>(B) * H * ((max_len + kTileM - 1) / kTileM) > 0x7fffffffll) return FMHA_ERR_TOO_LARGE;
+  return FMHA_OK;
+}
+
+int fmha_sm100_causal_fwd(const fmha_causal_fwd_params* p, void* stream_) {
+  if (p == nullptr) return FMHA_ERR_BAD_ARG;
+  int rc = validate_causal(p->struct_bytes, sizeof(fmha_causal_fwd_params), p->dtype, p->B, p->H, p->H_kv, p->max_seqlen, p->D, p->scale,
+                           p->total_rows);
+  if (rc != FMHA_OK) return rc;
+  if (p->B == 0 || p->H == 0 || p->total_rows == 0) return FMHA_OK;
+  if (p->max_seqlen == 0 || p->cu_seqlens == nullptr) return FMHA_ERR_BAD_ARG;
+  if (!tensor_ok(p->q, 1, p->H) || !tensor_ok(p->k, 1, p->H_kv) || !tensor_ok(p->v, 1, p->H_kv) || !tensor_ok(p->o, 1, p->H))
+    return FMHA_ERR_BAD_ARG;
+  rc = check_device();
+  if (rc != FMHA_OK) return rc;
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  const int rows = p->total_rows;
+  const fmha_tensor4 tq = sanitized(p->q, 1, p->H, rows, p->D), tk = sanitized(p->k, 1, p->H_kv, rows, p->D),
+                     tv = sanitized(p->v, 1, p->H_kv, rows, p->D), to = sanitized(p->o, 1, p->H, rows, p->D);
+  FwdArgs a;
+  std::memset(&a, 0, sizeof(a));
+  const int key_tile = fwd_key_tile(p->D, false);
+  if ((rc = make_tmap(&a.tm_q, tq, p->dtype, 1, p->H, rows, p->D, kTileM))) return rc;
+  if ((rc = make_tmap(&a.tm_k, tk, p->dtype, 1, p->H_kv, rows, p->D, key_tile))) return rc;
+  if ((rc = make_tmap(&a.tm_v, tv, p->dtype, 1, p->H_kv, rows, p->D, key_tile))) return rc;
+  if ((rc = make_tmap(&a.tm_o, to, p->dtype, 1, p->H, rows, p->D, kTileM))) return rc;
+  a.total_rows = rows;
+  a.kv_group = p->H / p->H_kv;
+  if (p->flags & FMHA_FLAG_ZERO_UNCOVERED) {
+    const UncoveredRows u = {{to}, rows, uncovered_mode(p->B, p->max_seqlen, rows)};
+    a.zero_uncovered = u.mode;
+    if (const int e = zero_outside_rows(u, p->B, p->H, p->D, p->cu_seqlens, stream)) return cuda_fail(static_cast<cudaError_t>(e));
+  }
+  a.o_ptr = to.ptr; a.o_ss = to.stride_s; a.o_sh = to.stride_h; a.o_sb = to.stride_b;
+  a.B = p->B; a.H = p->H; a.S_q = a.S_k = p->max_seqlen;
+  a.scale = p->scale;
+  a.scale_log2 = p->scale * 1.4426950408889634f;
+  a.lse = p->lse;
+  a.mask_kind = FMHA_MASK_CU_SEQLENS;
+  a.mask = p->cu_seqlens;
+  a.dropout_scale = 1.0f;
+  a.status = p->status;
+  const int e = launch_fwd_causal(a, p->D, p->dtype, stream);
+  return e != 0 ? cuda_fail(static_cast<cudaError_t>(e)) : FMHA_OK;
+}
+
+int fmha_sm100_causal_bwd_workspace_bytes(const fmha_causal_bwd_params* p, size_t* bytes) {
+  if (p == nullptr || bytes == nullptr) return FMHA_ERR_BAD_ARG;
+  const int rc = validate_causal(p->struct_bytes, sizeof(fmha_causal_bwd_params), p->dtype, p->B, p->H, p->H_kv, p->max_seqlen, p->D, p->scale,
+                                 p->total_rows);
+  if (rc != FMHA_OK) return rc;
+  const size_t bh = static_cast<size_t>(p->B) * p->H, pad = (static_cast<size_t>(p->max_seqlen) + kTileM - 1) / kTileM * kTileM;
+  *bytes = align256(bwd_accum_bytes(bh, pad, p->D)) + align256(bh * p->max_seqlen * sizeof(float)) + 256;
+  return FMHA_OK;
+}
+
+int fmha_sm100_causal_bwd(const fmha_causal_bwd_params* p, void* stream_) {
+  if (p == nullptr) return FMHA_ERR_BAD_ARG;
+  size_t need = 0;
+  int rc = fmha_sm100_causal_bwd_workspace_bytes(p, &need);   // validates the sizes
+  if (rc != FMHA_OK) return rc;
+  if (p->B == 0 || p->H == 0 || p->total_rows == 0) return FMHA_OK;
+  if (p->max_seqlen == 0 || p->cu_seqlens == nullptr || p->lse == nullptr) return FMHA_ERR_BAD_ARG;
+  const int H = p->H, Hk = p->H_kv, rows = p->total_rows, D = p->D;
+  if (!tensor_ok(p->q, 1, H) || !tensor_ok(p->k, 1, Hk) || !tensor_ok(p->v, 1, Hk) || !tensor_ok(p->o, 1, H) || !tensor_ok(p->d_o, 1, H) ||
+      !tensor_ok(p->dq, 1, H) || !tensor_ok(p->dk, 1, Hk) || !tensor_ok(p->dv, 1, Hk))
+    return FMHA_ERR_BAD_ARG;
+  if (p->workspace == nullptr || p->workspace_bytes < need || (reinterpret_cast<uintptr_t>(p->workspace) & 255)) return FMHA_ERR_BAD_ARG;
+  rc = check_device();
+  if (rc != FMHA_OK) return rc;
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  const fmha_tensor4 tq = sanitized(p->q, 1, H, rows, D), tk = sanitized(p->k, 1, Hk, rows, D), tv = sanitized(p->v, 1, Hk, rows, D),
+                     to = sanitized(p->o, 1, H, rows, D), tdo = sanitized(p->d_o, 1, H, rows, D), tdq = sanitized(p->dq, 1, H, rows, D),
+                     tdk = sanitized(p->dk, 1, Hk, rows, D), tdv = sanitized(p->dv, 1, Hk, rows, D);
+  BwdArgs a;
+  std::memset(&a, 0, sizeof(a));
+  if ((rc = make_tmap(&a.tm_q, tq, p->dtype, 1, H, rows, D, kTileM))) return rc;
+  if ((rc = make_tmap(&a.tm_k, tk, p->dtype, 1, Hk, rows, D, kTileN))) return rc;
+  if ((rc = make_tmap(&a.tm_v, tv, p->dtype, 1, Hk, rows, D, kTileN))) return rc;
+  if ((rc = make_tmap(&a.tm_do, tdo, p->dtype, 1, H, rows, D, kTileM))) return rc;
+  if ((rc = make_tmap(&a.tm_dk, tdk, p->dtype, 1, Hk, rows, D, 32, D / 4))) return rc;
+  if ((rc = make_tmap(&a.tm_dv, tdv, p->dtype, 1, Hk, rows, D, 32, D / 4))) return rc;
+  const size_t bh = static_cast<size_t>(p->B) * H;
+  const int pad = (p->max_seqlen + kTileM - 1) / kTileM * kTileM;
+  a.dq_accum = static_cast<float*>(p->workspace);
+  a.delta = reinterpret_cast<float*>(static_cast<uint8_t*>(p->workspace) + align256(bwd_accum_bytes(bh, pad, D)));
+  a.work_counter = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(a.delta) + align256(bh * p->max_seqlen * sizeof(float)));
+  a.total_rows = rows;
+  a.H_kv = Hk;
+  a.kv_group = H / Hk;
+  a.dk_ptr = tdk.ptr; a.dk_ss = tdk.stride_s; a.dk_sh = tdk.stride_h;
+  a.dv_ptr = tdv.ptr; a.dv_ss = tdv.stride_s; a.dv_sh = tdv.stride_h;
+  a.B = p->B; a.H = H; a.S_q = a.S_k = p->max_seqlen;
+  a.S_q_pad = pad;
+  a.scale = p->scale;
+  a.scale_log2 = p->scale * 1.4426950408889634f;
+  a.lse = p->lse;
+  a.mask_kind = FMHA_MASK_CU_SEQLENS;
+  a.mask = p->cu_seqlens;
+  a.dropout_scale = 1.0f;
+  a.status = p->status;
+  if (p->flags & FMHA_FLAG_ZERO_UNCOVERED) {
+    a.zero = {{tdq, tdk, tdv}, rows, uncovered_mode(p->B, p->max_seqlen, rows)};
+    int e0 = zero_outside_rows({{tdq}, rows, a.zero.mode}, p->B, H, D, p->cu_seqlens, stream);
+    if (e0 == 0) e0 = zero_outside_rows({{tdk, tdv}, rows, a.zero.mode}, p->B, Hk, D, p->cu_seqlens, stream);
+    if (e0 != 0) return cuda_fail(static_cast<cudaError_t>(e0));
+  }
+  a.o_ptr = to.ptr; a.o_sb = to.stride_b; a.o_sh = to.stride_h; a.o_ss = to.stride_s;
+  a.do_ptr = tdo.ptr; a.do_sb = tdo.stride_b; a.do_sh = tdo.stride_h; a.do_ss = tdo.stride_s;
+  a.dq_ptr = tdq.ptr; a.dq_ss = tdq.stride_s; a.dq_sh = tdq.stride_h; a.dq_sb = tdq.stride_b;
+  int e;
+  if (D == 128) {
+    if ((rc = make_tmap(&a.tm_dq, tdq, p->dtype, 1, H, rows, D, 32, 16))) return rc;
+    e = launch_bwd_dq(a, p->dtype, stream);
+  } else {
+    e = launch_bwd_prepare(to, tdo, a, p->dtype, stream);
+  }
+  if (e == 0) e = launch_bwd(a, D, p->dtype, stream);
+  if (e == 0 && D == 64)
+    e = launch_bwd_finish(a.dq_accum, tdq, p->B, H, p->max_seqlen, pad, p->dtype, p->scale, p->cu_seqlens, rows, stream);
+  return e != 0 ? cuda_fail(static_cast<cudaError_t>(e)) : FMHA_OK;
+}
+
 int fmha_sm100_check_status(int32_t* status, void* stream, int32_t* host_copy) {
   if (status == nullptr) return FMHA_ERR_BAD_ARG;
   int32_t h[4] = {0, 0, 0, 0};

@@ -89,7 +89,10 @@ struct FastSmem {
 // SPLIT: the keys of a query tile are dealt out over the CTAs of a cluster (see fwd_key_split); each runs its share of
 // the key steps and leaves its unnormalised O, row maximum and row sum in its own shared memory, and the cluster
 // combines them through distributed shared memory.
-template <int D, bool BF16, bool KEYADD, bool DROP, bool PACKED = false, bool SPLIT = false>
+// CAUSAL: a packed batch whose rows see the keys up to their own position, with a.kv_group query heads to a key head.  The grid counts
+// heads, sequences and, longest first, query tiles: with one tile of every head before the next shorter ones the last CTAs to start are short,
+// and the query heads of a key head, which are neighbours, find its keys and values in the L2 cache.
+template <int D, bool BF16, bool KEYADD, bool DROP, bool PACKED = false, bool SPLIT = false, bool CAUSAL = false>
 __global__ void __launch_bounds__(fast_threads<D>(), FastSmem<D, DROP>::kCtasPerSm) fmha_fwd_fast_kernel(const __grid_constant__ FwdArgs a) {
   griddep_wait();
   constexpr bool MERGED = (D == 64);          // one warp issues the loads and the MMAs
@@ -128,10 +131,12 @@ __global__ void __launch_bounds__(fast_threads<D>(), FastSmem<D, DROP>::kCtasPer
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const int h = blockIdx.y;
-  int b = blockIdx.z;
+  static_assert(!CAUSAL || (PACKED && !KEYADD && !DROP && !SPLIT), "causal: packed batches without dropout");
+  const int h = CAUSAL ? blockIdx.x : blockIdx.y;
+  const int hk = CAUSAL ? h / a.kv_group : h;   // head of K and V
+  int b = CAUSAL ? blockIdx.y : blockIdx.z;
   int ordered_len = 0;   // the valid length, where it is known already
-  if constexpr (D == 64 && !KEYADD && !SPLIT) {
+  if constexpr (D == 64 && !KEYADD && !SPLIT && !CAUSAL) {
     if (a.length_class_shift >= 0) {
       const int* len = reinterpret_cast<const int*>(a.mask);
       int n = 0;
@@ -143,7 +148,7 @@ __global__ void __launch_bounds__(fast_threads<D>(), FastSmem<D, DROP>::kCtasPer
   }
   const int n_split = SPLIT ? static_cast<int>(cluster_size()) : 1;
   const int split = SPLIT ? static_cast<int>(cluster_rank()) : 0;
-  const int q0 = (SPLIT ? blockIdx.x / n_split : blockIdx.x) * kTileM;
+  const int q0 = (CAUSAL ? gridDim.z - 1 - blockIdx.z : SPLIT ? blockIdx.x / n_split : blockIdx.x) * kTileM;
   const int bh = b * a.H + h;
 
   int k_limit = a.S_k;
@@ -162,13 +167,14 @@ __global__ void __launch_bounds__(fast_threads<D>(), FastSmem<D, DROP>::kCtasPer
     k_limit = len;
     q_limit = min(len, a.total_rows - row_base);   // offsets past the tensor, which the host cannot see: no row behind it is written
     tb = 0;
-    if (q0 >= len) {   // this sequence has no such query tile (whole CTA, before any barrier)
+    if (q0 >= (CAUSAL ? q_limit : len)) {   // this sequence has no such query tile (whole CTA, before any barrier)
       if (a.zero_uncovered)
         zero_uncovered_rows(a.o_ptr, a.o_ss, a.o_sh, h, b, a.B, cu, a.S_q, a.total_rows, D, q0, q0 + kTileM,
                             a.zero_uncovered == kUncoveredAll, threadIdx.x, blockDim.x);
       return;
     }
     if (threadIdx.x == 0) *uncovered = a.zero_uncovered && (q0 + kTileM > len || all > len);
+    if constexpr (CAUSAL) k_limit = min(q_limit, q0 + kTileM);
   }
   const int n_kv_all = (k_limit + TN - 1) / TN;
   // key steps of this CTA: [j0, j0 + n_kv); with SPLIT possibly none
@@ -201,7 +207,7 @@ __global__ void __launch_bounds__(fast_threads<D>(), FastSmem<D, DROP>::kCtasPer
     if (n_kv > 0) {
       mbar_arrive_expect_tx(k_full, L::kTileBytes);
 #pragma unroll
-      for (int c = 0; c < D / 64; ++c) tma_load_4d(sK + c * L::kSubTile, &a.tm_k, k_full, c * 64, row_base + j0 * TN, h, tb);
+      for (int c = 0; c < D / 64; ++c) tma_load_4d(sK + c * L::kSubTile, &a.tm_k, k_full, c * 64, row_base + j0 * TN, hk, tb);
     }
     tma_prefetch_desc(&a.tm_v);
     tma_prefetch_desc(&a.tm_o);
@@ -226,13 +232,13 @@ __global__ void __launch_bounds__(fast_threads<D>(), FastSmem<D, DROP>::kCtasPer
           mbar_arrive_expect_tx(k_full + s, L::kTileBytes);
 #pragma unroll
           for (int c = 0; c < D / 64; ++c)
-            tma_load_4d(sK + s * L::kTileBytes + c * L::kSubTile, &a.tm_k, k_full + s, c * 64, row_base + (j0 + j) * TN, h, tb);
+            tma_load_4d(sK + s * L::kTileBytes + c * L::kSubTile, &a.tm_k, k_full + s, c * 64, row_base + (j0 + j) * TN, hk, tb);
         }
         if (j >= ST) mbar_wait(v_empty + s, ((j / ST) - 1) & 1, wctx, kFVEmpty);
         mbar_arrive_expect_tx(v_full + s, L::kTileBytes);
 #pragma unroll
         for (int c = 0; c < D / 64; ++c)
-          tma_load_4d(sV + s * L::kTileBytes + c * L::kSubTile, &a.tm_v, v_full + s, c * 64, row_base + (j0 + j) * TN, h, tb);
+          tma_load_4d(sV + s * L::kTileBytes + c * L::kSubTile, &a.tm_v, v_full + s, c * 64, row_base + (j0 + j) * TN, hk, tb);
       }
     }
   } else if (warp == 0 && MERGED) {
@@ -253,12 +259,12 @@ __global__ void __launch_bounds__(fast_threads<D>(), FastSmem<D, DROP>::kCtasPer
       auto load_k = [&](int j) {
         const int s = j % ST;
         mbar_arrive_expect_tx(k_full + s, L::kTileBytes);
-        tma_load_4d(sK + s * L::kTileBytes, &a.tm_k, k_full + s, 0, row_base + (j0 + j) * TN, h, tb);
+        tma_load_4d(sK + s * L::kTileBytes, &a.tm_k, k_full + s, 0, row_base + (j0 + j) * TN, hk, tb);
       };
       auto load_v = [&](int j) {
         const int s = j % ST;
         mbar_arrive_expect_tx(v_full + s, L::kTileBytes);
-        tma_load_4d(sV + s * L::kTileBytes, &a.tm_v, v_full + s, 0, row_base + (j0 + j) * TN, h, tb);
+        tma_load_4d(sV + s * L::kTileBytes, &a.tm_v, v_full + s, 0, row_base + (j0 + j) * TN, hk, tb);
       };
       const uint64_t dq = make_smem_desc_sw128(smem_u32(sQ), 16, 1024);
       uint64_t aq[KQ];
@@ -302,6 +308,9 @@ __global__ void __launch_bounds__(fast_threads<D>(), FastSmem<D, DROP>::kCtasPer
           __syncwarp();
         }
         mbar_wait(v_full + s, (j / ST) & 1, wctx, kFVFull);
+        if constexpr (CAUSAL) {
+          if (!more && n_kv * TN > k_limit) zero_tile_rows<D / 64>(sV + s * L::kTileBytes, k_limit - j * TN, TN, L::kSubTile);
+        }
         if (more) mbar_wait(k_full + (j + 1) % ST, ((j + 1) / ST) & 1, wctx, kFKFull);
         mbar_wait(p_full, j & 1, wctx, kFPFull);
         tc_fence_after_sync();
@@ -350,6 +359,9 @@ __global__ void __launch_bounds__(fast_threads<D>(), FastSmem<D, DROP>::kCtasPer
         const bool more = j + 1 < n_kv;
         // what P V(j) and Q K^T(j+1) need is waited for under the softmax of step j, see the merged version
         mbar_wait(v_full + s, (j / ST) & 1, wctx, kFVFull);
+        if constexpr (CAUSAL) {
+          if (!more && n_kv * TN > k_limit) zero_tile_rows<D / 64>(sV + s * L::kTileBytes, k_limit - j * TN, TN, L::kSubTile);
+        }
         if (more) mbar_wait(k_full + (j + 1) % ST, ((j + 1) / ST) & 1, wctx, kFKFull);
         mbar_wait(p_full, j & 1, wctx, kFPFull);
         tc_fence_after_sync();
@@ -422,7 +434,11 @@ __global__ void __launch_bounds__(fast_threads<D>(), FastSmem<D, DROP>::kCtasPer
       }
       auto wait_s = [&]() { mbar_wait(s_full, j & 1, wctx, kFSFull, 32); };
       auto arrive = [&](int) { arrive_p(); };
-      if constexpr (D == 64)
+      if constexpr (CAUSAL) {
+        const int warp_cols = min(n_cols, q0 + quad * 32 + 32 - col0), own_cols = min(n_cols, q_row + 1 - col0);
+        if constexpr (D == 64) softmax_step_64_causal<BF16>(tS, tO, col0, warp_cols, own_cols, sl2, drop_row, m_ref, sum2, wait_s, arrive);
+        else softmax_step_128_causal<BF16, 0>(tS, tO, col0, warp_cols, own_cols, sl2, drop_row, m_ref, sum2, wait_s, arrive, [] {}, [] {});
+      } else if constexpr (D == 64)
         softmax_step_64<BF16, KEYADD, DROP>(tS, tO, col0, n_cols, sl2, mask_stage, kind, drop_row, m_ref, sum2, wait_s, arrive);
       else
         softmax_step_128<BF16, KEYADD, DROP, 0>(tS, tO, col0, n_cols, sl2, mask_stage, kind, drop_row, m_ref, sum2, wait_s, arrive, [] {}, [] {});
@@ -592,7 +608,7 @@ int fwd_length_class_shift(const FwdArgs& a, int D, int64_t ctas, bool no_length
   return shift;
 }
 
-template <int D, bool BF16, bool KEYADD, bool DROP, bool PACKED = false, bool SPLIT = false>
+template <int D, bool BF16, bool KEYADD, bool DROP, bool PACKED = false, bool SPLIT = false, bool CAUSAL = false>
 static int launch_fast_impl(const FwdArgs& a, cudaStream_t stream, int n_split = 1) {
   using L = FastSmem<D>;
   if constexpr (!PACKED && !SPLIT) {
@@ -600,7 +616,7 @@ static int launch_fast_impl(const FwdArgs& a, cudaStream_t stream, int n_split =
                                 KEYADD || DROP, sm_count());
     if (s > 1) return launch_fast_impl<D, BF16, KEYADD, DROP, false, true>(a, stream, s);
   }
-  auto kfn = fmha_fwd_fast_kernel<D, BF16, KEYADD, DROP, PACKED, SPLIT>;
+  auto kfn = fmha_fwd_fast_kernel<D, BF16, KEYADD, DROP, PACKED, SPLIT, CAUSAL>;
   static std::atomic<bool> configured[64] = {};   // per device; set after the attribute call succeeded
   int dev = 0;
   cudaGetDevice(&dev);
@@ -610,10 +626,18 @@ static int launch_fast_impl(const FwdArgs& a, cudaStream_t stream, int n_split =
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
   dim3 grid((a.S_q + kTileM - 1) / kTileM * n_split, a.H, a.B);
+  if constexpr (CAUSAL) grid = dim3(a.H, a.B, (a.S_q + kTileM - 1) / kTileM);
   FwdArgs args = a;
-  args.length_class_shift = fwd_length_class_shift(a, D, static_cast<int64_t>(grid.x) * grid.y * grid.z, KEYADD || SPLIT);
+  args.length_class_shift = fwd_length_class_shift(a, D, static_cast<int64_t>(grid.x) * grid.y * grid.z, KEYADD || SPLIT || CAUSAL);
   const cudaError_t e = launch_overlapped(kfn, grid, dim3(fast_threads<D>()), L::kDynBytes, stream, args, SPLIT ? n_split : 0);
   return static_cast<int>(e != cudaSuccess ? e : cudaGetLastError());
+}
+
+int launch_fwd_causal(const FwdArgs& a, int D, int dtype, cudaStream_t stream) {
+  if (D == 128 && fwd_pair_causal_pays(sm_count(), a.B, a.H, a.S_q, a.total_rows)) return launch_fwd_pair_causal(a, dtype, stream);
+  const bool bf = dtype == FMHA_DTYPE_BF16;
+  if (D == 64) return bf ? launch_fast_impl<64, true, false, false, true, false, true>(a, stream) : launch_fast_impl<64, false, false, false, true, false, true>(a, stream);
+  return bf ? launch_fast_impl<128, true, false, false, true, false, true>(a, stream) : launch_fast_impl<128, false, false, false, true, false, true>(a, stream);
 }
 
 int launch_fwd_fast(const FwdArgs& a, int D, int dtype, cudaStream_t stream) {

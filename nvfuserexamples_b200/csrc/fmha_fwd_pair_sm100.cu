@@ -116,7 +116,10 @@ __device__ __forceinline__ void o_warp_out(uint32_t tO, float out_scale, uint32_
   }
 }
 
-template <bool BF16, bool KEYADD, bool PACKED>
+// CAUSAL: a packed batch whose rows see the keys up to their own position, with a.kv_group query heads to a key head.  The second tile of a
+// pair has one key step more than the first; in that step nothing takes turns, and the first tile's MMA warp passes its K and V on unread.  The
+// grid counts heads, sequences and, longest first, pairs.
+template <bool BF16, bool KEYADD, bool PACKED, bool CAUSAL>
 __global__ void __launch_bounds__(kPairThreads, 1) fmha_fwd_pair_kernel(const __grid_constant__ FwdArgs a) {
   griddep_wait();
   using L = PairSmem;
@@ -126,6 +129,12 @@ __global__ void __launch_bounds__(kPairThreads, 1) fmha_fwd_pair_kernel(const __
   constexpr int kFmt = BF16 ? 1 : 0;
   constexpr uint32_t kIdescQK = make_idesc_f16(128, TN, kFmt, false, false);
   constexpr uint32_t kIdescPV = make_idesc_f16(128, D, kFmt, false, true);
+
+  static_assert(!CAUSAL || (PACKED && !KEYADD), "causal: packed batches");
+  // Key steps of tile g of an item: in a causal one up to its diagonal.
+  auto steps_of = [](const PairItem& it, int g) {
+    return ((CAUSAL ? min(it.k_limit, it.q0 + (g + 1) * kTileM) : it.k_limit) + TN - 1) / TN;
+  };
 
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t* sQ = smem + L::kOffQ;
@@ -228,7 +237,12 @@ __global__ void __launch_bounds__(kPairThreads, 1) fmha_fwd_pair_kernel(const __
     auto decode = [&](int x, int y, int z) {
       PairItem it;
       int b = z;
-      if constexpr (!KEYADD) {
+      if constexpr (CAUSAL) {
+        b = y;
+        y = x;
+        x = gridDim.z - 1 - z;
+      }
+      if constexpr (!KEYADD && !CAUSAL) {
         if (a.length_class_shift >= 0) {
           const int* len = reinterpret_cast<const int*>(a.mask);
           int n = 0;
@@ -251,6 +265,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) fmha_fwd_pair_kernel(const __
         it.row_base = cu[b];
         it.k_limit = it.row_base < 0 ? 0 : min(cu[b + 1] - it.row_base, a.S_q);   // a sequence longer than the stated maximum is cut there
         it.q_limit = min(it.k_limit, a.total_rows - it.row_base);   // offsets past the tensor, which the host cannot see: no row behind it
+        if constexpr (CAUSAL) it.k_limit = it.q_limit;
       }
       const int rows = it.q_limit - it.q0;
       it.tiles = rows <= 0 ? 0 : rows <= kTileM ? 1 : 2;
@@ -285,10 +300,10 @@ __global__ void __launch_bounds__(kPairThreads, 1) fmha_fwd_pair_kernel(const __
       ++n;
       if (it.tiles > 0) {
         const int tb = PACKED ? 0 : it.b;
-        const int n_kv = (it.k_limit + TN - 1) / TN;
+        const int n_kv = steps_of(it, it.tiles - 1), hk = CAUSAL ? it.h / a.kv_group : it.h;
         for (int j = 0; j < n_kv && lane == 0; ++j) {
-          load_tile(&a.tm_k, it.row_base + j * TN, it.h, tb);
-          load_tile(&a.tm_v, it.row_base + j * TN, it.h, tb);
+          load_tile(&a.tm_k, it.row_base + j * TN, hk, tb);
+          load_tile(&a.tm_v, it.row_base + j * TN, hk, tb);
           if (j == 0) {   // the buffers come free with the last Q K^T of the item before
             for (int g = 0; g < it.tiles; ++g) {
               const int wg = g == 0 ? w : w1;
@@ -352,13 +367,16 @@ __global__ void __launch_bounds__(kPairThreads, 1) fmha_fwd_pair_kernel(const __
       item_done(n);
       if (it.tiles < 0) break;
       if (it.tiles == 0) continue;
-      const int n_kv = (it.k_limit + TN - 1) / TN;
-      if (g >= it.tiles) {   // no such tile: only keep the ring going
-        for (int i = 0; i < 2 * n_kv; ++i, kv.next()) {
+      const int n_kv = steps_of(it, g);
+      auto pass_on = [&](int tiles) {   // K and V tiles that this warp's query tile does not need
+        for (int i = 0; i < tiles; ++i, kv.next()) {
           mbar_wait(kv_full + kv.slot, kv.phase, wctx, kPrKvFull, 200);
           __syncwarp();
           if (lane == 0) mbar_arrive(kv_empty + kv.slot);
         }
+      };
+      if (g >= it.tiles) {   // no such tile: only keep the ring going
+        pass_on(2 * steps_of(it, it.tiles - 1));
         continue;
       }
       mbar_wait(kv_full + kv.slot, kv.phase, wctx, kPrKvFull);
@@ -372,6 +390,9 @@ __global__ void __launch_bounds__(kPairThreads, 1) fmha_fwd_pair_kernel(const __
         const bool more = j + 1 < n_kv;
         const uint64_t dv = make_smem_desc_sw128(smem_u32(sKv + kv.slot * L::kTile), L::kSub, 1024);
         mbar_wait(kv_full + kv.slot, kv.phase, wctx, kPrKvFull);
+        if constexpr (CAUSAL) {   // in the last tile of a sequence, of which there is one
+          if (!more && n_kv * TN > it.k_limit) zero_tile_rows<D / 64>(sKv + kv.slot * L::kTile, it.k_limit - j * TN, TN, L::kSub);
+        }
         if (more) mbar_wait(kv_full + nk.slot, nk.phase, wctx, kPrKvFull);
         uint64_t y[KP];
 #pragma unroll
@@ -388,6 +409,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) fmha_fwd_pair_kernel(const __
         umma_commit_elect(kv_empty + kv.slot);
         kv = nk;
       }
+      if constexpr (CAUSAL) pass_on(2 * (steps_of(it, it.tiles - 1) - n_kv));
       ++w;
     }
   } else if constexpr (KEYADD) {
@@ -436,7 +458,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) fmha_fwd_pair_kernel(const __
       if (it.tiles < 0) break;
       int q_row = it.q0 + g * kTileM + row;
       if (g < it.tiles) {
-        const int n_kv = (it.k_limit + TN - 1) / TN;
+        const int n_kv = steps_of(it, g);
         float m_ref = -INFINITY;
         float2 sum2 = make_float2(0.f, 0.f);   // running sum of exp2(t - m_ref), two interleaved partial sums
         auto wait_s = [&]() { mbar_wait(s_full + g, s_par, wctx, kPrSFull, 32); };
@@ -446,7 +468,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) fmha_fwd_pair_kernel(const __
         };
         // Turns at the exponentials: warp `quad` of the one tile and of the other, which share a scheduler and its special-function
         // unit.
-        const bool turns = it.tiles == 2;
+        bool turns = it.tiles == 2;
         auto turn_begin = [&]() {
           if (turns) {
             mbar_wait(turn + g * 4 + quad, turn_par, wctx, kPrTurn);
@@ -463,6 +485,12 @@ __global__ void __launch_bounds__(kPairThreads, 1) fmha_fwd_pair_kernel(const __
             mbar_wait(mask_full + (t & 1), (t >> 1) & 1, wctx, kPrMaskFull, 32);
             kind = __shfl_sync(0xffffffffu, mask_kind[t & 1], 0);
           }
+          if constexpr (CAUSAL) {
+            const int n_cols = min(TN, it.k_limit - j * TN), diag = it.q0 + g * kTileM - j * TN;
+            if (j == steps_of(it, 0)) turns = false;   // the second tile's last step
+            softmax_step_128_causal<BF16, PF>(tS, tO, j * TN, min(n_cols, diag + quad * 32 + 32), min(n_cols, diag + row + 1), sl2, no_drop, m_ref, sum2,
+                                              wait_s, arrive_p, turn_begin, turn_end);
+          } else
           softmax_step_128<BF16, KEYADD, false, PF>(tS, tO, j * TN, min(TN, it.k_limit - j * TN), sl2, mask_stage, kind, no_drop, m_ref,
                                                       sum2, wait_s, arrive_p, turn_begin, turn_end);
           s_par ^= 1u;
@@ -563,10 +591,17 @@ bool fwd_pair_applies(const FwdArgs& a, int head_dim) {
   return fwd_pair_pays(sm_count(), a.B, a.H, a.S_q, a.S_k, packed || a.mask_kind == FMHA_MASK_SEQLEN, packed ? a.total_rows : 0);
 }
 
-template <bool BF16, bool KEYADD, bool PACKED>
+// Causal: grids of at least a pair of tiles per SM by the average length.
+bool fwd_pair_causal_pays(int64_t sms, int64_t B, int64_t H, int64_t max_len, int64_t total_rows) {
+  if (sms <= 0) return false;
+  const int64_t n_avg = (std::min(max_len, (total_rows + B - 1) / B) + kTileM - 1) / kTileM;
+  return max_len > 256 && B * H * ((n_avg + 1) / 2) >= sms;
+}
+
+template <bool BF16, bool KEYADD, bool PACKED, bool CAUSAL = false>
 static int launch_pair_impl(const FwdArgs& a, cudaStream_t stream) {
   using L = PairSmem;
-  auto kfn = fmha_fwd_pair_kernel<BF16, KEYADD, PACKED>;
+  auto kfn = fmha_fwd_pair_kernel<BF16, KEYADD, PACKED, CAUSAL>;
   static std::atomic<bool> configured[64] = {};   // per device; set after the attribute call succeeded
   int dev = 0;
   cudaGetDevice(&dev);
@@ -578,17 +613,22 @@ static int launch_pair_impl(const FwdArgs& a, cudaStream_t stream) {
     if (attr.numRegs < L::kRegsLaunch) return static_cast<int>(cudaErrorInvalidConfiguration);
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
-  const dim3 grid((a.S_q + 2 * kTileM - 1) / (2 * kTileM), a.H, a.B);
+  const unsigned pairs = (a.S_q + 2 * kTileM - 1) / (2 * kTileM);
+  const dim3 grid = CAUSAL ? dim3(a.H, a.B, pairs) : dim3(pairs, a.H, a.B);
   const int64_t items = static_cast<int64_t>(grid.x) * grid.y * grid.z;
   FwdArgs args = a;
   args.persist = items > sm_count();
   args.length_class_shift = -1;
-  if (args.persist && (a.mask_kind == FMHA_MASK_SEQLEN || a.mask_kind == FMHA_MASK_CU_SEQLENS) && a.B >= 2 && a.B <= kMaxOrdered) {
+  if (!CAUSAL && args.persist && (a.mask_kind == FMHA_MASK_SEQLEN || a.mask_kind == FMHA_MASK_CU_SEQLENS) && a.B >= 2 && a.B <= kMaxOrdered) {
     args.length_class_shift = 0;
     while ((a.S_k - 1) >> args.length_class_shift > 7) ++args.length_class_shift;
   }
   const cudaError_t e = launch_overlapped(kfn, grid, dim3(kPairThreads), L::kDynBytes, stream, args);
   return static_cast<int>(e != cudaSuccess ? e : cudaGetLastError());
+}
+
+int launch_fwd_pair_causal(const FwdArgs& a, int dtype, cudaStream_t stream) {
+  return dtype == FMHA_DTYPE_BF16 ? launch_pair_impl<true, false, true, true>(a, stream) : launch_pair_impl<false, false, true, true>(a, stream);
 }
 
 int launch_fwd_pair(const FwdArgs& a, int dtype, cudaStream_t stream) {

@@ -300,6 +300,39 @@ __device__ __forceinline__ void softmax_step_128(uint32_t tS, uint32_t tO, int k
     softmax_step<128, 64, BF16, KEYADD, DROP, P_FIRST, 0, 64>(tS, tO, key0, n_cols, sl2, mask_stage, kind, dr, m_ref, sum2, wait_s, arrive_p, turn_begin, turn_end);
 }
 
+// Causal variants.  A row sees the keys up to its own position, so the number of columns differs from lane to lane in the steps on the
+// diagonal; which copy of the step runs goes by the most that a row of the warp has (`warp_cols`), so that all lanes take the same one.
+// Rows 32 q to 32 q + 31 of a tile end in the columns 32 q + 1 to 32 q + 32 of its diagonal: where warp_cols passes half a step, every row has
+// at least half (rows past the end of the sequence, which may have fewer, are never stored).  A step in which a warp has no column leaves P
+// zero (64-key steps at head dimension 64, the first two warps).
+template <class WaitS, class ArriveP>
+__device__ __forceinline__ void softmax_step_none(uint32_t tS, int pairs, const WaitS& wait_s, const ArriveP& arrive_p) {
+  wait_s();
+  tc_fence_after_sync();
+  const uint32_t zero[16] = {};
+  for (int c = 0; c < pairs / 16; ++c) tmem_st16(tS + c * 16, zero);
+  tmem_wait_st();
+  tc_fence_before_sync();
+  arrive_p(1);
+}
+template <bool BF16, class WaitS, class ArriveP>
+__device__ __forceinline__ void softmax_step_64_causal(uint32_t tS, uint32_t tO, int key0, int warp_cols, int n_cols, float sl2, const DropRow& dr,
+                                                       float& m_ref, float2& sum2, const WaitS& wait_s, const ArriveP& arrive_p) {
+  auto none = [] {};
+  if (warp_cols > 32) softmax_step<64, 64, BF16, false, false, 0, 32, 0>(tS, tO, key0, n_cols, sl2, nullptr, kMaskZero, dr, m_ref, sum2, wait_s, arrive_p, none, none);
+  else if (warp_cols > 0) softmax_step<64, 32, BF16, false, false, 0, 0, 32>(tS, tO, key0, n_cols, sl2, nullptr, kMaskZero, dr, m_ref, sum2, wait_s, arrive_p, none, none);
+  else softmax_step_none(tS, 32, wait_s, arrive_p);
+}
+template <bool BF16, int P_FIRST, class WaitS, class ArriveP, class TurnBegin, class TurnEnd>
+__device__ __forceinline__ void softmax_step_128_causal(uint32_t tS, uint32_t tO, int key0, int warp_cols, int n_cols, float sl2, const DropRow& dr,
+                                                        float& m_ref, float2& sum2, const WaitS& wait_s, const ArriveP& arrive_p,
+                                                        const TurnBegin& turn_begin, const TurnEnd& turn_end) {
+  if (warp_cols > 64)
+    softmax_step<128, 128, BF16, false, false, P_FIRST, 64, 0>(tS, tO, key0, n_cols, sl2, nullptr, kMaskZero, dr, m_ref, sum2, wait_s, arrive_p, turn_begin, turn_end);
+  else
+    softmax_step<128, 64, BF16, false, false, P_FIRST, 0, 64>(tS, tO, key0, n_cols, sl2, nullptr, kMaskZero, dr, m_ref, sum2, wait_s, arrive_p, turn_begin, turn_end);
+}
+
 // O of a finished query tile out of tensor memory, scaled and rounded: into `tile` (shared memory, 128 rows in the swizzled
 // layout of the O tensor map), or, where the tile reaches into rows that are not its own, the valid rows straight to `grow`.
 template <int D, bool BF16>

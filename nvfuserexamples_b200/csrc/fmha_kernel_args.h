@@ -40,6 +40,7 @@ struct FwdArgs {
   int total_rows;
   int zero_uncovered;         // FMHA_FLAG_ZERO_UNCOVERED: 0, or an UncoveredMode
   int persist;                // pair kernel: a CTA takes further items of the grid when it has done its own
+  int kv_group;               // causal variants: query heads per key head (else 0)
   int length_class_shift;     // production kernels: -1, or the grid's last axis counts batch elements by (length - 1) >> shift
   const void* q_ptr;          // the kernel for a handful of query rows reads Q with plain loads
   int64_t q_ss, q_sh, q_sb;
@@ -94,6 +95,7 @@ struct BwdArgs {
   int64_t dq_ss, dq_sh, dq_sb;
   UncoveredRows zero;
   int persist;   // a CTA takes further work items of the grid when it has done its own
+  int H_kv, kv_group;   // causal variants: key heads, query heads per key head (else 0)
   int B, H, S_q, S_k;
   float scale;       // softmax scale
   float scale_log2;  // softmax scale * log2(e)
@@ -129,6 +131,10 @@ bool fwd_pair_applies(const FwdArgs& a, int D);
 // its rule on sizes, on a device of `sms` multiprocessors (lengths: sequences may differ; packed_rows: rows of a packed batch, else 0)
 bool fwd_pair_pays(int64_t sms, int64_t B, int64_t H, int64_t S_q, int64_t S_k, bool lengths, int64_t packed_rows);
 int launch_fwd_pair(const FwdArgs& a, int dtype, cudaStream_t stream);
+// causal attention of a packed batch with grouped heads: the one-tile kernel, or at head dimension 128 the pair kernel by its rule on sizes
+int launch_fwd_causal(const FwdArgs& a, int D, int dtype, cudaStream_t stream);
+bool fwd_pair_causal_pays(int64_t sms, int64_t B, int64_t H, int64_t max_len, int64_t total_rows);
+int launch_fwd_pair_causal(const FwdArgs& a, int dtype, cudaStream_t stream);
 // the one-tile kernel's choice of order: a shift that puts the lengths into classes, or -1
 int fwd_length_class_shift(const FwdArgs& a, int D, int64_t ctas, bool no_lengths);
 // the same at head dimension 64 for grids of more tiles than the chip holds: a CTA takes one tile after the other (fmha_fwd_chain_sm100.cu)

@@ -27,6 +27,7 @@
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/variable.h>
 
+#include <algorithm>
 #include <array>
 #include <cmath>
 #include <cstdlib>
@@ -601,6 +602,86 @@ at::Tensor fmha_varlen_qkvpacked_bwd(const at::Tensor& d_o, const at::Tensor& qk
   return dqkv;
 }
 
+// ---------------------------------------------------------------------------------------
+// causal attention of packed sequences with grouped heads: q, o [total, H, D]; k, v [total, H_kv, D]
+// ---------------------------------------------------------------------------------------
+void check_causal(const Packed& q, const Packed& k, const Packed& v, int64_t max_seqlen) {
+  TORCH_CHECK(q.D == 64 || q.D == 128, "mha_manual: head dimension must be 64 or 128, got ", q.D);
+  TORCH_CHECK(k.D == q.D && v.D == q.D && k.total == q.total && v.total == q.total,
+              "mha_manual: packed q, k, v must have the same rows and head dimension");
+  TORCH_CHECK(k.H == v.H && k.H > 0 && q.H % k.H == 0, "mha_manual: k and v must have the same number of heads, of which q has a multiple");
+  TORCH_CHECK(max_seqlen > 0, "mha_manual: max_seqlen must be positive");
+  TORCH_CHECK(q.total <= INT32_MAX, "mha_manual: too many rows");
+}
+template <typename Params>
+void fill_causal(Params& p, const at::Tensor& q, const Packed& vq, const Packed& vk, const at::Tensor& cu, int64_t max_seqlen,
+                 c10::optional<double> scale) {
+  p.struct_bytes = sizeof(p);
+  p.dtype = dtype_code(q);
+  p.B = static_cast<int32_t>(cu.numel() - 1); p.H = static_cast<int32_t>(vq.H); p.H_kv = static_cast<int32_t>(vk.H);
+  p.max_seqlen = static_cast<int32_t>(std::min<int64_t>(max_seqlen, vq.total)); p.D = static_cast<int32_t>(vq.D);
+  p.scale = scale.has_value() ? static_cast<float>(*scale) : 1.0f / std::sqrt(static_cast<float>(vq.D));
+  p.cu_seqlens = cu.data_ptr<int32_t>();
+  p.total_rows = static_cast<int32_t>(vq.total);
+  p.flags = FMHA_FLAG_ZERO_UNCOVERED;   // rows outside the sequences, or past max_seqlen of theirs, are returned as zeros
+}
+
+std::tuple<at::Tensor, at::Tensor> fmha_causal_varlen_fwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                                          const at::Tensor& cu_seqlens, int64_t max_seqlen, c10::optional<double> scale) {
+  const Packed vq = packed3(q, "q"), vk = packed3(k, "k"), vv = packed3(v, "v");
+  check_same(q, k, "k");
+  check_same(q, v, "v");
+  check_causal(vq, vk, vv, max_seqlen);
+  const c10::cuda::CUDAGuard guard(q.device());
+  const int dev = q.get_device();
+  const at::Tensor cu = check_cu_seqlens(cu_seqlens, q);
+  at::Tensor o = empty_on(q, q.sizes(), q.scalar_type());
+  at::Tensor lse = empty_on(q, {vq.H, vq.total}, at::kFloat);
+  if (vq.total == 0) return {o, lse};
+  fmha_causal_fwd_params p{};
+  fill_causal(p, q, vq, vk, cu, max_seqlen, scale);
+  p.q = vq.t; p.k = vk.t; p.v = vv.t; p.o = packed3(o, "o").t;
+  p.lse = lse.data_ptr<float>();
+  p.status = status_block(dev).data_ptr<int32_t>();
+  finish_call(fmha_sm100_causal_fwd(&p, at::cuda::getCurrentCUDAStream(dev).stream()), "fmha_causal_varlen_fwd", dev);
+  return {o, lse};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> fmha_causal_varlen_bwd(const at::Tensor& d_o, const at::Tensor& q, const at::Tensor& k,
+                                                                      const at::Tensor& v, const at::Tensor& o, const at::Tensor& lse,
+                                                                      const at::Tensor& cu_seqlens, int64_t max_seqlen,
+                                                                      c10::optional<double> scale) {
+  const Packed vq = packed3(q, "q"), vk = packed3(k, "k"), vv = packed3(v, "v"), vo = packed3(o, "o");
+  at::Tensor d_o_c = dense_if_needed(d_o);
+  const Packed vdo = packed3(d_o_c, "d_o");
+  check_same(q, k, "k"); check_same(q, v, "v"); check_same(q, o, "o"); check_same(q, d_o_c, "d_o");
+  TORCH_CHECK(o.sizes() == q.sizes() && d_o_c.sizes() == q.sizes(), "mha_manual: o and d_o must have the shape of q");
+  check_causal(vq, vk, vv, max_seqlen);
+  TORCH_CHECK(lse.device() == q.device() && lse.scalar_type() == at::kFloat && lse.numel() == vq.H * vq.total,
+              "mha_manual: lse must be float32 [H, total_rows] on the device of q");
+  const c10::cuda::CUDAGuard guard(q.device());
+  const int dev = q.get_device();
+  const at::Tensor cu = check_cu_seqlens(cu_seqlens, q);
+  at::Tensor lse_c = lse.contiguous();
+  at::Tensor dq = empty_on(q, q.sizes(), q.scalar_type());
+  at::Tensor dk = empty_on(k, k.sizes(), k.scalar_type());
+  at::Tensor dv = empty_on(v, v.sizes(), v.scalar_type());
+  if (vq.total == 0) return {dq, dk, dv};
+  fmha_causal_bwd_params p{};
+  fill_causal(p, q, vq, vk, cu, max_seqlen, scale);
+  p.q = vq.t; p.k = vk.t; p.v = vv.t; p.o = vo.t; p.d_o = vdo.t;
+  p.lse = lse_c.data_ptr<float>();
+  p.dq = packed3(dq, "dq").t; p.dk = packed3(dk, "dk").t; p.dv = packed3(dv, "dv").t;
+  size_t bytes = 0;
+  raise_if(fmha_sm100_causal_bwd_workspace_bytes(&p, &bytes), "causal_bwd_workspace_bytes");
+  at::Tensor ws = empty_on(q, {static_cast<int64_t>(bytes)}, at::kByte);
+  p.workspace = ws.data_ptr();
+  p.workspace_bytes = bytes;
+  p.status = status_block(dev).data_ptr<int32_t>();
+  finish_call(fmha_sm100_causal_bwd(&p, at::cuda::getCurrentCUDAStream(dev).stream()), "fmha_causal_varlen_bwd", dev);
+  return {dq, dk, dv};
+}
+
 at::Tensor philox_dropout_mask(int64_t B, int64_t H, int64_t S_q, int64_t S_k, double p, int64_t seed, int64_t offset,
                                int64_t bh_offset, bool on_device) {
   TORCH_CHECK(B >= 0 && H >= 0 && S_q >= 0 && S_k >= 0, "mha_manual: negative size");
@@ -857,7 +938,27 @@ at::Tensor fmha_varlen_qkvpacked_autograd(const at::Tensor& qkv, const at::Tenso
                                                 [&] { return op.call(qkv, cu_seqlens, max_seqlen, p_drop, seed, offset, scale, offset_tensor); });
 }
 
-// The same four operators below the autograd keys (torch.inference_mode(), a redispatch from another autograd
+struct FmhaCausalVarlenFunction : public OpFunction<FmhaCausalVarlenFunction> {
+  static variable_list gradients(const variable_list& saved, const Scalars& c, const at::Tensor& d_o) {
+    static auto op = find_op<Triple, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                             const at::Tensor&, const at::Tensor&, int64_t, c10::optional<double>>("mha_manual::fmha_causal_varlen_bwd");
+    const Recorded<3> r{saved};
+    return r.gradients([&]() -> variable_list {
+      auto [dq, dk, dv] = op.call(d_o, r.in(0), r.in(1), r.in(2), r.o(), r.lse(), *r.lens(), c.max_seqlen, c.scale);
+      return {dq, dk, dv};
+    });
+  }
+};
+at::Tensor fmha_causal_varlen_autograd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& cu_seqlens,
+                                       int64_t max_seqlen, c10::optional<double> scale) {
+  static auto op = find_op<Pair, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, int64_t, c10::optional<double>>(
+      "mha_manual::fmha_causal_varlen_fwd");
+  return record<FmhaCausalVarlenFunction, 3>({TensorRef(q), TensorRef(k), TensorRef(v)}, OptTensor(), cu_seqlens, OptTensor(),
+                                             {max_seqlen, 0.0, 0, 0, scale},
+                                             [&] { return op.call(q, k, v, cu_seqlens, max_seqlen, scale); });
+}
+
+// The same operators below the autograd keys (torch.inference_mode(), a redispatch from another autograd
 // layer): forward only, no graph is recorded.  Registered for the CUDA and Meta keys; they go through the dispatcher,
 // so a Meta call lands in the shape-only kernels.
 template <typename Ret, typename... Args>
@@ -894,6 +995,12 @@ at::Tensor fmha_varlen_qkvpacked_noautograd(const at::Tensor& qkv, const at::Ten
   return std::get<0>(call_op<std::tuple<at::Tensor, at::Tensor>, const at::Tensor&, const at::Tensor&, int64_t, double, int64_t,
                              int64_t, c10::optional<double>, const c10::optional<at::Tensor>&>(
       "mha_manual::fmha_varlen_qkvpacked_fwd", qkv, cu_seqlens, max_seqlen, p_drop, seed, offset, scale, offset_tensor));
+}
+
+at::Tensor fmha_causal_varlen_noautograd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& cu_seqlens,
+                                         int64_t max_seqlen, c10::optional<double> scale) {
+  return std::get<0>(call_op<std::tuple<at::Tensor, at::Tensor>, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                             int64_t, c10::optional<double>>("mha_manual::fmha_causal_varlen_fwd", q, k, v, cu_seqlens, max_seqlen, scale));
 }
 
 // ---------------------------------------------------------------------------------------
@@ -1052,6 +1159,31 @@ at::Tensor fmha_varlen_qkvpacked_bwd_meta(const at::Tensor& d_o, const at::Tenso
   return at::empty(qkv.sizes(), qkv.options());
 }
 
+void meta_check_causal(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& cu, int64_t max_seqlen) {
+  TORCH_CHECK(q.dim() == 3 && k.dim() == 3, "mha_manual: q and k must be [total_rows, H, D]");
+  TORCH_CHECK(q.scalar_type() == at::kHalf || q.scalar_type() == at::kBFloat16, "mha_manual: q must be float16 or bfloat16");
+  TORCH_CHECK(v.sizes() == k.sizes() && k.size(0) == q.size(0) && k.size(2) == q.size(2) && k.size(1) > 0 && q.size(1) % k.size(1) == 0 &&
+                  k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(),
+              "mha_manual: packed q, k, v must have the same rows, head dimension and dtype, and q a multiple of the heads of k and v");
+  TORCH_CHECK(q.size(2) == 64 || q.size(2) == 128, "mha_manual: head dimension must be 64 or 128, got ", q.size(2));
+  TORCH_CHECK(cu.dim() == 1 && cu.numel() >= 2, "mha_manual: cu_seqlens must be [B+1]");
+  TORCH_CHECK(max_seqlen > 0, "mha_manual: max_seqlen must be positive");
+}
+std::tuple<at::Tensor, at::Tensor> fmha_causal_varlen_fwd_meta(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                                               const at::Tensor& cu_seqlens, int64_t max_seqlen, c10::optional<double>) {
+  meta_check_causal(q, k, v, cu_seqlens, max_seqlen);
+  return {at::empty(q.sizes(), q.options()), at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat))};
+}
+std::tuple<at::Tensor, at::Tensor, at::Tensor> fmha_causal_varlen_bwd_meta(const at::Tensor& d_o, const at::Tensor& q, const at::Tensor& k,
+                                                                           const at::Tensor& v, const at::Tensor& o, const at::Tensor& lse,
+                                                                           const at::Tensor& cu_seqlens, int64_t max_seqlen,
+                                                                           c10::optional<double>) {
+  meta_check_causal(q, k, v, cu_seqlens, max_seqlen);
+  TORCH_CHECK(o.sizes() == q.sizes() && d_o.sizes() == q.sizes(), "mha_manual: o and d_o must have the shape of q");
+  TORCH_CHECK(lse.scalar_type() == at::kFloat && lse.numel() == q.size(0) * q.size(1), "mha_manual: lse must be float32 [H, total_rows]");
+  return {at::empty(q.sizes(), q.options()), at::empty(k.sizes(), k.options()), at::empty(v.sizes(), v.options())};
+}
+
 }  // namespace
 
 TORCH_LIBRARY(mha_manual, m) {
@@ -1083,6 +1215,10 @@ TORCH_LIBRARY(mha_manual, m) {
         "float p_drop=0.0, int seed=0, int offset=0, float? scale=None, Tensor? offset_tensor=None) -> Tensor");
   m.def("fmha_varlen_qkvpacked(Tensor qkv, Tensor cu_seqlens, int max_seqlen, float p_drop=0.0, int seed=0, "
         "int offset=0, float? scale=None, Tensor? offset_tensor=None) -> Tensor");
+  m.def("fmha_causal_varlen_fwd(Tensor q, Tensor k, Tensor v, Tensor cu_seqlens, int max_seqlen, float? scale=None) -> (Tensor, Tensor)");
+  m.def("fmha_causal_varlen_bwd(Tensor d_o, Tensor q, Tensor k, Tensor v, Tensor o, Tensor lse, Tensor cu_seqlens, int max_seqlen, "
+        "float? scale=None) -> (Tensor, Tensor, Tensor)");
+  m.def("fmha_causal_varlen(Tensor q, Tensor k, Tensor v, Tensor cu_seqlens, int max_seqlen, float? scale=None) -> Tensor");
   m.def("philox_dropout_mask(int B, int H, int S_q, int S_k, float p, int seed, int offset, int bh_offset=0, "
         "bool on_device=False) -> Tensor", philox_dropout_mask);
   m.def("check_status() -> ()", check_status);
@@ -1100,6 +1236,9 @@ TORCH_LIBRARY_IMPL(mha_manual, CUDA, m) {
   m.impl("fmha_qkvpacked_bwd", fmha_qkvpacked_bwd);
   m.impl("fmha_varlen_qkvpacked_fwd", fmha_varlen_qkvpacked_fwd);
   m.impl("fmha_varlen_qkvpacked_bwd", fmha_varlen_qkvpacked_bwd);
+  m.impl("fmha_causal_varlen_fwd", fmha_causal_varlen_fwd);
+  m.impl("fmha_causal_varlen_bwd", fmha_causal_varlen_bwd);
+  m.impl("fmha_causal_varlen", fmha_causal_varlen_noautograd);
   m.impl("fmha", fmha_noautograd);
   m.impl("fmha_varlen", fmha_varlen_noautograd);
   m.impl("fmha_qkvpacked", fmha_qkvpacked_noautograd);
@@ -1118,6 +1257,9 @@ TORCH_LIBRARY_IMPL(mha_manual, Meta, m) {
   m.impl("fmha_qkvpacked_bwd", fmha_qkvpacked_bwd_meta);
   m.impl("fmha_varlen_qkvpacked_fwd", fmha_varlen_qkvpacked_fwd_meta);
   m.impl("fmha_varlen_qkvpacked_bwd", fmha_varlen_qkvpacked_bwd_meta);
+  m.impl("fmha_causal_varlen_fwd", fmha_causal_varlen_fwd_meta);
+  m.impl("fmha_causal_varlen_bwd", fmha_causal_varlen_bwd_meta);
+  m.impl("fmha_causal_varlen", fmha_causal_varlen_noautograd);
   m.impl("fmha", fmha_noautograd);
   m.impl("fmha_varlen", fmha_varlen_noautograd);
   m.impl("fmha_qkvpacked", fmha_qkvpacked_noautograd);
@@ -1127,6 +1269,7 @@ TORCH_LIBRARY_IMPL(mha_manual, Meta, m) {
 TORCH_LIBRARY_IMPL(mha_manual, Autograd, m) {
   m.impl("fmha", fmha_autograd);
   m.impl("fmha_varlen", fmha_varlen_autograd);
+  m.impl("fmha_causal_varlen", fmha_causal_varlen_autograd);
   m.impl("fmha_qkvpacked", fmha_qkvpacked_autograd);
   m.impl("fmha_varlen_qkvpacked", fmha_varlen_qkvpacked_autograd);
 }

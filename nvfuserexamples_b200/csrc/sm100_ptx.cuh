@@ -625,4 +625,16 @@ __device__ __forceinline__ uint32_t sw128_offset(int row, int chunk) {
   return static_cast<uint32_t>(row) * 128u + (static_cast<uint32_t>(chunk ^ (row & 7)) << 4);
 }
 
+// Zeroes rows [from, to) of a tile of SUBS 64-column sub-tiles `sub` bytes apart, by a whole warp, before MMAs of that warp read it: rows
+// behind the end of a sequence belong to another one, or to nobody, and an infinity or NaN there times a zero probability is a NaN.
+template <int SUBS>
+__device__ __forceinline__ void zero_tile_rows(uint8_t* tile, int from, int to, int sub) {
+  const uint32_t at = smem_u32(tile);
+  for (int i = from * 8 + static_cast<int>(threadIdx.x & 31); i < to * 8; i += 32)   // 16-byte pieces of 128-byte rows, whatever their order
+#pragma unroll
+    for (int c = 0; c < SUBS; ++c) sts128(at + c * sub + i * 16, 0u, 0u, 0u, 0u);
+  fence_proxy_async_smem();
+  __syncwarp();
+}
+
 }  // namespace fmha
