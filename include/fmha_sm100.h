@@ -22,6 +22,7 @@
  *                          tensor (fmha/fmha_manual.cpp:433-449); these regenerate that
  *                          mask from (seed, offset) so that it never has to be stored.
  *   fmha_sm100_causal_*  — no counterpart: the reference has no causal mask and one key head per query head.
+ *   fmha_sm100_kv_append, _kv_read, _paged_fwd — no counterpart: the reference keeps no keys and values.
  */
 #ifndef FMHA_SM100_H_
 #define FMHA_SM100_H_
@@ -199,6 +200,76 @@ typedef struct {
   int32_t* status;
 } fmha_causal_bwd_params;
 
+/* A paged cache of keys and values.  Row p of a sequence lies in row p % page_rows of the page that entry p / page_rows of the sequence's
+   line of the page table names; a page holds page_rows rows of every key head.
+     16 bits: k and v are [pages, H_kv, page_rows, D] views of 16-bit values (stride_b is that of the pages).
+     4 bits:  k and v are [pages, H_kv, page_rows, D/2] views of bytes (strides in bytes), values 2i and 2i+1 in the low and high half of byte
+              i, and k_params, v_params [pages, H_kv, page_rows, D/32, 2] fp16 with dense last three axes (strides in halves): scale s and
+              base b of 32 values; code c stands for b + s (1 + c/16).  Rows are coded with s = (max - min) 16/15 and b = min - s, both
+              rounded to fp16, and the nearest code; values beyond +-20000 are held as that, 32 values with an infinity or NaN as NaNs.
+   D in {64, 128}; page_rows a multiple of 16, at most 2^16.  Pointers 16-byte aligned, strides multiples of 16 bytes.
+   A table entry outside [0, pages) is never followed: rows on such a page are not written, and read as zeros. */
+typedef struct {
+  int32_t bits;                 /* 16 or 4 */
+  int32_t pages, page_rows, H_kv, D;
+  fmha_tensor4 k, v, k_params, v_params;
+  const int32_t* table;         /* device int32 [B, table_width], lines table_stride apart */
+  int32_t table_width;
+  int64_t table_stride;
+} fmha_kv_cache;
+
+/* New rows of B sequences, packed: sequence b has rows [cu_rows[b], cu_rows[b+1]) of k, v (and q), or, with cu_rows null, total_rows / B
+   rows each.  They are its LAST rows: with them it has seqlens[b], so the i-th of n has position seqlens[b] - n + i.  k (and q) are rotated by
+   their positions: pair j by the angle position * inv_freq[j]; the pairs are values (j, j + n_freq) of a row, or with FMHA_KV_INTERLEAVED (2j, 2j+1);
+   values from 2 n_freq on are not rotated.  Rows outside the sequences, at a negative position or past the page table are not appended;
+   rows of q_out that belong to none or have a negative position are written as zeros.  No two rows may have the same place in the cache. */
+enum { FMHA_KV_INTERLEAVED = 1 };
+typedef struct {
+  int32_t struct_bytes; /* sizeof(fmha_kv_append_params) */
+  int32_t dtype;        /* of q, k, v and a 16-bit cache */
+  int32_t B, H, total_rows;   /* H: heads of q (0: none) */
+  fmha_tensor4 q, k, v; /* [total_rows, H or H_kv, D] views (stride_h, stride_s) */
+  fmha_tensor4 q_out;   /* rotated q, if there is one */
+  fmha_kv_cache cache;
+  const int32_t* seqlens;     /* device int32 [B] */
+  const int32_t* cu_rows;     /* optional device int32 [B+1] */
+  const float* inv_freq;      /* device [n_freq] */
+  int32_t n_freq;             /* 0: no rotation; else 2 n_freq a multiple of 16 (4 bits: of 64), at most D */
+  int32_t flags;              /* FMHA_KV_* */
+} fmha_kv_append_params;
+
+/* Rows [0, cu_rows[b+1] - cu_rows[b]) of every sequence out of the cache, as 16-bit values in order.  Rows outside the sequences are written
+   as zeros. */
+typedef struct {
+  int32_t struct_bytes; /* sizeof(fmha_kv_read_params) */
+  int32_t dtype;        /* of the result; with 16 bits that of the cache */
+  int32_t B, total_rows;
+  fmha_tensor4 k, v;    /* [total_rows, H_kv, D] outputs */
+  fmha_kv_cache cache;
+  const int32_t* cu_rows;
+} fmha_kv_read_params;
+
+/* Attention of the last rows of sequences over all their rows in a paged cache.  q, o are packed like the rows of fmha_kv_append_params; the i-th of n
+   new rows sees positions 0 to seqlens[b] - n + i, query head h reads key head h / (H / H_kv).  A row that sees no key gets zeros and a logsumexp of
+   -infinity, as do rows outside the sequences and past max_rows of theirs.  What the cache holds behind a sequence's last row does not matter; an infinite or
+   NaN value in V of a LATER new row can reach the earlier ones.  From a 4-bit cache products are formed in fp16: q is rounded to it (finite
+   values stay finite). */
+typedef struct {
+  int32_t struct_bytes; /* sizeof(fmha_paged_params) */
+  int32_t dtype;        /* of q, o and a 16-bit cache */
+  int32_t B, H, total_rows;
+  int32_t max_rows;     /* most new rows of a sequence (it sizes the grid) */
+  float scale;
+  fmha_tensor4 q, o;    /* [total_rows, H, D] views (stride_h, stride_s) */
+  float* lse;           /* optional [H, total_rows] */
+  fmha_kv_cache cache;
+  const int32_t* seqlens;
+  const int32_t* cu_rows;     /* optional */
+  void* workspace;            /* device scratch, 256-byte aligned, of fmha_sm100_paged_workspace_bytes() bytes */
+  size_t workspace_bytes;
+  int32_t* status;
+} fmha_paged_params;
+
 /* ---- entry points --------------------------------------------------------------- */
 
 /* Forward: O = dropout(softmax(scale * Q K^T + mask)) V, plus the row logsumexp.
@@ -238,6 +309,13 @@ int fmha_sm100_bwd_static_scratch(const fmha_bwd_params* p, void* stream);
 int fmha_sm100_causal_fwd(const fmha_causal_fwd_params* p, void* stream);
 int fmha_sm100_causal_bwd(const fmha_causal_bwd_params* p, void* stream);
 int fmha_sm100_causal_bwd_workspace_bytes(const fmha_causal_bwd_params* p, size_t* bytes);
+
+/* Paged caches: appending rows, reading rows back, attention of a few new rows.  fmha_sm100_paged_workspace_bytes may give 0 (the keys of a
+   sequence are not dealt out over CTAs then); it depends on the sizes and on the current device. */
+int fmha_sm100_kv_append(const fmha_kv_append_params* p, void* stream);
+int fmha_sm100_kv_read(const fmha_kv_read_params* p, void* stream);
+int fmha_sm100_paged_fwd(const fmha_paged_params* p, void* stream);
+int fmha_sm100_paged_workspace_bytes(const fmha_paged_params* p, size_t* bytes);
 
 /* 7-bit dropout threshold T for a drop probability: T = round(128 p) clamped to [0,127]. */
 int32_t fmha_sm100_dropout_threshold(float p_drop);

@@ -37,6 +37,7 @@ EXPORTS = [
     "fmha_sm100_strerror", "fmha_sm100_last_cuda_error", "fmha_sm100_abi_version",
     "fmha_sm100_selftest_wait_timeout", "fmha_sm100_bwd_static_scratch",
     "fmha_sm100_causal_fwd", "fmha_sm100_causal_bwd", "fmha_sm100_causal_bwd_workspace_bytes",
+    "fmha_sm100_kv_append", "fmha_sm100_kv_read", "fmha_sm100_paged_fwd", "fmha_sm100_paged_workspace_bytes",
 ]
 
 
@@ -106,6 +107,43 @@ class CausalBwdParams(C.Structure):
     ]
 
 
+KV_INTERLEAVED = 1
+
+
+class KvCache(C.Structure):
+    _fields_ = [
+        ("bits", C.c_int32), ("pages", C.c_int32), ("page_rows", C.c_int32), ("H_kv", C.c_int32), ("D", C.c_int32),
+        ("k", Tensor4), ("v", Tensor4), ("k_params", Tensor4), ("v_params", Tensor4),
+        ("table", C.c_void_p), ("table_width", C.c_int32), ("table_stride", C.c_int64),
+    ]
+
+
+class KvAppendParams(C.Structure):
+    _fields_ = [
+        ("struct_bytes", C.c_int32), ("dtype", C.c_int32), ("B", C.c_int32), ("H", C.c_int32), ("total_rows", C.c_int32),
+        ("q", Tensor4), ("k", Tensor4), ("v", Tensor4), ("q_out", Tensor4),
+        ("cache", KvCache), ("seqlens", C.c_void_p), ("cu_rows", C.c_void_p),
+        ("inv_freq", C.c_void_p), ("n_freq", C.c_int32), ("flags", C.c_int32),
+    ]
+
+
+class KvReadParams(C.Structure):
+    _fields_ = [
+        ("struct_bytes", C.c_int32), ("dtype", C.c_int32), ("B", C.c_int32), ("total_rows", C.c_int32),
+        ("k", Tensor4), ("v", Tensor4), ("cache", KvCache), ("cu_rows", C.c_void_p),
+    ]
+
+
+class PagedParams(C.Structure):
+    _fields_ = [
+        ("struct_bytes", C.c_int32), ("dtype", C.c_int32), ("B", C.c_int32), ("H", C.c_int32), ("total_rows", C.c_int32),
+        ("max_rows", C.c_int32), ("scale", C.c_float),
+        ("q", Tensor4), ("o", Tensor4), ("lse", C.c_void_p), ("cache", KvCache),
+        ("seqlens", C.c_void_p), ("cu_rows", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("status", C.c_void_p),
+    ]
+
+
 class FmhaError(RuntimeError):
     def __init__(self, code: int, what: str, detail: str = ""):
         self.code = code
@@ -139,6 +177,11 @@ def load() -> C.CDLL:
     lib.fmha_sm100_causal_bwd.restype = C.c_int
     lib.fmha_sm100_causal_bwd_workspace_bytes.argtypes = [C.POINTER(CausalBwdParams), C.POINTER(C.c_size_t)]
     lib.fmha_sm100_causal_bwd_workspace_bytes.restype = C.c_int
+    for name, params in (("kv_append", KvAppendParams), ("kv_read", KvReadParams), ("paged_fwd", PagedParams)):
+        fn = getattr(lib, f"fmha_sm100_{name}")
+        fn.argtypes, fn.restype = [C.POINTER(params), C.c_void_p], C.c_int
+    lib.fmha_sm100_paged_workspace_bytes.argtypes = [C.POINTER(PagedParams), C.POINTER(C.c_size_t)]
+    lib.fmha_sm100_paged_workspace_bytes.restype = C.c_int
     lib.fmha_sm100_dropout_threshold.argtypes = [C.c_float]
     lib.fmha_sm100_dropout_threshold.restype = C.c_int32
     lib.fmha_sm100_philox_mask_host.argtypes = [C.c_uint64, C.c_uint64, C.c_int32, C.c_int32, C.c_int32, C.c_int32,

@@ -12,6 +12,7 @@
 #include <mutex>
 
 #include "../../include/fmha_sm100.h"
+#include "fmha_capi_common.h"
 #include "fmha_kernel_args.h"
 #include "philox.cuh"
 #include "sm100_ptx.cuh"
@@ -20,14 +21,14 @@ namespace fmha {
 
 static thread_local int g_last_cuda_error = 0;
 
-static int cuda_fail(cudaError_t e) {
+int cuda_fail(cudaError_t e) {
   g_last_cuda_error = static_cast<int>(e);
   return FMHA_ERR_LAUNCH;
 }
 
 // cuTensorMapEncodeTiled, fetched through the runtime so that the library does not link
 // against libcuda directly.
-static PFN_cuTensorMapEncodeTiled_v12000 get_encode_fn() {
+PFN_cuTensorMapEncodeTiled_v12000 get_encode_fn() {
   static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
   static std::once_flag once;
   std::call_once(once, [] {
@@ -152,7 +153,7 @@ static int zero_outside_rows(const UncoveredRows& u, int B, int H, int D, const 
   return static_cast<int>(e != cudaSuccess ? e : cudaGetLastError());
 }
 
-static int check_device() {
+int check_device() {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) { g_last_cuda_error = static_cast<int>(e); return FMHA_ERR_NO_DEVICE; }

@@ -40,6 +40,8 @@
 namespace {
 
 constexpr int kMaxDevices = 64;
+using OptTensor = c10::optional<at::Tensor>;
+using Pair = std::tuple<at::Tensor, at::Tensor>;
 
 // One int32[4] status block per device, allocated on first use and kept for the process.
 at::Tensor& status_block(int device) {
@@ -682,6 +684,216 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> fmha_causal_varlen_bwd(const at::
   return {dq, dk, dv};
 }
 
+// ---------------------------------------------------------------------------------------
+// paged caches: [pages, H_kv, page rows, D] in 16 bits, or [.., D/2] bytes of 4-bit codes with [.., D/32, 2] fp16 scales and bases
+// ---------------------------------------------------------------------------------------
+void check_pages(const at::Tensor& x, const char* name, const at::Tensor& like, int64_t last) {
+  TORCH_CHECK(x.dim() == 4 && x.size(3) == last && x.sizes() == like.sizes(), "mha_manual: ", name, " must be [pages, H_kv, page rows, ",
+              last, "], as the other cache");
+}
+void check_params(const OptTensor& x, const char* name, const at::Tensor& cache, int64_t D) {
+  TORCH_CHECK(x.has_value(), "mha_manual: a 4-bit cache has ", name);
+  TORCH_CHECK(x->dim() == 5 && x->size(0) == cache.size(0) && x->size(1) == cache.size(1) && x->size(2) == cache.size(2) && x->size(3) == D / 32 &&
+                  x->size(4) == 2 && x->scalar_type() == at::kHalf,
+              "mha_manual: ", name, " must be float16 [pages, H_kv, page rows, D/32, 2]");
+}
+// What the shapes say, without looking at memory: the head dimension.
+int64_t check_cache_shapes(const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& table, const OptTensor& k_params,
+                           const OptTensor& v_params) {
+  const bool four = k_cache.scalar_type() == at::kByte;
+  TORCH_CHECK(four || k_cache.scalar_type() == at::kHalf || k_cache.scalar_type() == at::kBFloat16,
+              "mha_manual: k_cache must be float16, bfloat16 or uint8 (4-bit codes)");
+  TORCH_CHECK(v_cache.scalar_type() == k_cache.scalar_type(), "mha_manual: v_cache has a different dtype");
+  TORCH_CHECK(k_cache.dim() == 4, "mha_manual: k_cache must be [pages, H_kv, page rows, D]");
+  const int64_t D = k_cache.size(3) * (four ? 2 : 1);
+  TORCH_CHECK(D == 64 || D == 128, "mha_manual: head dimension must be 64 or 128, got ", D);
+  check_pages(v_cache, "v_cache", k_cache, k_cache.size(3));
+  TORCH_CHECK(k_cache.size(2) > 0 && k_cache.size(2) % 16 == 0, "mha_manual: pages must have a multiple of 16 rows");
+  TORCH_CHECK(k_cache.size(1) > 0, "mha_manual: k_cache has no heads");
+  TORCH_CHECK(k_cache.size(0) <= INT32_MAX && k_cache.size(2) <= (1 << 16), "mha_manual: cache too large");
+  if (four) {
+    check_params(k_params, "k_params", k_cache, D);
+    check_params(v_params, "v_params", k_cache, D);
+  } else {
+    TORCH_CHECK(!k_params.has_value() && !v_params.has_value(), "mha_manual: only a 4-bit cache has k_params and v_params");
+  }
+  TORCH_CHECK(table.dim() == 2 && table.scalar_type() == at::kInt, "mha_manual: block_table must be int32 [B, pages of a sequence]");
+  return D;
+}
+fmha_tensor4 page_view(const at::Tensor& x, const char* name, const at::Tensor& on, bool dense_rows) {
+  TORCH_CHECK(x.is_cuda() && x.device() == on.device(), "mha_manual: ", name, " is on a different device");
+  const int64_t unit = 16 / x.element_size();
+  TORCH_CHECK((reinterpret_cast<uintptr_t>(x.data_ptr()) & 15) == 0, "mha_manual: ", name, " must be 16-byte aligned");
+  TORCH_CHECK(x.stride(-1) == 1, "mha_manual: ", name, " must be contiguous along its last axis");
+  if (dense_rows) {
+    TORCH_CHECK(x.stride(3) == 2 && x.stride(2) == 2 * x.size(3), "mha_manual: ", name, " must be contiguous along its last three axes");
+  } else {
+    TORCH_CHECK(x.stride(2) > 0 && x.stride(2) % unit == 0, "mha_manual: rows of ", name, " must lie at multiples of 16 bytes");
+  }
+  TORCH_CHECK((x.size(1) == 1 || (x.stride(1) > 0 && x.stride(1) % unit == 0)) && (x.size(0) <= 1 || (x.stride(0) > 0 && x.stride(0) % unit == 0)),
+              "mha_manual: strides of ", name, " must be multiples of 16 bytes");
+  return {x.data_ptr(), x.stride(0), x.stride(1), x.stride(2)};
+}
+// Fills p.cache; `on`: a tensor of the device that all others have to be on.
+void fill_cache(fmha_kv_cache& c, const at::Tensor& on, const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& table,
+                const OptTensor& k_params, const OptTensor& v_params) {
+  c.D = static_cast<int32_t>(check_cache_shapes(k_cache, v_cache, table, k_params, v_params));
+  c.bits = k_cache.scalar_type() == at::kByte ? 4 : 16;
+  c.pages = static_cast<int32_t>(k_cache.size(0)); c.H_kv = static_cast<int32_t>(k_cache.size(1)); c.page_rows = static_cast<int32_t>(k_cache.size(2));
+  c.k = page_view(k_cache, "k_cache", on, false);
+  c.v = page_view(v_cache, "v_cache", on, false);
+  if (c.bits == 4) {
+    c.k_params = page_view(*k_params, "k_params", on, true);
+    c.v_params = page_view(*v_params, "v_params", on, true);
+  }
+  TORCH_CHECK(table.device() == on.device(), "mha_manual: block_table is on a different device");
+  TORCH_CHECK(table.size(1) <= 1 || table.stride(1) == 1, "mha_manual: lines of block_table must be contiguous");
+  TORCH_CHECK(table.size(1) <= INT32_MAX && (table.size(0) <= 1 || table.stride(0) >= 0), "mha_manual: bad block_table");
+  c.table = table.data_ptr<int32_t>();
+  c.table_width = static_cast<int32_t>(table.size(1));
+  c.table_stride = table.size(0) > 1 ? table.stride(0) : 0;
+}
+// Lengths and offsets, by shape; then as the kernels read them.
+void check_lens_shapes(const at::Tensor& table, const OptTensor& seqlens, const OptTensor& cu, int64_t rows) {
+  const int64_t B = table.size(0);
+  if (seqlens.has_value()) TORCH_CHECK(seqlens->dim() == 1 && seqlens->numel() == B, "mha_manual: seqlens must be [B], B lines of block_table");
+  if (cu.has_value()) {
+    TORCH_CHECK(cu->dim() == 1 && cu->numel() == B + 1 && B > 0, "mha_manual: cu_seqlens must be [B+1], B lines of block_table");
+  } else {
+    TORCH_CHECK(rows == 0 || (B > 0 && rows % B == 0), "mha_manual: without cu_seqlens every sequence has the same number of rows");
+  }
+  TORCH_CHECK(rows <= INT32_MAX, "mha_manual: too many rows");
+}
+at::Tensor as_ints(const at::Tensor& x, const at::Tensor& on, const char* name) {
+  TORCH_CHECK(x.device() == on.device(), "mha_manual: ", name, " is on a different device");
+  return x.scalar_type() == at::kInt && x.is_contiguous() ? x : x.to(at::kInt).contiguous();
+}
+
+void check_append_shapes(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_cache, int64_t D, const OptTensor& q, const OptTensor& inv_freq) {
+  TORCH_CHECK(k.dim() == 3 && k.sizes() == v.sizes() && k.size(1) == k_cache.size(1) && k.size(2) == D, "mha_manual: k and v must be [total_rows, H_kv, D]");
+  TORCH_CHECK(k.scalar_type() == at::kHalf || k.scalar_type() == at::kBFloat16, "mha_manual: k must be float16 or bfloat16");
+  TORCH_CHECK(v.scalar_type() == k.scalar_type() && (k_cache.scalar_type() == at::kByte || k_cache.scalar_type() == k.scalar_type()),
+              "mha_manual: k, v and a 16-bit cache must have the same dtype");
+  if (q.has_value())
+    TORCH_CHECK(q->dim() == 3 && q->size(0) == k.size(0) && q->size(2) == D && q->scalar_type() == k.scalar_type(),
+                "mha_manual: q must be [total_rows, H, D] of the dtype of k");
+  if (inv_freq.has_value()) {
+    const int64_t n = inv_freq->numel(), step = k_cache.scalar_type() == at::kByte ? 32 : 8;
+    TORCH_CHECK(inv_freq->dim() == 1 && inv_freq->scalar_type() == at::kFloat, "mha_manual: inv_freq must be float32 [pairs]");
+    TORCH_CHECK(2 * n <= D && n % step == 0, "mha_manual: inv_freq must have a multiple of ", step, " pairs, at most D/2, got ", n);
+  }
+}
+OptTensor kv_append(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& block_table,
+                    const at::Tensor& seqlens, const OptTensor& cu_seqlens, const OptTensor& q, const OptTensor& inv_freq, bool interleaved,
+                    const OptTensor& k_params, const OptTensor& v_params) {
+  fmha_kv_append_params p{};
+  TORCH_CHECK(k.is_cuda(), "mha_manual: k must be a CUDA tensor");
+  fill_cache(p.cache, k, k_cache, v_cache, block_table, k_params, v_params);
+  check_append_shapes(k, v, k_cache, p.cache.D, q, inv_freq);
+  check_lens_shapes(block_table, seqlens, cu_seqlens, k.size(0));
+  const c10::cuda::CUDAGuard guard(k.device());
+  const int dev = k.get_device();
+  check_same(k, v, "v");
+  p.struct_bytes = sizeof(p);
+  p.dtype = dtype_code(k);
+  p.B = static_cast<int32_t>(block_table.size(0)); p.total_rows = static_cast<int32_t>(k.size(0));
+  p.k = packed3(k, "k").t; p.v = packed3(v, "v").t;
+  OptTensor out;
+  if (q.has_value()) {
+    check_same(k, *q, "q");
+    out = empty_on(k, q->sizes(), k.scalar_type());
+    p.H = static_cast<int32_t>(q->size(1));
+    p.q = packed3(*q, "q").t; p.q_out = packed3(*out, "q").t;
+  }
+  const at::Tensor lens = as_ints(seqlens, k, "seqlens");
+  at::Tensor cu, freq;
+  p.seqlens = lens.data_ptr<int32_t>();
+  if (cu_seqlens.has_value()) {
+    cu = as_ints(*cu_seqlens, k, "cu_seqlens");
+    p.cu_rows = cu.data_ptr<int32_t>();
+  }
+  if (inv_freq.has_value()) {
+    TORCH_CHECK(inv_freq->device() == k.device(), "mha_manual: inv_freq is on a different device");
+    freq = inv_freq->contiguous();
+    p.inv_freq = freq.data_ptr<float>();
+    p.n_freq = static_cast<int32_t>(freq.numel());
+  }
+  p.flags = interleaved ? FMHA_KV_INTERLEAVED : 0;
+  finish_call(fmha_sm100_kv_append(&p, at::cuda::getCurrentCUDAStream(dev).stream()), "kv_append", dev);
+  return out;
+}
+
+at::ScalarType read_type(const at::Tensor& k_cache, bool bf16) {
+  return k_cache.scalar_type() != at::kByte ? k_cache.scalar_type() : bf16 ? at::kBFloat16 : at::kHalf;
+}
+Pair kv_read(const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& block_table, const at::Tensor& cu_seqlens, int64_t total_rows,
+             const OptTensor& k_params, const OptTensor& v_params, bool bf16) {
+  fmha_kv_read_params p{};
+  TORCH_CHECK(k_cache.is_cuda(), "mha_manual: k_cache must be a CUDA tensor");
+  fill_cache(p.cache, k_cache, k_cache, v_cache, block_table, k_params, v_params);
+  check_lens_shapes(block_table, OptTensor(), cu_seqlens, total_rows);
+  TORCH_CHECK(total_rows >= 0, "mha_manual: total_rows must not be negative");
+  const c10::cuda::CUDAGuard guard(k_cache.device());
+  const int dev = k_cache.get_device();
+  const at::Tensor cu = as_ints(cu_seqlens, k_cache, "cu_seqlens");
+  at::Tensor k = empty_on(k_cache, {total_rows, k_cache.size(1), p.cache.D}, read_type(k_cache, bf16));
+  at::Tensor v = empty_on(k_cache, k.sizes(), k.scalar_type());
+  p.struct_bytes = sizeof(p);
+  p.dtype = dtype_code(k);
+  p.B = static_cast<int32_t>(block_table.size(0)); p.total_rows = static_cast<int32_t>(total_rows);
+  p.k = packed3(k, "k").t; p.v = packed3(v, "v").t;
+  p.cu_rows = cu.data_ptr<int32_t>();
+  finish_call(fmha_sm100_kv_read(&p, at::cuda::getCurrentCUDAStream(dev).stream()), "kv_read", dev);
+  return {k, v};
+}
+
+void check_paged_shapes(const at::Tensor& q, const at::Tensor& k_cache, int64_t D, bool with_cu, int64_t max_rows) {
+  TORCH_CHECK(q.dim() == 3 && q.size(2) == D && q.size(1) > 0 && q.size(1) % k_cache.size(1) == 0,
+              "mha_manual: q must be [total_rows, H, D], H a multiple of the heads of the cache");
+  TORCH_CHECK(q.scalar_type() == at::kHalf || q.scalar_type() == at::kBFloat16, "mha_manual: q must be float16 or bfloat16");
+  TORCH_CHECK(k_cache.scalar_type() == at::kByte || k_cache.scalar_type() == q.scalar_type(), "mha_manual: q and a 16-bit cache must have the same dtype");
+  TORCH_CHECK(!with_cu || max_rows > 0, "mha_manual: with cu_seqlens, max_seqlen_q must be positive");
+  TORCH_CHECK(k_cache.size(0) > 0, "mha_manual: k_cache has no pages");
+}
+std::tuple<at::Tensor, at::Tensor> fmha_paged_fwd(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& block_table,
+                                                  const at::Tensor& seqlens, const OptTensor& cu_seqlens, int64_t max_seqlen_q,
+                                                  c10::optional<double> scale, const OptTensor& k_params, const OptTensor& v_params) {
+  fmha_paged_params p{};
+  TORCH_CHECK(q.is_cuda(), "mha_manual: q must be a CUDA tensor");
+  fill_cache(p.cache, q, k_cache, v_cache, block_table, k_params, v_params);
+  check_paged_shapes(q, k_cache, p.cache.D, cu_seqlens.has_value(), max_seqlen_q);
+  check_lens_shapes(block_table, seqlens, cu_seqlens, q.size(0));
+  const c10::cuda::CUDAGuard guard(q.device());
+  const int dev = q.get_device();
+  at::Tensor o = empty_on(q, q.sizes(), q.scalar_type());
+  at::Tensor lse = empty_on(q, {q.size(1), q.size(0)}, at::kFloat);
+  if (q.size(0) == 0) return {o, lse};
+  p.struct_bytes = sizeof(p);
+  p.dtype = dtype_code(q);
+  p.B = static_cast<int32_t>(block_table.size(0)); p.H = static_cast<int32_t>(q.size(1)); p.total_rows = static_cast<int32_t>(q.size(0));
+  p.max_rows = static_cast<int32_t>(cu_seqlens.has_value() ? std::min<int64_t>(max_seqlen_q, q.size(0)) : q.size(0) / block_table.size(0));
+  p.scale = scale.has_value() ? static_cast<float>(*scale) : 1.0f / std::sqrt(static_cast<float>(p.cache.D));
+  p.q = packed3(q, "q").t; p.o = packed3(o, "o").t;
+  p.lse = lse.data_ptr<float>();
+  const at::Tensor lens = as_ints(seqlens, q, "seqlens");
+  at::Tensor cu, ws;
+  p.seqlens = lens.data_ptr<int32_t>();
+  if (cu_seqlens.has_value()) {
+    cu = as_ints(*cu_seqlens, q, "cu_seqlens");
+    p.cu_rows = cu.data_ptr<int32_t>();
+  }
+  size_t bytes = 0;
+  raise_if(fmha_sm100_paged_workspace_bytes(&p, &bytes), "paged_workspace_bytes");
+  if (bytes > 0) {
+    ws = empty_on(q, {static_cast<int64_t>(bytes)}, at::kByte);
+    p.workspace = ws.data_ptr();
+    p.workspace_bytes = bytes;
+  }
+  p.status = status_block(dev).data_ptr<int32_t>();
+  finish_call(fmha_sm100_paged_fwd(&p, at::cuda::getCurrentCUDAStream(dev).stream()), "fmha_paged_fwd", dev);
+  return {o, lse};
+}
+
 at::Tensor philox_dropout_mask(int64_t B, int64_t H, int64_t S_q, int64_t S_k, double p, int64_t seed, int64_t offset,
                                int64_t bh_offset, bool on_device) {
   TORCH_CHECK(B >= 0 && H >= 0 && S_q >= 0 && S_k >= 0, "mha_manual: negative size");
@@ -723,8 +935,6 @@ void check_status() {
 // ---------------------------------------------------------------------------------------
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
-using OptTensor = c10::optional<at::Tensor>;
-using Pair = std::tuple<at::Tensor, at::Tensor>;
 using Triple = std::tuple<at::Tensor, at::Tensor, at::Tensor>;
 using TensorRef = std::reference_wrapper<const at::Tensor>;
 
@@ -1184,6 +1394,29 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> fmha_causal_varlen_bwd_meta(const
   return {at::empty(q.sizes(), q.options()), at::empty(k.sizes(), k.options()), at::empty(v.sizes(), v.options())};
 }
 
+OptTensor kv_append_meta(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& block_table,
+                         const at::Tensor& seqlens, const OptTensor& cu_seqlens, const OptTensor& q, const OptTensor& inv_freq, bool,
+                         const OptTensor& k_params, const OptTensor& v_params) {
+  check_append_shapes(k, v, k_cache, check_cache_shapes(k_cache, v_cache, block_table, k_params, v_params), q, inv_freq);
+  check_lens_shapes(block_table, seqlens, cu_seqlens, k.size(0));
+  return q.has_value() ? OptTensor(at::empty(q->sizes(), q->options())) : OptTensor();
+}
+Pair kv_read_meta(const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& block_table, const at::Tensor& cu_seqlens, int64_t total_rows,
+                  const OptTensor& k_params, const OptTensor& v_params, bool bf16) {
+  const int64_t D = check_cache_shapes(k_cache, v_cache, block_table, k_params, v_params);
+  check_lens_shapes(block_table, OptTensor(), cu_seqlens, total_rows);
+  const auto options = k_cache.options().dtype(read_type(k_cache, bf16));
+  return {at::empty({total_rows, k_cache.size(1), D}, options), at::empty({total_rows, k_cache.size(1), D}, options)};
+}
+std::tuple<at::Tensor, at::Tensor> fmha_paged_fwd_meta(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                                                       const at::Tensor& block_table, const at::Tensor& seqlens, const OptTensor& cu_seqlens,
+                                                       int64_t max_seqlen_q, c10::optional<double>, const OptTensor& k_params,
+                                                       const OptTensor& v_params) {
+  check_paged_shapes(q, k_cache, check_cache_shapes(k_cache, v_cache, block_table, k_params, v_params), cu_seqlens.has_value(), max_seqlen_q);
+  check_lens_shapes(block_table, seqlens, cu_seqlens, q.size(0));
+  return {at::empty(q.sizes(), q.options()), at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat))};
+}
+
 }  // namespace
 
 TORCH_LIBRARY(mha_manual, m) {
@@ -1219,6 +1452,12 @@ TORCH_LIBRARY(mha_manual, m) {
   m.def("fmha_causal_varlen_bwd(Tensor d_o, Tensor q, Tensor k, Tensor v, Tensor o, Tensor lse, Tensor cu_seqlens, int max_seqlen, "
         "float? scale=None) -> (Tensor, Tensor, Tensor)");
   m.def("fmha_causal_varlen(Tensor q, Tensor k, Tensor v, Tensor cu_seqlens, int max_seqlen, float? scale=None) -> Tensor");
+  m.def("kv_append(Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor block_table, Tensor seqlens, Tensor? cu_seqlens=None, *, "
+        "Tensor? q=None, Tensor? inv_freq=None, bool interleaved=False, Tensor(c!)? k_params=None, Tensor(d!)? v_params=None) -> Tensor?");
+  m.def("kv_read(Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor cu_seqlens, int total_rows, *, Tensor? k_params=None, "
+        "Tensor? v_params=None, bool bf16=False) -> (Tensor, Tensor)");
+  m.def("fmha_paged_fwd(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor seqlens, Tensor? cu_seqlens=None, "
+        "int max_seqlen_q=0, float? scale=None, *, Tensor? k_params=None, Tensor? v_params=None) -> (Tensor, Tensor)");
   m.def("philox_dropout_mask(int B, int H, int S_q, int S_k, float p, int seed, int offset, int bh_offset=0, "
         "bool on_device=False) -> Tensor", philox_dropout_mask);
   m.def("check_status() -> ()", check_status);
@@ -1236,6 +1475,9 @@ TORCH_LIBRARY_IMPL(mha_manual, CUDA, m) {
   m.impl("fmha_qkvpacked_bwd", fmha_qkvpacked_bwd);
   m.impl("fmha_varlen_qkvpacked_fwd", fmha_varlen_qkvpacked_fwd);
   m.impl("fmha_varlen_qkvpacked_bwd", fmha_varlen_qkvpacked_bwd);
+  m.impl("kv_append", kv_append);
+  m.impl("kv_read", kv_read);
+  m.impl("fmha_paged_fwd", fmha_paged_fwd);
   m.impl("fmha_causal_varlen_fwd", fmha_causal_varlen_fwd);
   m.impl("fmha_causal_varlen_bwd", fmha_causal_varlen_bwd);
   m.impl("fmha_causal_varlen", fmha_causal_varlen_noautograd);
@@ -1257,6 +1499,9 @@ TORCH_LIBRARY_IMPL(mha_manual, Meta, m) {
   m.impl("fmha_qkvpacked_bwd", fmha_qkvpacked_bwd_meta);
   m.impl("fmha_varlen_qkvpacked_fwd", fmha_varlen_qkvpacked_fwd_meta);
   m.impl("fmha_varlen_qkvpacked_bwd", fmha_varlen_qkvpacked_bwd_meta);
+  m.impl("kv_append", kv_append_meta);
+  m.impl("kv_read", kv_read_meta);
+  m.impl("fmha_paged_fwd", fmha_paged_fwd_meta);
   m.impl("fmha_causal_varlen_fwd", fmha_causal_varlen_fwd_meta);
   m.impl("fmha_causal_varlen_bwd", fmha_causal_varlen_bwd_meta);
   m.impl("fmha_causal_varlen", fmha_causal_varlen_noautograd);
