@@ -310,8 +310,8 @@ int fmha_sm100_causal_fwd(const fmha_causal_fwd_params* p, void* stream);
 int fmha_sm100_causal_bwd(const fmha_causal_bwd_params* p, void* stream);
 int fmha_sm100_causal_bwd_workspace_bytes(const fmha_causal_bwd_params* p, size_t* bytes);
 
-/* Paged caches: appending rows, reading rows back, attention of a few new rows.  fmha_sm100_paged_workspace_bytes may give 0 (the keys of a
-   sequence are not dealt out over CTAs then); it depends on the sizes and on the current device. */
+/* Paged caches: appending rows, reading rows back, attention of a few new rows.  fmha_sm100_paged_workspace_bytes may give 0 (no sequence's
+   keys are dealt out over CTAs then); it depends on the sizes and on the current device. */
 int fmha_sm100_kv_append(const fmha_kv_append_params* p, void* stream);
 int fmha_sm100_kv_read(const fmha_kv_read_params* p, void* stream);
 int fmha_sm100_paged_fwd(const fmha_paged_params* p, void* stream);

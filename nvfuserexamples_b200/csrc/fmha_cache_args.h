@@ -11,8 +11,6 @@ namespace fmha {
 
 constexpr int kCacheGroup = 32;            // values of a row that share a scale and a base in a 4-bit cache
 constexpr float kCacheLimit = 20000.0f;    // what a 4-bit cache holds at most: scale <= 42 667 and base >= -62 667 then fit fp16
-constexpr int kPagedKeyStep = 64;          // keys per step of the paged attention kernel
-constexpr int kPagedRows = 16;             // query rows of one of its tiles
 constexpr int kMaxPageRows = 1 << 16;
 
 struct KvAppendArgs {
@@ -50,16 +48,25 @@ struct PagedArgs {
   const int* seqlens;
   const int* cu;     // null: rows_each rows a sequence
   int B, H, H_kv, group, total_rows, rows_each, max_rows;
-  int n_split;       // CTAs that may share a sequence's keys
+  int tile_rows, row_tiles, whole, ctas;   // PagedGrid
   float scale_log2;
-  float* part_o;     // [total_rows * H, n_split, D] unnormalised shares of O, when n_split > 1
-  float2* part_ml;   // [total_rows * H, n_split] their maximum (log2 domain) and sum
+  float* part_o;     // [ctas, 2, tile_rows, D] unnormalised O of pieces of units
+  float2* part_ml;   // [ctas, 2, tile_rows] their maximum (log2 domain) and sum
+  int2* part_info;   // [ctas] the unit that a CTA begins in the middle of, or -1; the place of its last part, if that is not its unit's end
   int* status;
 };
 
 int launch_kv_append(const KvAppendArgs& a, int dtype, bool interleaved, cudaStream_t stream);
 int launch_kv_read(const KvReadArgs& a, int dtype, cudaStream_t stream);
-int paged_splits(int64_t sms, int64_t tiles, int64_t max_keys, int D, int bits);   // n_split for these sizes
+struct PagedGrid {
+  int tile_rows;       // (new row, head of the group) pairs of a tile: 8 or 16
+  int64_t row_tiles;   // that max_rows new rows make
+  bool whole;          // no unit is cut
+  int ctas;
+};
+PagedGrid paged_grid(int64_t sms, int64_t max_rows, int64_t group, int64_t heads, int64_t max_keys);   // heads: key heads of all sequences
+size_t paged_workspace(const PagedGrid& g, int D);
+void paged_places(PagedArgs& a, void* workspace, const PagedGrid& g, int D);   // lays the workspace out
 int launch_paged(const PagedArgs& a, int dtype, int D, int bits, cudaStream_t stream);
 
 #ifdef __CUDACC__

@@ -86,16 +86,14 @@ static int validate_paged(const fmha_paged_params* p) {
   if (rc != FMHA_OK) return rc;
   if (p->H % p->cache.H_kv != 0) return FMHA_ERR_BAD_ARG;
   if (!(p->scale > 0.f) || !std::isfinite(p->scale)) return FMHA_ERR_BAD_ARG;
-  const int64_t tiles = (static_cast<int64_t>(p->max_rows) * (p->H / p->cache.H_kv) + kPagedRows - 1) / kPagedRows;
-  if (p->H > 65535 || tiles * p->cache.H_kv > 65535 || static_cast<int64_t>(p->total_rows) * p->H > 0x7fffffffll) return FMHA_ERR_TOO_LARGE;
+  // units are counted in 32 bits
+  const int64_t tiles = (static_cast<int64_t>(p->max_rows) * (p->H / p->cache.H_kv) + 7) / 8;
+  if (p->H > 65535 || tiles * p->cache.H_kv > (1 << 20) || tiles * p->cache.H_kv * p->B > 0x7fffffffll) return FMHA_ERR_TOO_LARGE;
   return FMHA_OK;
 }
-static int paged_n_split(const fmha_paged_params* p) {
-  const int64_t tiles = (static_cast<int64_t>(p->max_rows) * (p->H / p->cache.H_kv) + kPagedRows - 1) / kPagedRows * p->cache.H_kv * p->B;
-  return paged_splits(sm_count(), tiles, static_cast<int64_t>(p->cache.table_width) * p->cache.page_rows, p->cache.D, p->cache.bits);
-}
-static size_t share_bytes(const fmha_paged_params* p, int n_split) {   // of O; maxima and sums follow
-  return static_cast<size_t>(p->total_rows) * p->H * n_split * p->cache.D * sizeof(float);
+static PagedGrid grid_of(const fmha_paged_params* p) {
+  return paged_grid(sm_count(), p->max_rows, p->H / p->cache.H_kv, static_cast<int64_t>(p->cache.H_kv) * p->B,
+                    static_cast<int64_t>(p->cache.table_width) * p->cache.page_rows);
 }
 
 }  // namespace fmha
@@ -151,8 +149,7 @@ int fmha_sm100_paged_workspace_bytes(const fmha_paged_params* p, size_t* bytes) 
   if (bytes == nullptr) return FMHA_ERR_BAD_ARG;
   const int rc = validate_paged(p);
   if (rc != FMHA_OK) return rc;
-  const int n = paged_n_split(p);
-  *bytes = n > 1 ? share_bytes(p, n) + static_cast<size_t>(p->total_rows) * p->H * n * sizeof(float2) : 0;
+  *bytes = paged_workspace(grid_of(p), p->cache.D);
   return FMHA_OK;
 }
 
@@ -167,14 +164,13 @@ int fmha_sm100_paged_fwd(const fmha_paged_params* p, void* stream) {
   if (!rows_ok(p->q, p->H) || !rows_ok(p->o, p->H) || c.pages == 0) return FMHA_ERR_BAD_ARG;
   rc = check_device();
   if (rc != FMHA_OK) return rc;
-  a.n_split = paged_n_split(p);
-  const size_t shares = share_bytes(p, a.n_split), need = a.n_split > 1 ? shares + static_cast<size_t>(p->total_rows) * p->H * a.n_split * sizeof(float2) : 0;
+  const PagedGrid grid = grid_of(p);
+  const size_t need = paged_workspace(grid, c.D);
   if (need > 0 && (p->workspace == nullptr || p->workspace_bytes < need || (reinterpret_cast<uintptr_t>(p->workspace) & 255))) return FMHA_ERR_BAD_ARG;
-  a.part_o = static_cast<float*>(p->workspace);
-  a.part_ml = need > 0 ? reinterpret_cast<float2*>(static_cast<uint8_t*>(p->workspace) + shares) : nullptr;
+  paged_places(a, p->workspace, grid, c.D);
   a.piece = c.page_rows % 64 == 0 ? 64 : c.page_rows % 32 == 0 ? 32 : 16;
   if (c.bits == 4) {
-    const CUtensorMapSwizzle sw = c.D == 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_NONE;
+    const CUtensorMapSwizzle sw = c.D == 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B;   // that of a row's length
     if ((rc = map_rows(&a.tm_k, c.k, c, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, c.D / 2, c.D / 2, a.piece, sw))) return rc;
     if ((rc = map_rows(&a.tm_v, c.v, c, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, c.D / 2, c.D / 2, a.piece, sw))) return rc;
     if ((rc = map_params(&a.tm_kp, c.k_params, c, a.piece))) return rc;

@@ -1,18 +1,26 @@
 // fmha_paged_sm100.cu — attention of a few new rows per sequence over all its rows in a paged cache, held in 16 or 4 bits ("decode").
 //
-// Bound by bringing the cache in: a key row is used by the T x group query rows of its head, 4 flops per byte and row in 16 bits.  As in
-// fmha_fwd_rows_sm100.cu, m16n8k16 MMAs from registers fit the row count, each of four consumer warps takes 16 of every 64 keys with a running
-// softmax of its own, and a producer warp keeps several steps in flight through TMA, a copy per page (or per 64 rows of one).  The query rows of a
-// tile are the group's heads of consecutive new rows, so K and V are read once for all of them.  A page number outside the cache is a coordinate
-// outside the tensor map, which TMA fills with zeros.
+// Bound by bringing the cache in: a key row is used by the T x group query rows of its head, 4 flops per byte and row in 16 bits.  Four consumer warps
+// take their own keys of a step, each with a running softmax of its own; a producer warp keeps several steps in flight through TMA, a copy per page (or
+// per 64 rows of one).  The query rows of a tile are the group's heads of consecutive new rows, so K and V are read once for all of them.  A page
+// number outside the cache is a coordinate outside the tensor map, which TMA fills with zeros.
 //
-// The keys of a sequence are dealt out over CTAs (splits_of) by its own length, which only the device knows; each leaves its unnormalised O, maximum and
-// sum in the workspace, and a second kernel joins them.  Where a sequence has one share, its CTA writes the result itself.
+// Products.  m16n8k16 MMAs from registers with the cache as the operand of 16 rows: S^T = K Q^T and O^T = V^T P^T, so that 8 query rows (a group of
+// heads and one new row, as a rule) cost half of what a tile of 16 would, and the accumulators half of the registers; 9 to 16 rows take two such columns.  P^T
+// comes out of the first product with keys along the rows and goes into the second with keys along the pairs: an 8 x 8 transposition per 8 keys.
 //
-// 4 bits: a thread takes eight codes from a word as four pairs of halves: a code in the low bits of the half 1024 is 1024 + c, one in bits 4 to 7 of the half
-// 64 is 64 + c; minus 1024 or 64 that is c, exactly, and b + s + (s / 16) c is one fused multiply-add.  The dimensions of K are permuted in the
-// MMA's contraction, and those of V over its columns, so that a word's codes are one thread's operands; keys keep their order, in which P comes out of
-// the first MMA.
+// Work.  A unit is (8 or 16 query rows, key head, sequence), its weight its key steps, which only the device knows.  The units stand in one line, and each
+// CTA takes an equal piece of it, cutting through units where that falls: all CTAs are busy to the end whatever the lengths are, and there is no bubble
+// between units, for the producer goes on to the next one.  A CTA that has a unit from its first to its last step writes the result; a piece of one
+// goes to the workspace (at most two of a CTA), and a second kernel joins the pieces of the units that were cut.
+//
+// 4 bits: b + s (1 + c/16).  Codes are operands of the MMA as they are: four bits at the bottom of a half are the subnormal c 2^-24, those above it c 2^-20, and
+// tensor cores take subnormals.  A word of codes thus costs four ANDs and a shift for four pairs.  K: the sums over the 32 dimensions that share a
+// scale (the query's even values are taken 16-fold) are multiplied by it in 32 bits; what does not depend on codes, the sum of (b + s) times the query's
+// values, is one more MMA of the scales and bases as they lie in memory against those values' sums (in two parts of 11 bits).  So scores are as exact
+// as 32 bits allow.  V: P is multiplied by the key's scale of each 32 dimensions, the product with the codes is scaled at the end, and the sum of P (b + s)
+// is one more MMA of the transposed scales and bases.  The row maximum is kept exactly here (16 bits: up to 2^8), for P times a scale of up to 65 504 has to fit
+// fp16.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -29,44 +37,49 @@ namespace fmha {
 
 namespace {
 
-constexpr int kPgWarps = 4;   // consumer warps, 16 keys of a step each
+constexpr int kPgWarps = 4;   // consumer warps
 constexpr int kPgThreads = 32 * (kPgWarps + 1);
-constexpr int kPgMinSteps = 4;   // key steps of a share
+constexpr int kPgMinKeys = 256;   // a CTA's piece of the line holds at least so many
 constexpr float kPgLn2 = 0.6931471805599453f;
 
 enum PgWaitSite { kPgFull = 191, kPgEmpty = 192 };
 
-template <int D, bool FOUR>
+// NQ: columns of 8 query rows.
+template <int D, bool FOUR, int NQ>
 struct PgSmem {
+  static constexpr int kUnits = FOUR ? 2 : 1;                  // 16-key blocks of a warp's share of a step
+  static constexpr int kKeys = kPgWarps * 16 * kUnits;         // keys of a step
   static constexpr int kRowBytes = FOUR ? D / 2 : D * 2;
   static constexpr int kParBytes = FOUR ? D / kCacheGroup * 4 : 0;
-  static constexpr int kTile = kPagedKeyStep * kRowBytes;      // K or V of a step
-  static constexpr int kParTile = kPagedKeyStep * kParBytes;   // its scales and bases
-  static constexpr int kSub = kPagedKeyStep * 128;             // 16 bits: a 64-column sub-tile (128-byte swizzle)
+  static constexpr int kTile = kKeys * kRowBytes;              // K or V of a step
+  static constexpr int kParTile = kKeys * kParBytes;           // its scales and bases
+  static constexpr int kSub = kKeys * 128;                     // 16 bits: a 64-column sub-tile (128-byte swizzle)
   static constexpr int kStage = 2 * (kTile + kParTile);        // K, V, parameters of K, of V
-  static constexpr int kStages = FOUR ? (D == 128 ? 8 : 12) : D == 128 ? 3 : 6;
-  static constexpr int kOffBar = kStages * kStage;
+  static constexpr int kStages = FOUR ? (D == 128 ? 4 : 7) : D == 128 ? 3 : 6;
+  // O of the four warps on its way to be added up, kRows rows at a time ([D + 4] fp32 each: rows 2t of a store lie 8 banks apart), and statistics
+  static constexpr int kRows = D == 128 && !FOUR ? 4 : 8;
+  static constexpr int kRowFloats = D + 4;
+  static constexpr int kShare = kRows * kRowFloats * 4;
+  static constexpr int kOffShare = kStages * kStage;
+  static constexpr int kOffStats = kOffShare + kPgWarps * kShare;
+  static constexpr int kOffBar = kOffStats + kPgWarps * 8 * NQ * 8;
   static constexpr int kOffMisc = kOffBar + 2 * kStages * 8;
   static constexpr int kDynBytes = kOffMisc + 16 + 1024;
-  // after the key loop, over the stages: O of the four warps, [16][D + 8] fp32 each, and their row statistics
-  static constexpr int kRowFloats = D + 8;
-  static constexpr int kShare = kPagedRows * kRowFloats * 4;
-  static constexpr int kOffStats = kPgWarps * kShare;
-  static_assert(kOffStats + kPgWarps * kPagedRows * 8 <= kOffBar, "the shares fit over the stages");
-  static_assert(kStage % 1024 == 0 || FOUR, "swizzled tiles begin at multiples of 1024 bytes");
-  static_assert(kStage % 512 == 0, "and those of 64-byte rows at multiples of 512");
+  static_assert(2 * (kDynBytes + 1024) <= 233472, "two CTAs share an SM");
+  static_assert(kStage % 1024 == 0 || (FOUR && kStage % 512 == 0), "swizzled tiles begin at multiples of 1024 bytes (64-byte rows: 512)");
 };
 
+// D = A B + C
 template <bool BF16>
-__device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]) {
   if constexpr (BF16)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
   else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
 template <bool TRANS>
 __device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t saddr) {
@@ -77,46 +90,39 @@ __device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t saddr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(saddr) : "memory");
 }
+template <bool TRANS>
+__device__ __forceinline__ void ldmatrix_x2(uint32_t& r0, uint32_t& r1, uint32_t saddr) {
+  if constexpr (TRANS) asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0, %1}, [%2];" : "=r"(r0), "=r"(r1) : "r"(saddr) : "memory");
+  else asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0, %1}, [%2];" : "=r"(r0), "=r"(r1) : "r"(saddr) : "memory");
+}
+// Lane (g, t) holds elements (g, 2t) and (g, 2t + 1) of an 8 x 8 matrix: afterwards (2t, g) and (2t + 1, g).
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
+  uint32_t d;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(x));
+  return d;
+}
 __device__ __forceinline__ uint32_t lds32(uint32_t saddr) {
   uint32_t v;
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(saddr));
   return v;
 }
-__device__ __forceinline__ uint32_t hadd2(uint32_t a, uint32_t b) {
-  uint32_t d;
-  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-  return d;
+__device__ __forceinline__ uint2 lds64(uint32_t saddr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(saddr));
+  return v;
 }
 __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
   uint32_t d;
   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
 }
-__device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
-  uint32_t d;
-  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
-  return d;
-}
-// (w & mask) | magic, one instruction
-__device__ __forceinline__ uint32_t mask_or(uint32_t w, uint32_t mask, uint32_t magic) {
-  uint32_t d;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(w), "r"(mask), "r"(magic));
-  return d;
-}
-// The values of a word's eight codes as four pairs: pair j holds codes j (low half) and j + 4.  step = s / 16 and first = b + s of either half.
-__device__ __forceinline__ void values4(uint32_t w, uint32_t step, uint32_t first, uint32_t (&v)[4]) {
-  const uint32_t w8 = w >> 8;
-  v[0] = hfma2(hadd2(mask_or(w, 0x000F000Fu, 0x64006400u), 0xE400E400u), step, first);
-  v[1] = hfma2(hadd2(mask_or(w, 0x00F000F0u, 0x54005400u), 0xD400D400u), step, first);
-  v[2] = hfma2(hadd2(mask_or(w8, 0x000F000Fu, 0x64006400u), 0xE400E400u), step, first);
-  v[3] = hfma2(hadd2(mask_or(w8, 0x00F000F0u, 0x54005400u), 0xD400D400u), step, first);
-}
-// Two finite 16-bit values of the query type as halves that stay finite.
-template <bool BF16>
-__device__ __forceinline__ uint32_t to_half2(uint32_t w) {
-  if constexpr (!BF16) return w;
-  auto clamp = [](float x) { return fabsf(x) < INFINITY ? fminf(fmaxf(x, -65504.f), 65504.f) : x; };
-  return pack2<false>(clamp(unpack_lo<true>(w)), clamp(unpack_hi<true>(w)));
+// The eight codes of a word, or four codes of either of two keys, as pairs of subnormal halves: codes 0 and 4 (times 2^-24), 1 and 5 (2^-20), 2 and 6
+// (2^-24), 3 and 7 (2^-20).
+__device__ __forceinline__ void code_pairs(uint32_t w, uint32_t (&v)[4]) {
+  v[0] = w & 0x000F000Fu;
+  v[1] = w & 0x00F000F0u;
+  v[2] = (w >> 8) & 0x000F000Fu;
+  v[3] = (w >> 8) & 0x00F000F0u;
 }
 
 // A sequence: its new rows and its keys.
@@ -141,58 +147,122 @@ __device__ __forceinline__ int keys_of(const PagedArgs& a, const PgSeq& s, int r
   const int64_t most = static_cast<int64_t>(a.table_width) * a.page_rows;
   return static_cast<int>(max(min(static_cast<int64_t>(s.len) - s.n_all + row + 1, most), static_cast<int64_t>(0)));
 }
-// Over how many CTAs the keys of a tile are dealt out: by their number alone, so that both kernels find the same.
-__device__ __forceinline__ int splits_of(int keys, int n_split) {
-  const int steps = (keys + kPagedKeyStep - 1) / kPagedKeyStep;
-  return max(1, min(n_split, steps / kPgMinSteps));
+// A group of units: the key heads of a tile of query rows.
+struct PgGroup {
+  int n_rows, k_limit, steps, weight;   // rows that exist; keys that the last of them sees; what a unit of it counts in the line
+};
+__device__ __forceinline__ PgGroup group_of(const PagedArgs& a, int b, int tile, int keys) {
+  PgGroup u = {0, 0, 0, 0};
+  const PgSeq s = sequence(a, b);
+  const int r0 = tile * a.tile_rows;
+  u.n_rows = min(a.tile_rows, s.n_new * a.group - r0);
+  if (u.n_rows <= 0) return u;
+  u.k_limit = keys_of(a, s, (r0 + u.n_rows - 1) / a.group);
+  u.steps = (u.k_limit + keys - 1) / keys;
+  u.weight = a.whole ? 1 : max(1, u.steps);   // rows that see no key are written as well
+  return u;
+}
+
+// A CTA's way along the line, the same in each of its warps: its piece of a unit, then the next.
+struct PgWay {
+  int tiles, groups;   // row tiles of a sequence, groups in all
+  int g, b, tile, hk;  // the unit
+  PgGroup u;
+  int j0, j1;          // its steps
+  int left, n;         // of the CTA's piece of the line, this part included; how many parts came before
+  bool first, last;    // the part holds the unit's first step, its last one
+};
+template <int KEYS>
+__device__ __forceinline__ void way_part(const PagedArgs& a, PgWay& w, int off) {
+  const int take = min(w.u.weight - off, w.left);
+  w.first = off == 0;
+  w.last = off + take == w.u.weight;
+  w.j0 = a.whole ? 0 : min(off, w.u.steps);
+  w.j1 = a.whole ? w.u.steps : min(off + take, w.u.steps);
+  w.left -= take;
+}
+// False: nothing for this CTA.
+template <int KEYS>
+__device__ __forceinline__ bool way_begin(const PagedArgs& a, PgWay& w) {
+  const int lane = threadIdx.x & 31;
+  w.tiles = a.row_tiles;
+  w.groups = a.B * w.tiles;
+  long long total = 0;
+  int mine = 0;   // weight of the lane's group among the first 32
+  for (int g0 = 0; g0 < w.groups; g0 += 32) {
+    const int g = g0 + lane, x = g < w.groups ? group_of(a, g / w.tiles, g % w.tiles, KEYS).weight : 0;
+    if (g0 == 0) mine = x;
+    total += __reduce_add_sync(0xffffffffu, x);
+  }
+  total *= a.H_kv;
+  const long long least = a.whole ? 1 : kPgMinKeys / KEYS;
+  const long long chunk = max(least, (total + gridDim.x - 1) / gridDim.x);
+  const long long w0 = chunk * blockIdx.x;
+  if (w0 >= total) return false;
+  w.left = static_cast<int>(min(chunk, total - w0));
+  long long before = 0;   // of the groups passed
+  for (int g0 = 0;; g0 += 32) {
+    const int g = g0 + lane, x = g0 == 0 ? mine : g < w.groups ? group_of(a, g / w.tiles, g % w.tiles, KEYS).weight : 0;
+    int sum = x;   // inclusive
+#pragma unroll
+    for (int m = 1; m < 32; m *= 2) {
+      const int y = __shfl_up_sync(0xffffffffu, sum, m);
+      if (lane >= m) sum += y;
+    }
+    const uint32_t beyond = __ballot_sync(0xffffffffu, (before + sum) * a.H_kv > w0);
+    if (beyond != 0u) {
+      const int at = __ffs(beyond) - 1;
+      w.g = g0 + at;
+      before += __shfl_sync(0xffffffffu, sum - x, at);
+      break;
+    }
+    before += __shfl_sync(0xffffffffu, sum, 31);
+  }
+  w.b = w.g / w.tiles;
+  w.tile = w.g % w.tiles;
+  w.u = group_of(a, w.b, w.tile, KEYS);
+  const int within = static_cast<int>(w0 - before * a.H_kv);
+  w.hk = within / w.u.weight;
+  w.n = 0;
+  way_part<KEYS>(a, w, within % w.u.weight);
+  return true;
+}
+template <int KEYS>
+__device__ __forceinline__ bool way_next(const PagedArgs& a, PgWay& w) {
+  if (w.left == 0) return false;
+  ++w.n;
+  if (++w.hk == a.H_kv) {
+    w.hk = 0;
+    do {
+      ++w.g;
+      if (++w.tile == w.tiles) {
+        w.tile = 0;
+        ++w.b;
+      }
+      w.u = group_of(a, w.b, w.tile, KEYS);
+    } while (w.u.weight == 0);
+  }
+  way_part<KEYS>(a, w, 0);
+  return true;
 }
 
 }  // namespace
 
-template <int D, bool BF16, bool FOUR>
+template <int D, bool BF16, bool FOUR, int NQ>
 __global__ void __launch_bounds__(kPgThreads, 2) fmha_paged_kernel(const __grid_constant__ PagedArgs a) {
   griddep_wait();
-  using L = PgSmem<D, FOUR>;
-  constexpr int ST = L::kStages;
+  using L = PgSmem<D, FOUR, NQ>;
+  constexpr int ST = L::kStages, UN = L::kUnits, KEYS = L::kKeys, ROWS = 8 * NQ;
   constexpr bool MMA_BF16 = BF16 && !FOUR;
+  constexpr float kLazy = FOUR ? 0.f : 8.f;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kOffBar);   // [ST] a step has landed
   uint64_t* empty = full + ST;                                       // [ST] ... and the four consumer warps are done with it
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kOffMisc);
   const WaitCtx wctx{abort_flag, a.status};
-
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const int split = blockIdx.x, hk = blockIdx.y % a.H_kv, tile = blockIdx.y / a.H_kv, b = blockIdx.z;
-  const PgSeq seq = sequence(a, b);
-
-  // Rows that no tile of the grid stands for: outside the sequences, or past max_rows of theirs.
-  if (split == 0 && tile == 0) {
-    auto zero = [&](int64_t from, int64_t to, int h0, int h1) {
-      from = max(from, static_cast<int64_t>(0));
-      to = min(to, static_cast<int64_t>(a.total_rows));
-      const int per_row = (h1 - h0) * (D / 8);
-      for (int64_t i = threadIdx.x; i < (to - from) * per_row; i += kPgThreads) {
-        const int64_t row = from + i / per_row;
-        const int h = h0 + static_cast<int>(i % per_row) / (D / 8), ch = static_cast<int>(i % (D / 8));
-        *reinterpret_cast<uint4*>(static_cast<unsigned short*>(a.o_ptr) + row * a.o_ss + h * a.o_sh + ch * 8) = make_uint4(0u, 0u, 0u, 0u);
-        if (ch == 0 && a.lse != nullptr) a.lse[static_cast<int64_t>(h) * a.total_rows + row] = -INFINITY;
-      }
-    };
-    const int h0 = hk * a.group, h1 = h0 + a.group;
-    if (seq.n_all > a.max_rows) zero(static_cast<int64_t>(seq.row0) + a.max_rows, static_cast<int64_t>(seq.row0) + seq.n_all, h0, h1);
-    if (b == 0) zero(0, seq.row0, h0, h1);
-    if (b == a.B - 1) zero(static_cast<int64_t>(seq.row0) + max(seq.n_all, 0), a.total_rows, h0, h1);
-  }
-  const int r0 = tile * kPagedRows;                                  // row r of the head's (new row, head of the group) pairs
-  const int n_rows = min(kPagedRows, seq.n_new * a.group - r0);
-  if (n_rows <= 0) return;
-  const int k_limit = keys_of(a, seq, (r0 + n_rows - 1) / a.group);  // of the tile's last row
-  const int n_split = splits_of(k_limit, a.n_split);
-  if (split >= n_split) return;
-  const int n_steps = (k_limit + kPagedKeyStep - 1) / kPagedKeyStep;
-  const int j0 = static_cast<int>(static_cast<int64_t>(n_steps) * split / n_split), j1 = static_cast<int>(static_cast<int64_t>(n_steps) * (split + 1) / n_split);
 
   if (threadIdx.x == 0) {
     *abort_flag = 0;
@@ -202,386 +272,566 @@ __global__ void __launch_bounds__(kPgThreads, 2) fmha_paged_kernel(const __grid_
     }
     mbar_fence_init();
   }
+  // Rows that no unit stands for: outside the sequences, or past max_rows of theirs.
+  {
+    auto zero = [&](int64_t from, int64_t to) {
+      from = max(from, static_cast<int64_t>(0));
+      to = min(to, static_cast<int64_t>(a.total_rows));
+      const int per_row = a.H * (D / 8);
+      for (int64_t i = threadIdx.x; i < (to - from) * per_row; i += kPgThreads) {
+        const int64_t row = from + i / per_row;
+        const int h = static_cast<int>(i % per_row) / (D / 8), ch = static_cast<int>(i % (D / 8));
+        *reinterpret_cast<uint4*>(static_cast<unsigned short*>(a.o_ptr) + row * a.o_ss + h * a.o_sh + ch * 8) = make_uint4(0u, 0u, 0u, 0u);
+        if (ch == 0 && a.lse != nullptr) a.lse[static_cast<int64_t>(h) * a.total_rows + row] = -INFINITY;
+      }
+    };
+    if (a.cu != nullptr) {
+      for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
+        const int64_t from = a.cu[b], to = a.cu[b + 1];
+        if (to - from > a.max_rows) zero(from + a.max_rows, to);
+        if (b == 0) zero(0, from);
+        if (b == a.B - 1) zero(max(from, to), a.total_rows);
+      }
+    }
+  }
+  PgWay w;
+  const bool any = way_begin<KEYS>(a, w);
+  // What the second kernel needs to know: the unit that this CTA begins in the middle of, and which of its two places its last part is in.
+  if (threadIdx.x == 0 && a.part_info != nullptr) a.part_info[blockIdx.x] = make_int2(any && !w.first ? w.g * a.H_kv + w.hk : -1, -1);
   __syncthreads();
-
-  const int g = lane >> 2, t = lane & 3;   // this thread's MMA rows are g and g + 8
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-  float o[D / 8][4];
-#pragma unroll
-  for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  if (!any) return;
 
   if (warp == kPgWarps) {
     // ============================ TMA producer ======================================
     // Lane i brings piece i of the step: the page number of the next step is read while this one's buffers are waited for.
-    const int pieces = kPagedKeyStep / a.piece;   // 1, 2 or 4
-    const int* line = a.table + b * a.table_stride;
-    auto page_of = [&](int j) {
-      const int key = j * kPagedKeyStep + lane * a.piece;
-      return lane < pieces && key < k_limit ? line[key / a.page_rows] : -1;   // rows behind the last key: zeros
-    };
-    int page = j0 < j1 ? page_of(j0) : -1;
-    for (int j = j0; j < j1; ++j) {
-      const int i = j - j0, s = i % ST;
-      const int now = page;
-      if (j + 1 < j1) page = page_of(j + 1);
-      if (lane == 0) {
-        if (i >= ST) mbar_wait(empty + s, (i / ST - 1) & 1, wctx, kPgEmpty);
-        mbar_arrive_expect_tx(full + s, L::kStage);
-      }
-      __syncwarp();
-      if (lane < pieces) {
-        uint8_t* k = smem + s * L::kStage;
-        uint8_t* v = k + L::kTile;
-        const int at = lane * a.piece, row = (j * kPagedKeyStep + at) % a.page_rows;
-        const int pg = now < 0 ? a.pages : now;   // (a negative one is outside as well)
-        if constexpr (FOUR) {
-          tma_load_4d(k + at * L::kRowBytes, &a.tm_k, full + s, 0, row, hk, pg);
-          tma_load_4d(v + at * L::kRowBytes, &a.tm_v, full + s, 0, row, hk, pg);
-          uint8_t* par = v + L::kTile + at * L::kParBytes;
-          tma_load_3d(par, &a.tm_kp, full + s, row * (D / kCacheGroup), hk, pg);
-          tma_load_3d(par + L::kParTile, &a.tm_vp, full + s, row * (D / kCacheGroup), hk, pg);
-        } else {
-#pragma unroll
-          for (int c = 0; c < D / 64; ++c) tma_load_4d(k + c * L::kSub + at * 128, &a.tm_k, full + s, c * 64, row, hk, pg);
-#pragma unroll
-          for (int c = 0; c < D / 64; ++c) tma_load_4d(v + c * L::kSub + at * 128, &a.tm_v, full + s, c * 64, row, hk, pg);
+    const int pieces = KEYS / a.piece;   // up to 8
+    int i = 0;
+    do {
+      const int* line = a.table + w.b * a.table_stride;
+      const int k_limit = w.u.k_limit, hk = w.hk;
+      auto page_of = [&](int j) {
+        const int key = j * KEYS + lane * a.piece;
+        return lane < pieces && key < k_limit ? line[key / a.page_rows] : -1;   // rows behind the last key: zeros
+      };
+      int page = w.j0 < w.j1 ? page_of(w.j0) : -1;
+      for (int j = w.j0; j < w.j1; ++j, ++i) {
+        const int s = i % ST;
+        const int now = page;
+        if (j + 1 < w.j1) page = page_of(j + 1);
+        if (lane == 0) {
+          if (i >= ST) mbar_wait(empty + s, (i / ST - 1) & 1, wctx, kPgEmpty);
+          mbar_arrive_expect_tx(full + s, L::kStage);
         }
+        __syncwarp();
+        if (lane < pieces) {
+          uint8_t* k = smem + s * L::kStage;
+          uint8_t* v = k + L::kTile;
+          const int at = lane * a.piece, row = (j * KEYS + at) % a.page_rows;
+          const int pg = now < 0 ? a.pages : now;   // (a negative one is outside as well)
+          if constexpr (FOUR) {
+            tma_load_4d(k + at * L::kRowBytes, &a.tm_k, full + s, 0, row, hk, pg);
+            tma_load_4d(v + at * L::kRowBytes, &a.tm_v, full + s, 0, row, hk, pg);
+            uint8_t* par = v + L::kTile + at * L::kParBytes;
+            tma_load_3d(par, &a.tm_kp, full + s, row * (D / kCacheGroup), hk, pg);
+            tma_load_3d(par + L::kParTile, &a.tm_vp, full + s, row * (D / kCacheGroup), hk, pg);
+          } else {
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c) tma_load_4d(k + c * L::kSub + at * 128, &a.tm_k, full + s, c * 64, row, hk, pg);
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c) tma_load_4d(v + c * L::kSub + at * 128, &a.tm_v, full + s, c * 64, row, hk, pg);
+          }
+        }
+        __syncwarp();
       }
-      __syncwarp();
-    }
+    } while (way_next<KEYS>(a, w));
   } else {
     // ============================ consumers =========================================
-    // Q fragments of the 16 rows (rows that do not exist are zeros), and the keys that rows g and g + 8 see
-    uint32_t qf[D / 16][4];
-    int limit[2];
+    const int g = lane >> 2, t = lane & 3;   // this thread's MMA rows are g and g + 8, its columns (query rows) 2t and 2t + 1
+    const int tid = threadIdx.x;
+    float* share = reinterpret_cast<float*>(smem + L::kOffShare);
+    float2* stats = reinterpret_cast<float2*>(smem + L::kOffStats);   // [4][ROWS] (maximum, sum)
+    const int mi = lane >> 3, r8 = lane & 7;   // ldmatrix: lane (mi, r8) addresses row r8 of 8x8 block mi
+    int i = 0;   // steps so far
+    do {
+      const PgSeq seq = sequence(a, w.b);
+      const int r0 = w.tile * ROWS, n_rows = w.u.n_rows, k_limit = w.u.k_limit;
+      const int lim_min = keys_of(a, seq, r0 / a.group);   // all rows see the keys before it
+      // ---- Q^T: column n of k-step ks is query row n; the keys that rows 2t and 2t + 1 see ----
+      uint32_t qf[NQ][D / 16][2];
+      int limit[NQ][2];
+      float sl2[NQ][2];
+      [[maybe_unused]] uint32_t af[NQ][2];   // the row's sums over the groups of 32 dimensions, twice: high and low part
 #pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
-      const int r = r0 + g + hf * 8;
-      const bool exists = g + hf * 8 < n_rows;
-      const int row = r / a.group, h = hk * a.group + r % a.group;
-      limit[hf] = exists ? keys_of(a, seq, row) : 0;
-      const unsigned short* q = static_cast<const unsigned short*>(a.q_ptr) + static_cast<int64_t>(seq.row0 + row) * a.q_ss + h * a.q_sh;
-      if constexpr (FOUR) {
-        // thread t has the dimensions [t D/4, +D/4) of the contraction, eight (a word of codes) to two k-steps; pair j is (j, j + 4)
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-          uint4 w = make_uint4(0u, 0u, 0u, 0u);
-          if (exists) w = __ldg(reinterpret_cast<const uint4*>(q + t * (D / 4) + i * 8));
-          const uint32_t x = to_half2<BF16>(w.x), y = to_half2<BF16>(w.y), z = to_half2<BF16>(w.z), u = to_half2<BF16>(w.w);
-          qf[2 * i][hf] = prmt(x, z, 0x5410u);
-          qf[2 * i][2 + hf] = prmt(x, z, 0x7632u);
-          qf[2 * i + 1][hf] = prmt(y, u, 0x5410u);
-          qf[2 * i + 1][2 + hf] = prmt(y, u, 0x7632u);
-        }
-      } else {
-#pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks)
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-            qf[ks][e * 2 + hf] = exists ? __ldg(reinterpret_cast<const unsigned int*>(q + ks * 16 + e * 8 + 2 * t)) : 0u;
-      }
-    }
-    const float sl2 = a.scale_log2;
-    // 16 bits, ldmatrix: lane (mi, r) addresses row r of 8x8 block mi
-    const int mi = lane >> 3, r = lane & 7;
-    const int k_row = warp * 16 + (mi >> 1) * 8 + r, k_ch = mi & 1;
-    const int v_row = warp * 16 + (mi & 1) * 8 + r, v_ch = mi >> 1;
-
-    for (int j = j0; j < j1; ++j) {
-      const int i = j - j0, s = i % ST;
-      const int key0 = j * kPagedKeyStep + warp * 16;   // this warp's 16 keys
-      mbar_wait(full + s, (i / ST) & 1, wctx, kPgFull);
-      if (key0 < k_limit) {
-        const uint32_t sk = smem_u32(smem + s * L::kStage), sv = sk + L::kTile;
-        const bool whole = key0 + 16 <= k_limit;
-        float sc[2][4] = {};
+      for (int nq = 0; nq < NQ; ++nq) {
+        const int r = r0 + nq * 8 + g;
+        const bool exists = nq * 8 + g < n_rows;
+        const int row = r / a.group, h = w.hk * a.group + r % a.group;
+        const unsigned short* q = static_cast<const unsigned short*>(a.q_ptr) + static_cast<int64_t>(seq.row0 + row) * a.q_ss + h * a.q_sh;
+        float mul = a.scale_log2;
         if constexpr (FOUR) {
-          const uint32_t par = sv + L::kTile;
+          // thread t has dimensions 32 c + 8 t to + 7 of group c, one word of codes: two k-steps
+          uint4 x[D / 32];
+          float top = 0.f;
 #pragma unroll
-          for (int nt = 0; nt < 2; ++nt) {
-            const int key = warp * 16 + nt * 8 + g;
-            // thread t's D / 4 dimensions lie in one group of 32
-            const uint32_t sb = lds32(par + key * L::kParBytes + (D == 128 ? t : t >> 1) * 4);
-            const uint32_t ss = prmt(sb, sb, 0x1010u), bb = prmt(sb, sb, 0x3232u);
-            const uint32_t step = hmul2(ss, 0x2C002C00u), first = hadd2(bb, ss);   // s / 16, b + s
-            uint32_t w[D / 32];
-            if constexpr (D == 128) {
-              const uint4 x = lds128(sk + key * 64 + ((t ^ ((key >> 1) & 3)) << 4));   // 64-byte swizzle
-              w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
-            } else {
-              w[0] = lds32(sk + key * 32 + t * 8);
-              w[1] = lds32(sk + key * 32 + t * 8 + 4);
+          for (int c = 0; c < D / 32; ++c) {
+            x[c] = make_uint4(0u, 0u, 0u, 0u);
+            if (exists) x[c] = __ldg(reinterpret_cast<const uint4*>(q + c * 32 + t * 8));
+            const uint32_t ws[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) top = fmax3(top, fabsf(unpack_lo<BF16>(ws[e])), fabsf(unpack_hi<BF16>(ws[e])));
+          }
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          // Rows with values of 1024 and more are scaled down by a power of two, so that the sums of 32, and 16-fold values, fit fp16; the scores are scaled back.
+          const int e2 = top >= 1024.f && top < INFINITY ? ilogbf(top) - 9 : 0;
+          const float down = __int_as_float((127 - e2) << 23);
+          mul *= __int_as_float((127 + e2) << 23);
+          af[nq][0] = af[nq][1] = 0u;
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            const uint32_t ws[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
+            uint32_t hs[4];
+            float sum = 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              hs[e] = pack2<false>(unpack_lo<BF16>(ws[e]) * down, unpack_hi<BF16>(ws[e]) * down);
+              sum += unpack_lo<false>(hs[e]) + unpack_hi<false>(hs[e]);
             }
-#pragma unroll
-            for (int q = 0; q < D / 32; ++q) {
-              uint32_t v[4];
-              values4(w[q], step, first, v);
-              mma_16816<false>(sc[nt], qf[2 * q], v[0], v[1]);
-              mma_16816<false>(sc[nt], qf[2 * q + 1], v[2], v[3]);
+            // pairs (0, 4) and (2, 6) 16-fold, see code_pairs
+            qf[nq][2 * c][0] = hmul2(prmt(hs[0], hs[2], 0x5410u), 0x4C004C00u);
+            qf[nq][2 * c][1] = prmt(hs[0], hs[2], 0x7632u);
+            qf[nq][2 * c + 1][0] = hmul2(prmt(hs[1], hs[3], 0x5410u), 0x4C004C00u);
+            qf[nq][2 * c + 1][1] = prmt(hs[1], hs[3], 0x7632u);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            if (c == t) {
+              const float hi = unpack_lo<false>(pack2<false>(sum, 0.f));
+              af[nq][0] = pack2<false>(hi, hi);
+              af[nq][1] = pack2<false>(sum - hi, sum - hi);
             }
           }
         } else {
 #pragma unroll
-          for (int ks = 0; ks < D / 16; ++ks) {
-            uint32_t kf[4];
-            ldmatrix_x4<false>(kf, sk + (ks / 4) * L::kSub + sw128_offset(k_row, (ks % 4) * 2 + k_ch));
-            mma_16816<MMA_BF16>(sc[0], qf[ks], kf[0], kf[1]);
-            mma_16816<MMA_BF16>(sc[1], qf[ks], kf[2], kf[3]);
-          }
+          for (int ks = 0; ks < D / 16; ++ks)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              qf[nq][ks][e] = exists ? __ldg(reinterpret_cast<const unsigned int*>(q + ks * 16 + e * 8 + 2 * t)) : 0u;
         }
-        // scaled scores in the log2 domain
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float x = sc[nt][e] * sl2;
-            if (key0 + nt * 8 + 2 * t + (e & 1) >= limit[e >> 1]) x = -INFINITY;
-            sc[nt][e] = x;
-          }
-        uint32_t p[4];
-        float alpha[2];
-        bool moved = false;
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          float mx = fmaxf(fmaxf(sc[0][2 * hf], sc[0][2 * hf + 1]), fmaxf(sc[1][2 * hf], sc[1][2 * hf + 1]));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-          float m_new = fmaxf(m[hf], mx);
-          if (m[hf] != -INFINITY && m_new - m[hf] <= 8.0f) m_new = m[hf];   // lazy: exponentials stay below 2^8
-          alpha[hf] = m_new == m[hf] ? 1.0f : fast_exp2(m[hf] - m_new);
-          moved |= m_new != m[hf];
-          m[hf] = m_new;
-          const float neg_m = m_new == -INFINITY ? 0.f : -m_new;   // no key seen so far
-          float e[2][2];
-#pragma unroll
-          for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) e[nt][c] = fast_exp2(sc[nt][2 * hf + c] + neg_m);
-          l[hf] = l[hf] * alpha[hf] + ((e[0][0] + e[0][1]) + (e[1][0] + e[1][1]));
-          p[hf] = pack2<MMA_BF16>(e[0][0], e[0][1]);
-          p[2 + hf] = pack2<MMA_BF16>(e[1][0], e[1][1]);
+        for (int e = 0; e < 2; ++e) {   // of the columns this thread has in the accumulators
+          sl2[nq][e] = FOUR ? __shfl_sync(0xffffffffu, mul, (2 * t + e) * 4) : mul;
+          const int rr = nq * 8 + 2 * t + e;
+          limit[nq][e] = rr < n_rows ? keys_of(a, seq, (r0 + rr) / a.group) : 0;
         }
-        if (__any_sync(0xffffffffu, moved)) {
+      }
+
+      float m[NQ][2], l[NQ][2];
+      float o[NQ][D / 16][4];   // 16 bits: dimensions 16 mt + g and + 8; 4 bits: block 2 c + e has 32 c + 4 g + 2 e and + 1
+      [[maybe_unused]] float ob[NQ][4];   // 4 bits: rows are scales and bases
 #pragma unroll
-          for (int nt = 0; nt < D / 8; ++nt) {
-            o[nt][0] *= alpha[0];
-            o[nt][1] *= alpha[0];
-            o[nt][2] *= alpha[1];
-            o[nt][3] *= alpha[1];
+      for (int nq = 0; nq < NQ; ++nq) {
+        m[nq][0] = m[nq][1] = -INFINITY;
+        l[nq][0] = l[nq][1] = 0.f;
+#pragma unroll
+        for (int c = 0; c < D / 16; ++c) o[nq][c][0] = o[nq][c][1] = o[nq][c][2] = o[nq][c][3] = 0.f;
+        ob[nq][0] = ob[nq][1] = ob[nq][2] = ob[nq][3] = 0.f;
+      }
+
+      for (int j = w.j0; j < w.j1; ++j, ++i) {
+        const int s = i % ST;
+        const int kw = warp * 16 * UN, key0 = j * KEYS + kw;   // this warp's keys in the step, in the sequence
+        mbar_wait(full + s, (i / ST) & 1, wctx, kPgFull);
+        if (key0 < k_limit) {
+          const uint32_t sk = smem_u32(smem + s * L::kStage), sv = sk + L::kTile;
+          const bool whole = key0 + 16 * UN <= k_limit;
+          // ---- S^T ----------------------------------------------------------------------
+          float sc[UN][NQ][4];   // keys 16 un + g (rows 2t, 2t + 1), + 8
+#pragma unroll
+          for (int un = 0; un < UN; ++un) {
+            const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+            const int kb = kw + un * 16;
+            if constexpr (FOUR) {
+              const uint32_t par = sv + L::kTile;
+              // scales of keys g and g + 8 in 32 bits; (scale, base) of group t of either as the operand of the sums
+              float ks[2][D / 32];
+              uint32_t pw[4];
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const uint32_t at = par + (kb + g + 8 * e) * L::kParBytes;
+                if constexpr (D == 128) {
+                  const uint4 x = lds128(at);
+                  ks[e][0] = unpack_lo<false>(x.x); ks[e][1] = unpack_lo<false>(x.y); ks[e][2] = unpack_lo<false>(x.z); ks[e][3] = unpack_lo<false>(x.w);
+                } else {
+                  const uint2 x = lds64(at);
+                  ks[e][0] = unpack_lo<false>(x.x); ks[e][1] = unpack_lo<false>(x.y);
+                }
+                pw[e] = pw[2 + e] = lds32(at + (t % (D / 32)) * 4);
+              }
+              float acc[NQ][4];
+#pragma unroll
+              for (int nq = 0; nq < NQ; ++nq) acc[nq][0] = acc[nq][1] = acc[nq][2] = acc[nq][3] = 0.f;
+#pragma unroll
+              for (int c = 0; c < D / 32; c += 2) {
+                // blocks: (keys 0-7, group c), (keys 8-15, group c), (keys 0-7, group c + 1), (keys 8-15, group c + 1): word t of key g
+                const int key = kb + (mi & 1) * 8 + r8, ch = c + (mi >> 1);
+                uint32_t wd[4];
+                ldmatrix_x4<false>(wd, sk + key * L::kRowBytes + ((D == 128 ? ch ^ ((key >> 1) & 3) : ch ^ ((key >> 2) & 1)) << 4));
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  uint32_t v0[4], v1[4];
+                  code_pairs(wd[2 * e], v0);
+                  code_pairs(wd[2 * e + 1], v1);
+                  const uint32_t a0[4] = {v0[0], v1[0], v0[1], v1[1]}, a1[4] = {v0[2], v1[2], v0[3], v1[3]};
+#pragma unroll
+                  for (int nq = 0; nq < NQ; ++nq) {
+                    float mm[4], m2[4];
+                    mma_16816<false>(mm, a0, qf[nq][2 * (c + e)][0], qf[nq][2 * (c + e)][1], zero);
+                    mma_16816<false>(m2, a1, qf[nq][2 * (c + e) + 1][0], qf[nq][2 * (c + e) + 1][1], mm);
+                    acc[nq][0] = fmaf(ks[0][c + e], m2[0], acc[nq][0]);
+                    acc[nq][1] = fmaf(ks[0][c + e], m2[1], acc[nq][1]);
+                    acc[nq][2] = fmaf(ks[1][c + e], m2[2], acc[nq][2]);
+                    acc[nq][3] = fmaf(ks[1][c + e], m2[3], acc[nq][3]);
+                  }
+                }
+              }
+#pragma unroll
+              for (int nq = 0; nq < NQ; ++nq) {
+                float base[4];
+                mma_16816<false>(base, pw, af[nq][0], af[nq][1], zero);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sc[un][nq][e] = fmaf(acc[nq][e], 65536.f, base[e]);   // c 2^-20 times 2^16 is c / 16
+              }
+            } else {
+#pragma unroll
+              for (int nq = 0; nq < NQ; ++nq) sc[un][nq][0] = sc[un][nq][1] = sc[un][nq][2] = sc[un][nq][3] = 0.f;
+#pragma unroll
+              for (int ks = 0; ks < D / 16; ++ks) {
+                uint32_t kf[4];   // blocks: (keys 0-7, dims lo), (keys 8-15, dims lo), (0-7, hi), (8-15, hi)
+                ldmatrix_x4<false>(kf, sk + (ks / 4) * L::kSub + sw128_offset(kb + (mi & 1) * 8 + r8, (ks % 4) * 2 + (mi >> 1)));
+#pragma unroll
+                for (int nq = 0; nq < NQ; ++nq) mma_16816<MMA_BF16>(sc[un][nq], kf, qf[nq][ks][0], qf[nq][ks][1], sc[un][nq]);
+              }
+            }
           }
-        }
-        // What lies behind the last key is not a number that a zero probability could be trusted with: keys 2t, 2t + 1 and 8 + 2t, 9 + 2t
-        auto keep = [&](int nt) {
-          const int left = k_limit - key0 - nt * 8 - 2 * t;
-          return left >= 2 ? 0xffffffffu : left == 1 ? 0x0000ffffu : 0u;
-        };
-        if constexpr (FOUR) {
-          // Thread (g, t) has the codes of keys 2t, 2t + 1, 8 + 2t, 9 + 2t in word g (D = 128: and g + 8) of their rows.  In a load the threads of odd t
-          // (D = 64: of upper t) take the keys of a pair in the other order, which spreads the rows over the banks; `sel` undoes it.
-          const uint32_t par = sv + L::kTile + L::kParTile;
-          const int odd = D == 128 ? t & 1 : t >> 1;
-          const uint32_t sel_lo = odd ? 0x1054u : 0x5410u, sel_hi = odd ? 0x3276u : 0x7632u;
-          auto word = [&](int key, int h) {
-            const int wd = g + 8 * h;
-            return lds32(sv + key * L::kRowBytes + (D == 128 ? (((wd >> 2) ^ ((key >> 1) & 3)) << 4) + (wd & 3) * 4 : wd * 4));
+          // ---- running maximum, exponentials -------------------------------------------------------
+          if (key0 + 16 * UN > lim_min) {
+#pragma unroll
+            for (int un = 0; un < UN; ++un)
+#pragma unroll
+              for (int nq = 0; nq < NQ; ++nq)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  if (key0 + un * 16 + (e >> 1) * 8 + g >= limit[nq][e & 1]) sc[un][nq][e] = -INFINITY;
+          }
+          float mx[NQ][2];
+          bool more = false;
+#pragma unroll
+          for (int nq = 0; nq < NQ; ++nq)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float x = fmaxf(sc[0][nq][e], sc[0][nq][2 + e]);
+#pragma unroll
+              for (int un = 1; un < UN; ++un) x = fmax3(x, sc[un][nq][e], sc[un][nq][2 + e]);
+              mx[nq][e] = x * sl2[nq][e];
+              more |= mx[nq][e] > m[nq][e] + kLazy;
+            }
+          if (__any_sync(0xffffffffu, more)) {   // the maximum of a row has moved
+#pragma unroll
+            for (int nq = 0; nq < NQ; ++nq) {
+              float alpha[2];
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                float x = mx[nq][e];
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                const float m_new = x > m[nq][e] + kLazy ? x : m[nq][e];
+                alpha[e] = m_new == m[nq][e] ? 1.0f : fast_exp2(m[nq][e] - m_new);
+                m[nq][e] = m_new;
+                l[nq][e] *= alpha[e];
+              }
+#pragma unroll
+              for (int c = 0; c < D / 16; ++c) {
+                o[nq][c][0] *= alpha[0];
+                o[nq][c][1] *= alpha[1];
+                o[nq][c][2] *= alpha[0];
+                o[nq][c][3] *= alpha[1];
+              }
+              if constexpr (FOUR) {
+                ob[nq][0] *= alpha[0];
+                ob[nq][1] *= alpha[1];
+              }
+            }
+          }
+          uint32_t p[UN][NQ][2];   // P^T as the second operand: keys 2t, 2t + 1 (and 8 further on) of row g
+#pragma unroll
+          for (int nq = 0; nq < NQ; ++nq) {
+            const float n0 = m[nq][0] == -INFINITY ? 0.f : -m[nq][0], n1 = m[nq][1] == -INFINITY ? 0.f : -m[nq][1];   // no key seen so far
+#pragma unroll
+            for (int un = 0; un < UN; ++un)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const float e0 = fast_exp2(fmaf(sc[un][nq][2 * e], sl2[nq][0], n0)), e1 = fast_exp2(fmaf(sc[un][nq][2 * e + 1], sl2[nq][1], n1));
+                l[nq][0] += e0;
+                l[nq][1] += e1;
+                p[un][nq][e] = transpose_8x8(pack2<MMA_BF16>(e0, e1));
+              }
+          }
+          // ---- O^T --------------------------------------------------------------------------------
+          // What lies behind the last key is not a number that a zero probability could be trusted with: keys 16 un + 8 e + 2t and the next
+          auto keep = [&](int un, int e) {
+            const int rest = k_limit - key0 - un * 16 - e * 8 - 2 * t;
+            return rest >= 2 ? 0xffffffffu : rest == 1 ? 0x0000ffffu : 0u;
           };
 #pragma unroll
-          for (int h = 0; h < D / 64; ++h) {
-            uint32_t vb[2][8];   // B fragments: [key pair][value of the word], (key, key + 1)
+          for (int un = 0; un < UN; ++un) {
+            const int kb = kw + un * 16;
+            if constexpr (FOUR) {
+              const uint32_t par = sv + L::kTile + L::kParTile;
+              uint32_t ss[2][D / 32], pt[4] = {};   // scales of keys 2t, 2t + 1 (8 e further on); transposed scales and bases: row g = value g of a key's
 #pragma unroll
-            for (int kp = 0; kp < 2; ++kp) {
-              const int key = warp * 16 + kp * 8 + 2 * t;
-              const uint32_t x = word(key + odd, h), y = word(key + (odd ^ 1), h);
-              const int grp = 2 * h + (g >> 2);   // of dimensions 64 h + 8 g ...
-              const uint32_t px = lds32(par + (key + odd) * L::kParBytes + grp * 4), py = lds32(par + (key + (odd ^ 1)) * L::kParBytes + grp * 4);
-              uint32_t ss = prmt(px, py, sel_lo), bb = prmt(px, py, sel_hi);
-              if (!whole) {
-                const uint32_t kpm = keep(kp);
-                ss &= kpm;
-                bb &= kpm;
+              for (int e = 0; e < 2; ++e) {
+                const uint32_t at = par + (kb + 8 * e + 2 * t) * L::kParBytes;
+                if constexpr (D == 128) {
+                  const uint4 x = lds128(at), y = lds128(at + 16);
+                  ss[e][0] = prmt(x.x, y.x, 0x5410u); ss[e][1] = prmt(x.y, y.y, 0x5410u); ss[e][2] = prmt(x.z, y.z, 0x5410u); ss[e][3] = prmt(x.w, y.w, 0x5410u);
+                } else {
+                  const uint4 x = lds128(at);   // both keys
+                  ss[e][0] = prmt(x.x, x.z, 0x5410u); ss[e][1] = prmt(x.y, x.w, 0x5410u);
+                  const uint32_t lo = g & 2 ? x.y : x.x, hi = g & 2 ? x.w : x.z;
+                  pt[2 * e] = g < 4 ? prmt(lo, hi, g & 1 ? 0x7632u : 0x5410u) : 0u;
+                }
               }
-              const uint32_t step = hmul2(ss, 0x2C002C00u), first = hadd2(bb, ss);
-              const uint32_t lo = prmt(x, y, sel_lo), hi = prmt(x, y, sel_hi);   // codes 0..3 of either key, codes 4..7
-              const uint32_t lo8 = lo >> 8, hi8 = hi >> 8;
-              vb[kp][0] = hfma2(hadd2(mask_or(lo, 0x000F000Fu, 0x64006400u), 0xE400E400u), step, first);
-              vb[kp][1] = hfma2(hadd2(mask_or(lo, 0x00F000F0u, 0x54005400u), 0xD400D400u), step, first);
-              vb[kp][2] = hfma2(hadd2(mask_or(lo8, 0x000F000Fu, 0x64006400u), 0xE400E400u), step, first);
-              vb[kp][3] = hfma2(hadd2(mask_or(lo8, 0x00F000F0u, 0x54005400u), 0xD400D400u), step, first);
-              vb[kp][4] = hfma2(hadd2(mask_or(hi, 0x000F000Fu, 0x64006400u), 0xE400E400u), step, first);
-              vb[kp][5] = hfma2(hadd2(mask_or(hi, 0x00F000F0u, 0x54005400u), 0xD400D400u), step, first);
-              vb[kp][6] = hfma2(hadd2(mask_or(hi8, 0x000F000Fu, 0x64006400u), 0xE400E400u), step, first);
-              vb[kp][7] = hfma2(hadd2(mask_or(hi8, 0x00F000F0u, 0x54005400u), 0xD400D400u), step, first);
-            }
+              if constexpr (D == 128) ldmatrix_x2<true>(pt[0], pt[2], par + (kb + (lane & 15)) * 16);
+              if (!whole) {
 #pragma unroll
-            for (int c = 0; c < 8; ++c) mma_16816<false>(o[8 * h + c], p, vb[0][c], vb[1][c]);
+                for (int e = 0; e < 2; ++e) {
+                  const uint32_t kp = keep(un, e);
+                  pt[2 * e] &= kp;
+#pragma unroll
+                  for (int c = 0; c < D / 32; ++c) ss[e][c] &= kp;
+                }
+              }
+#pragma unroll
+              for (int nq = 0; nq < NQ; ++nq) mma_16816<false>(ob[nq], pt, p[un][nq][0], p[un][nq][1], ob[nq]);
+#pragma unroll
+              for (int c = 0; c < D / 32; c += 2) {
+                // as for K, transposed: four codes (4g and on of the group) of keys 2t and 2t + 1
+                const int key = kb + (mi & 1) * 8 + r8, ch = c + (mi >> 1);
+                uint32_t wd[4];
+                ldmatrix_x4<true>(wd, sv + key * L::kRowBytes + ((D == 128 ? ch ^ ((key >> 1) & 3) : ch ^ ((key >> 2) & 1)) << 4));
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  uint32_t v0[4], v1[4];
+                  code_pairs(wd[2 * e], v0);
+                  code_pairs(wd[2 * e + 1], v1);
+                  const uint32_t a0[4] = {v0[0], v0[1], v1[0], v1[1]}, a1[4] = {v0[2], v0[3], v1[2], v1[3]};
+#pragma unroll
+                  for (int nq = 0; nq < NQ; ++nq) {
+                    const uint32_t b0 = hmul2(p[un][nq][0], ss[0][c + e]), b1 = hmul2(p[un][nq][1], ss[1][c + e]);
+                    mma_16816<false>(o[nq][2 * (c + e)], a0, b0, b1, o[nq][2 * (c + e)]);
+                    mma_16816<false>(o[nq][2 * (c + e) + 1], a1, b0, b1, o[nq][2 * (c + e) + 1]);
+                  }
+                }
+              }
+            } else {
+#pragma unroll
+              for (int mt = 0; mt < D / 16; ++mt) {
+                uint32_t vf[4];   // transposed blocks: (keys 0-7, dims lo), (keys 0-7, dims hi), (8-15, lo), (8-15, hi)
+                ldmatrix_x4<true>(vf, sv + (mt / 4) * L::kSub + sw128_offset(kb + (mi >> 1) * 8 + r8, (mt % 4) * 2 + (mi & 1)));
+                if (!whole) {
+                  const uint32_t k0 = keep(un, 0), k1 = keep(un, 1);
+                  vf[0] &= k0;
+                  vf[1] &= k0;
+                  vf[2] &= k1;
+                  vf[3] &= k1;
+                }
+#pragma unroll
+                for (int nq = 0; nq < NQ; ++nq) mma_16816<MMA_BF16>(o[nq][mt], vf, p[un][nq][0], p[un][nq][1], o[nq][mt]);
+              }
+            }
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(empty + s);
+      }
+
+      // ============================ add up the four warps ===============================
+#pragma unroll
+      for (int nq = 0; nq < NQ; ++nq)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+          for (int k = 4; k < 32; k *= 2) l[nq][e] += __shfl_xor_sync(0xffffffffu, l[nq][e], k);
+          if (g == 0) stats[warp * ROWS + nq * 8 + 2 * t + e] = make_float2(m[nq][e], l[nq][e]);
+        }
+      const bool done = w.first && w.last;
+      const int place = 2 * blockIdx.x + (w.n == 0 ? 0 : 1);
+#pragma unroll
+      for (int rd = 0; rd < ROWS / L::kRows; ++rd) {
+        const int rows_from = rd * L::kRows;
+        if (rows_from >= n_rows) break;
+        const int nq = rows_from / 8;
+        float* mine = share + warp * (L::kShare / 4);
+        if constexpr (FOUR) {
+          static_assert(L::kRows == 8, "a round is a column of rows");
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float* dst = mine + (2 * t + e) * L::kRowFloats + 4 * g;
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+              // the sum of P (b + s) of the group is in lanes 2c and 2c + 1 of the rows of scales and bases
+              const float both = __shfl_sync(0xffffffffu, ob[nq][e], 8 * c + t) + __shfl_sync(0xffffffffu, ob[nq][e], 8 * c + 4 + t);
+              *reinterpret_cast<float4*>(dst + 32 * c) =
+                  make_float4(fmaf(o[nq][2 * c][e], 1048576.f, both), fmaf(o[nq][2 * c][2 + e], 65536.f, both),
+                              fmaf(o[nq][2 * c + 1][e], 1048576.f, both), fmaf(o[nq][2 * c + 1][2 + e], 65536.f, both));
+            }
           }
         } else {
 #pragma unroll
-          for (int np = 0; np < D / 16; ++np) {
-            uint32_t vf[4];
-            ldmatrix_x4<true>(vf, sv + (np / 4) * L::kSub + sw128_offset(v_row, (np % 4) * 2 + v_ch));
-            if (!whole) {
-              const uint32_t m0 = keep(0), m1 = keep(1);
-              vf[0] &= m0;
-              vf[1] &= m1;
-              vf[2] &= m0;
-              vf[3] &= m1;
+          for (int e = 0; e < 2; ++e)
+            if ((2 * t + e) / L::kRows == rd % (8 / L::kRows)) {
+              float* dst = mine + ((2 * t + e) % L::kRows) * L::kRowFloats + g;
+#pragma unroll
+              for (int mt = 0; mt < D / 16; ++mt) {
+                dst[16 * mt] = o[nq][mt][e];
+                dst[16 * mt + 8] = o[nq][mt][2 + e];
+              }
             }
-            mma_16816<MMA_BF16>(o[2 * np], p, vf[0], vf[1]);
-            mma_16816<MMA_BF16>(o[2 * np + 1], p, vf[2], vf[3]);
+        }
+        named_bar_sync(1, 32 * kPgWarps);
+        const int items = *abort_flag ? 0 : min(L::kRows, n_rows - rows_from) * (D / 8);   // (row, 8 columns)
+        for (int x = tid; x < items; x += 32 * kPgWarps) {
+          const int row = rows_from + x / (D / 8), ch = x % (D / 8);
+          float m_all = -INFINITY, l_all = 0.f, acc[8] = {};
+#pragma unroll
+          for (int k = 0; k < kPgWarps; ++k) m_all = fmaxf(m_all, stats[k * ROWS + row].x);
+#pragma unroll
+          for (int k = 0; k < kPgWarps; ++k) {
+            const float2 st = stats[k * ROWS + row];
+            const float f = st.x == -INFINITY ? 0.f : fast_exp2(st.x - m_all);   // a warp without keys
+            l_all = fmaf(f, st.y, l_all);
+            const float4* src = reinterpret_cast<const float4*>(share + k * (L::kShare / 4) + (row - rows_from) * L::kRowFloats + ch * 8);
+            const float4 x0 = src[0], x1 = src[1];
+            acc[0] = fmaf(f, x0.x, acc[0]); acc[1] = fmaf(f, x0.y, acc[1]); acc[2] = fmaf(f, x0.z, acc[2]); acc[3] = fmaf(f, x0.w, acc[3]);
+            acc[4] = fmaf(f, x1.x, acc[4]); acc[5] = fmaf(f, x1.y, acc[5]); acc[6] = fmaf(f, x1.z, acc[6]); acc[7] = fmaf(f, x1.w, acc[7]);
+          }
+          if (done) {
+            const int64_t at = seq.row0 + (r0 + row) / a.group;
+            const int h = w.hk * a.group + (r0 + row) % a.group;
+            const float inv = l_all > 0.f ? 1.0f / l_all : 0.f;   // no key: zeros (a NaN among the scores stays one: its accumulator is)
+            *reinterpret_cast<uint4*>(static_cast<unsigned short*>(a.o_ptr) + at * a.o_ss + h * a.o_sh + ch * 8) =
+                make_uint4(pack2<BF16>(acc[0] * inv, acc[1] * inv), pack2<BF16>(acc[2] * inv, acc[3] * inv), pack2<BF16>(acc[4] * inv, acc[5] * inv),
+                           pack2<BF16>(acc[6] * inv, acc[7] * inv));
+            if (ch == 0 && a.lse != nullptr)
+              a.lse[static_cast<int64_t>(h) * a.total_rows + at] = l_all == 0.f ? -INFINITY : (m_all + fast_log2(l_all)) * kPgLn2;
+          } else {
+            float4* dst = reinterpret_cast<float4*>(a.part_o + (static_cast<int64_t>(place) * ROWS + row) * D + ch * 8);
+            dst[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+            dst[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+            if (ch == 0) a.part_ml[place * ROWS + row] = make_float2(m_all, l_all);
           }
         }
+        named_bar_sync(1, 32 * kPgWarps);   // the shares (and at the end the statistics) may be overwritten
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(empty + s);
-    }
-#pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
-      l[hf] += __shfl_xor_sync(0xffffffffu, l[hf], 1);
-      l[hf] += __shfl_xor_sync(0xffffffffu, l[hf], 2);
-    }
-  }
-  __syncthreads();   // every stage has been read: the shares may overwrite them
-
-  // ============================ combine the four warps ================================
-  float2* stats = reinterpret_cast<float2*>(smem + L::kOffStats);   // [4][16] (maximum, sum)
-  if (warp < kPgWarps) {
-    float* share = reinterpret_cast<float*>(smem + warp * L::kShare);
-    if constexpr (FOUR) {
-      // n-tile 8 h + c: columns 2t, 2t + 1 are dimensions 64 h + 16 t + c and + 8
-#pragma unroll
-      for (int h = 0; h < D / 64; ++h)
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-#pragma unroll
-          for (int c = 0; c < 8; c += 4) {
-            float* dst = share + g * L::kRowFloats + 64 * h + 16 * t + 8 * e + c;
-            *reinterpret_cast<float4*>(dst) = make_float4(o[8 * h + c][e], o[8 * h + c + 1][e], o[8 * h + c + 2][e], o[8 * h + c + 3][e]);
-            *reinterpret_cast<float4*>(dst + 8 * L::kRowFloats) =
-                make_float4(o[8 * h + c][2 + e], o[8 * h + c + 1][2 + e], o[8 * h + c + 2][2 + e], o[8 * h + c + 3][2 + e]);
-          }
-    } else {
-#pragma unroll
-      for (int nt = 0; nt < D / 8; ++nt) {
-        *reinterpret_cast<float2*>(share + g * L::kRowFloats + nt * 8 + 2 * t) = make_float2(o[nt][0], o[nt][1]);
-        *reinterpret_cast<float2*>(share + (g + 8) * L::kRowFloats + nt * 8 + 2 * t) = make_float2(o[nt][2], o[nt][3]);
-      }
-    }
-    if (t == 0) {
-      stats[warp * kPagedRows + g] = make_float2(m[0], l[0]);
-      stats[warp * kPagedRows + g + 8] = make_float2(m[1], l[1]);
-    }
+      if (tid == 0 && !w.last) a.part_info[blockIdx.x].y = place;   // the CTA's last part, whose unit goes on in the next CTA
+    } while (way_next<KEYS>(a, w));
   }
   __syncthreads();
-  const int items = *abort_flag ? 0 : n_rows * (D / 8);   // (row, 8 columns)
-  for (int i = threadIdx.x; i < items; i += kPgThreads) {
-    const int row = i / (D / 8), ch = i % (D / 8);
-    float m_all = -INFINITY, l_all = 0.f, acc[8] = {};
-#pragma unroll
-    for (int k = 0; k < kPgWarps; ++k) m_all = fmaxf(m_all, stats[k * kPagedRows + row].x);
-#pragma unroll
-    for (int k = 0; k < kPgWarps; ++k) {
-      const float2 st = stats[k * kPagedRows + row];
-      const float w = st.x == -INFINITY ? 0.f : fast_exp2(st.x - m_all);   // a warp without keys
-      l_all = fmaf(w, st.y, l_all);
-      const float4* src = reinterpret_cast<const float4*>(smem + k * L::kShare + (row * L::kRowFloats + ch * 8) * 4);
-      const float4 x = src[0], y = src[1];
-      acc[0] = fmaf(w, x.x, acc[0]); acc[1] = fmaf(w, x.y, acc[1]); acc[2] = fmaf(w, x.z, acc[2]); acc[3] = fmaf(w, x.w, acc[3]);
-      acc[4] = fmaf(w, y.x, acc[4]); acc[5] = fmaf(w, y.y, acc[5]); acc[6] = fmaf(w, y.z, acc[6]); acc[7] = fmaf(w, y.w, acc[7]);
-    }
-    const int64_t at = seq.row0 + (r0 + row) / a.group;
-    const int h = hk * a.group + (r0 + row) % a.group;
-    if (n_split == 1) {
-      const float inv = l_all > 0.f ? 1.0f / l_all : 0.f;   // no key: zeros (a NaN among the scores stays one: its accumulator is)
-      *reinterpret_cast<uint4*>(static_cast<unsigned short*>(a.o_ptr) + at * a.o_ss + h * a.o_sh + ch * 8) =
-          make_uint4(pack2<BF16>(acc[0] * inv, acc[1] * inv), pack2<BF16>(acc[2] * inv, acc[3] * inv), pack2<BF16>(acc[4] * inv, acc[5] * inv),
-                     pack2<BF16>(acc[6] * inv, acc[7] * inv));
-      if (ch == 0 && a.lse != nullptr)
-        a.lse[static_cast<int64_t>(h) * a.total_rows + at] = l_all == 0.f ? -INFINITY : (m_all + fast_log2(l_all)) * kPgLn2;
-    } else {
-      const int64_t share = (at * a.H + h) * a.n_split + split;
-      float4* dst = reinterpret_cast<float4*>(a.part_o + share * D + ch * 8);
-      dst[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-      dst[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
-      if (ch == 0) a.part_ml[share] = make_float2(m_all, l_all);
-    }
-  }
   if (*abort_flag) {
     for (int k = 0; k < 20; ++k) __nanosleep(1000000);   // copies in flight end before the CTA does
     __syncthreads();
   }
 }
 
-// Joins the shares of rows whose keys were dealt out: a warp per (new row, head).
+// Joins the pieces of a unit that was cut: block c takes the unit that CTA c begins in the middle of, if CTA c - 1 began elsewhere; the
+// pieces are the last part of CTA c - 1 and the first ones of CTA c and all after it that begin in the same unit.
 template <int D, bool BF16>
 __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__ PagedArgs a) {
   griddep_wait();
-  const int lane = threadIdx.x & 31;
-  const int64_t rh = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  if (rh >= static_cast<int64_t>(a.total_rows) * a.H) return;
-  const int row = static_cast<int>(rh / a.H), h = static_cast<int>(rh % a.H);
-  const int b = a.cu != nullptr ? sequence_of_row(a.cu, a.B, row) : row / a.rows_each;
-  if (b < 0 || b >= a.B) return;
+  const int c = blockIdx.x + 1;   // of a.ctas CTAs
+  const int unit = a.part_info[c].x;
+  const int2 before = a.part_info[c - 1];
+  if (unit < 0 || before.x == unit) return;
+  int n = 2;   // pieces
+  while (c + n - 1 < a.ctas && a.part_info[c + n - 1].x == unit) ++n;
+  const int hk = unit % a.H_kv, tile = unit / a.H_kv % a.row_tiles, b = unit / a.H_kv / a.row_tiles;
   const PgSeq seq = sequence(a, b);
-  const int i = row - seq.row0;
-  if (i >= seq.n_new) return;
-  // the tile of this row, and how many shares it had
-  const int r0 = (i * a.group + h % a.group) / kPagedRows * kPagedRows, n_rows = min(kPagedRows, seq.n_new * a.group - r0);
-  const int n = splits_of(keys_of(a, seq, (r0 + n_rows - 1) / a.group), a.n_split);
-  if (n == 1) return;
-  const float2* ml = a.part_ml + rh * a.n_split;
-  const float* po = a.part_o + rh * a.n_split * D;
-  float m_all = -INFINITY;
-  for (int s = lane; s < n; s += 32) m_all = fmaxf(m_all, ml[s].x);
+  const int r0 = tile * a.tile_rows, n_rows = min(a.tile_rows, seq.n_new * a.group - r0);
+  constexpr int V = D / 32;   // values of a lane; a warp per row
+  const int lane = threadIdx.x & 31;
+  auto place = [&](int k) { return k == 0 ? before.y : 2 * (c + k - 1); };
+  for (int row = threadIdx.x >> 5; row < n_rows; row += 4) {
+    float m_all = -INFINITY;
+    for (int k = lane; k < n; k += 32) m_all = fmaxf(m_all, a.part_ml[place(k) * a.tile_rows + row].x);
 #pragma unroll
-  for (int k = 16; k > 0; k /= 2) m_all = fmaxf(m_all, __shfl_xor_sync(0xffffffffu, m_all, k));
-  float l_all = 0.f;
-  constexpr int V = D / 32;   // values of a lane
-  float acc[V] = {};
-  for (int s0 = 0; s0 < n; s0 += 32) {
-    float w = 0.f;
-    if (s0 + lane < n) {
-      const float2 x = ml[s0 + lane];
-      w = x.x == -INFINITY ? 0.f : fast_exp2(x.x - m_all);   // a share without keys that this row sees
-      l_all = fmaf(w, x.y, l_all);
-    }
-    const int some = min(32, n - s0);
-#pragma unroll 4
-    for (int s = 0; s < some; ++s) {
-      const float ws = __shfl_sync(0xffffffffu, w, s);
-      const float* src = po + static_cast<int64_t>(s0 + s) * D + lane * V;
-      if constexpr (V == 4) {
-        const float4 x = *reinterpret_cast<const float4*>(src);
-        acc[0] = fmaf(ws, x.x, acc[0]); acc[1] = fmaf(ws, x.y, acc[1]); acc[2] = fmaf(ws, x.z, acc[2]); acc[3] = fmaf(ws, x.w, acc[3]);
-      } else {
-        const float2 x = *reinterpret_cast<const float2*>(src);
-        acc[0] = fmaf(ws, x.x, acc[0]); acc[1] = fmaf(ws, x.y, acc[1]);
+    for (int k = 16; k > 0; k /= 2) m_all = fmaxf(m_all, __shfl_xor_sync(0xffffffffu, m_all, k));
+    float l_all = 0.f;
+    float acc[V] = {};
+    for (int k0 = 0; k0 < n; k0 += 32) {
+      float f = 0.f;
+      if (k0 + lane < n) {
+        const float2 x = a.part_ml[place(k0 + lane) * a.tile_rows + row];
+        f = x.x == -INFINITY ? 0.f : fast_exp2(x.x - m_all);   // a piece without keys that this row sees
+        l_all = fmaf(f, x.y, l_all);
+      }
+      const int some = min(32, n - k0);
+#pragma unroll 8
+      for (int k = 0; k < some; ++k) {
+        const float fk = __shfl_sync(0xffffffffu, f, k);
+        const float* src = a.part_o + (static_cast<int64_t>(place(k0 + k)) * a.tile_rows + row) * D + lane * V;
+        if constexpr (V == 4) {
+          const float4 x = *reinterpret_cast<const float4*>(src);
+          acc[0] = fmaf(fk, x.x, acc[0]); acc[1] = fmaf(fk, x.y, acc[1]); acc[2] = fmaf(fk, x.z, acc[2]); acc[3] = fmaf(fk, x.w, acc[3]);
+        } else {
+          const float2 x = *reinterpret_cast<const float2*>(src);
+          acc[0] = fmaf(fk, x.x, acc[0]); acc[1] = fmaf(fk, x.y, acc[1]);
+        }
       }
     }
-  }
 #pragma unroll
-  for (int k = 16; k > 0; k /= 2) l_all += __shfl_xor_sync(0xffffffffu, l_all, k);
-  const float inv = l_all > 0.f ? 1.0f / l_all : 0.f;
-  unsigned short* dst = static_cast<unsigned short*>(a.o_ptr) + static_cast<int64_t>(row) * a.o_ss + h * a.o_sh + lane * V;
-  if constexpr (V == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<BF16>(acc[0] * inv, acc[1] * inv), pack2<BF16>(acc[2] * inv, acc[3] * inv));
-  else *reinterpret_cast<uint32_t*>(dst) = pack2<BF16>(acc[0] * inv, acc[1] * inv);
-  if (lane == 0 && a.lse != nullptr)
-    a.lse[static_cast<int64_t>(h) * a.total_rows + row] = l_all == 0.f ? -INFINITY : (m_all + fast_log2(l_all)) * kPgLn2;
+    for (int k = 16; k > 0; k /= 2) l_all += __shfl_xor_sync(0xffffffffu, l_all, k);
+    const float inv = l_all > 0.f ? 1.0f / l_all : 0.f;
+    const int64_t at = seq.row0 + (r0 + row) / a.group;
+    const int h = hk * a.group + (r0 + row) % a.group;
+    unsigned short* dst = static_cast<unsigned short*>(a.o_ptr) + at * a.o_ss + h * a.o_sh + lane * V;
+    if constexpr (V == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<BF16>(acc[0] * inv, acc[1] * inv), pack2<BF16>(acc[2] * inv, acc[3] * inv));
+    else *reinterpret_cast<uint32_t*>(dst) = pack2<BF16>(acc[0] * inv, acc[1] * inv);
+    if (lane == 0 && a.lse != nullptr)
+      a.lse[static_cast<int64_t>(h) * a.total_rows + at] = l_all == 0.f ? -INFINITY : (m_all + fast_log2(l_all)) * kPgLn2;
+  }
 }
 
-// CTAs that may share a tile's keys: enough of them for two on every SM and a few to spare, since sequences differ in length.
-int paged_splits(int64_t sms, int64_t tiles, int64_t max_keys, int D, int bits) {
-  (void)D;
-  (void)bits;
-  if (sms <= 0 || tiles <= 0) return 1;
-  const int64_t most = std::max<int64_t>(1, (max_keys + kPagedKeyStep - 1) / kPagedKeyStep / kPgMinSteps);
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({most, 4 * sms / tiles, 128})));
+// Where no sequence can have more keys than a CTA takes at the least, units stay whole (no workspace, no second kernel).  Else two CTAs per SM, but no
+// more than the most keys that there can be would occupy.
+PagedGrid paged_grid(int64_t sms, int64_t max_rows, int64_t group, int64_t heads, int64_t max_keys) {
+  PagedGrid g;
+  g.tile_rows = max_rows * group <= 8 ? 8 : 16;
+  g.row_tiles = (max_rows * group + g.tile_rows - 1) / g.tile_rows;
+  g.whole = max_keys <= kPgMinKeys;
+  const int64_t units = g.row_tiles * heads, most = units * std::max<int64_t>(1, (max_keys + kPgMinKeys - 1) / kPgMinKeys);
+  g.ctas = static_cast<int>(std::max<int64_t>(1, std::min(2 * sms, most)));
+  return g;
+}
+size_t paged_workspace(const PagedGrid& g, int D) {
+  return g.whole ? 0 : static_cast<size_t>(g.ctas) * (2 * g.tile_rows * (D * sizeof(float) + sizeof(float2)) + sizeof(int2));
+}
+void paged_places(PagedArgs& a, void* workspace, const PagedGrid& g, int D) {
+  a.whole = g.whole;
+  a.ctas = g.ctas;
+  a.tile_rows = g.tile_rows;
+  a.row_tiles = static_cast<int>(g.row_tiles);
+  if (g.whole) return;
+  const size_t rows = static_cast<size_t>(g.ctas) * 2 * g.tile_rows;
+  a.part_o = static_cast<float*>(workspace);
+  a.part_ml = reinterpret_cast<float2*>(a.part_o + rows * D);
+  a.part_info = reinterpret_cast<int2*>(a.part_ml + rows);
 }
 
-template <int D, bool BF16, bool FOUR>
+template <int D, bool BF16, bool FOUR, int NQ>
 static int launch_paged_impl(const PagedArgs& a, cudaStream_t stream) {
-  using L = PgSmem<D, FOUR>;
-  auto kfn = fmha_paged_kernel<D, BF16, FOUR>;
+  using L = PgSmem<D, FOUR, NQ>;
+  auto kfn = fmha_paged_kernel<D, BF16, FOUR, NQ>;
   static std::atomic<bool> configured[64] = {};   // per device; set after the attribute call succeeded
   int dev = 0;
   cudaGetDevice(&dev);
@@ -590,19 +840,15 @@ static int launch_paged_impl(const PagedArgs& a, cudaStream_t stream) {
     if (e != cudaSuccess) return static_cast<int>(e);
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
-  const int64_t row_tiles = (static_cast<int64_t>(a.max_rows) * a.group + kPagedRows - 1) / kPagedRows;
-  cudaError_t e = launch_overlapped(kfn, dim3(a.n_split, static_cast<unsigned>(a.H_kv * row_tiles), a.B), dim3(kPgThreads), L::kDynBytes, stream, a);
-  if (e == cudaSuccess && a.n_split > 1) {
-    const int64_t rows = static_cast<int64_t>(a.total_rows) * a.H;
-    e = launch_overlapped(paged_join_kernel<D, BF16>, dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(128), 0, stream, a);
-  }
+  cudaError_t e = launch_overlapped(kfn, dim3(a.ctas), dim3(kPgThreads), L::kDynBytes, stream, a);
+  if (e == cudaSuccess && !a.whole && a.ctas > 1) e = launch_overlapped(paged_join_kernel<D, BF16>, dim3(a.ctas - 1), dim3(128), 0, stream, a);
   return static_cast<int>(e != cudaSuccess ? e : cudaGetLastError());
 }
 
 int launch_paged(const PagedArgs& a, int dtype, int D, int bits, cudaStream_t stream) {
   const bool bf = dtype == FMHA_DTYPE_BF16, four = bits == 4;
 #define FMHA_PAGED_CASE(DD, BF, F4) \
-  if (D == DD && bf == BF && four == F4) return launch_paged_impl<DD, BF, F4>(a, stream);
+  if (D == DD && bf == BF && four == F4) return a.tile_rows == 8 ? launch_paged_impl<DD, BF, F4, 1>(a, stream) : launch_paged_impl<DD, BF, F4, 2>(a, stream);
   FMHA_PAGED_CASE(64, false, false)
   FMHA_PAGED_CASE(64, true, false)
   FMHA_PAGED_CASE(128, false, false)

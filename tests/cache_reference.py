@@ -45,14 +45,15 @@ class Cache:
                 getattr(self, name)[at], self.params[name + "_params"][at] = encode(x)
 
     def rows(self, name, b, n):
-        """The first n rows of sequence b: values [n, H, D] in 64 bits, and how far what a 4-bit kernel multiplies with may be from them."""
+        """The first n rows of sequence b [n, H, D] in 64 bits: their values, what these are sums of in absolute values, and the part of that in which
+        P has been multiplied by a scale and rounded again (4 bits)."""
         at = self.where(b, torch.arange(n, device=self.k.device))
         x = getattr(self, name)[at]
         if self.bits == 16:
-            return x.double(), torch.zeros_like(x, dtype=torch.float64)
+            return x.double(), x.double().abs(), torch.zeros_like(x, dtype=torch.float64)
         c, s, base = decode_parts(x, self.params[name + "_params"][at])
-        value, first = base + s * (1 + c / 16), base + s
-        return value.flatten(-2), (2.0 ** -11 * (value.abs() + first.abs()) + 2.0 ** -24).flatten(-2)   # both sums are rounded to fp16
+        by_code = (s * c / 16).flatten(-2)
+        return (base + s * (1 + c / 16)).flatten(-2), (base.abs() + s + s * c / 16).flatten(-2), by_code
 
 
 def encode(x):
@@ -89,22 +90,20 @@ def attention(cache, q, lens, new, scale=None):
     for b, n in enumerate(new):
         total = max(lens[b], 0)
         if total:
-            k, dk = cache.rows("k", b, total)
-            v, dv = cache.rows("v", b, total)
+            k = cache.rows("k", b, total)[0]
+            v, v_abs, v_twice = cache.rows("v", b, total)
         for i in range(n):
             seen = lens[b] - n + i + 1
             if seen > 0:
                 qq = q[r].double().reshape(cache.H, G, D)
                 s = torch.einsum("hgd,jhd->hgj", qq, k[:seen]) * scale
-                es = torch.einsum("hgd,jhd->hgj", qq.abs(), dk[:seen]) * scale   # of a score
                 top = torch.logsumexp(s, -1, keepdim=True)
                 p = (s - top).exp()
                 out = torch.einsum("hgj,jhd->hgd", p, v[:seen])
-                ep = p * es
-                e = (torch.einsum("hgj,jhd->hgd", ep + (up + SLACK) * p + tp, v[:seen].abs()) + torch.einsum("hgj,jhd->hgd", p, dv[:seen]) +
-                     ep.sum(-1, keepdim=True) * out.abs() + u * out.abs())
+                e = (torch.einsum("hgj,jhd->hgd", (up + SLACK) * p + tp, v_abs[:seen]) + up * torch.einsum("hgj,jhd->hgd", p, v_twice[:seen]) +
+                     seen * tp * (cache.bits == 4) + u * out.abs())
                 o[r], ob[r] = out.reshape(H, D), 1.01 * e.reshape(H, D)
-                lse[:, r], lb[:, r] = top.reshape(H), es.amax(-1).reshape(H) + 2.0 ** -12
+                lse[:, r], lb[:, r] = top.reshape(H), 2.0 ** -12
             r += 1
     return (o, ob), (lse, lb)
 
