@@ -50,8 +50,8 @@ struct PagedArgs {
   int B, H, H_kv, group, total_rows, rows_each, max_rows;
   int tile_rows, row_tiles, whole, ctas;   // PagedGrid
   float scale_log2;
-  float* part_o;     // [ctas, 2, tile_rows, D] unnormalised O of pieces of units
-  float2* part_ml;   // [ctas, 2, tile_rows] their maximum (log2 domain) and sum
+  float4* part_o;    // [ctas, 2, tile_rows / 8, D / 16, 32] unnormalised O of pieces of units, in the accumulators' order
+  float4* part_ml;   // [ctas, 2, tile_rows / 8, 4] maximum (log2 domain) and sum of two rows each
   int2* part_info;   // [ctas] the unit that a CTA begins in the middle of, or -1; the place of its last part, if that is not its unit's end
   int* status;
 };

@@ -42,7 +42,7 @@ constexpr int kPgThreads = 32 * (kPgWarps + 1);
 constexpr int kPgMinKeys = 256;   // a CTA's piece of the line holds at least so many
 constexpr float kPgLn2 = 0.6931471805599453f;
 
-enum PgWaitSite { kPgFull = 191, kPgEmpty = 192 };
+enum PgWaitSite { kPgFull = 191, kPgEmpty = 192, kPgSmemBase = 193 };
 
 // NQ: columns of 8 query rows.
 template <int D, bool FOUR, int NQ>
@@ -56,15 +56,13 @@ struct PgSmem {
   static constexpr int kSub = kKeys * 128;                     // 16 bits: a 64-column sub-tile (128-byte swizzle)
   static constexpr int kStage = 2 * (kTile + kParTile);        // K, V, parameters of K, of V
   static constexpr int kStages = FOUR ? (D == 128 ? 4 : 7) : D == 128 ? 3 : 6;
-  // O of the four warps on its way to be added up, kRows rows at a time ([D + 4] fp32 each: rows 2t of a store lie 8 banks apart), and statistics
-  static constexpr int kRows = D == 128 && !FOUR ? 4 : 8;
-  static constexpr int kRowFloats = D + 4;
-  static constexpr int kShare = kRows * kRowFloats * 4;
+  // O of the four warps on its way to be added up, a column of 8 rows at a time, in the accumulators' order (16 bytes of a lane), and statistics
+  static constexpr int kBlocks = D / 16;
   static constexpr int kOffShare = kStages * kStage;
-  static constexpr int kOffStats = kOffShare + kPgWarps * kShare;
+  static constexpr int kOffStats = kOffShare + kPgWarps * kBlocks * 512;
   static constexpr int kOffBar = kOffStats + kPgWarps * 8 * NQ * 8;
   static constexpr int kOffMisc = kOffBar + 2 * kStages * 8;
-  static constexpr int kDynBytes = kOffMisc + 16 + 1024;
+  static constexpr int kDynBytes = kOffMisc + 16;   // 1024-byte aligned base: checked by the kernel
   static_assert(2 * (kDynBytes + 1024) <= 233472, "two CTAs share an SM");
   static_assert(kStage % 1024 == 0 || (FOUR && kStage % 512 == 0), "swizzled tiles begin at multiples of 1024 bytes (64-byte rows: 512)");
 };
@@ -246,6 +244,37 @@ __device__ __forceinline__ bool way_next(const PagedArgs& a, PgWay& w) {
   return true;
 }
 
+// Block c of O^T of the 8 rows from r0 on (of which n exist): a lane's dimensions of rows 2t and 2t + 1, divided by their sums, to O.
+template <bool BF16, bool FOUR>
+__device__ __forceinline__ void store_block(const PagedArgs& a, const PgSeq& seq, int r0, int n, int hk, int c, const float4& x, const float (&l)[2]) {
+  const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    if (2 * t + e >= n) continue;
+    const int r = r0 + 2 * t + e;
+    const float inv = l[e] > 0.f ? 1.0f / l[e] : 0.f;   // no key: zeros (a NaN among the scores stays one: its accumulator is)
+    unsigned short* dst = static_cast<unsigned short*>(a.o_ptr) + static_cast<int64_t>(seq.row0 + r / a.group) * a.o_ss + (hk * a.group + r % a.group) * a.o_sh;
+    const uint32_t v = pack2<BF16>((e ? x.y : x.x) * inv, (e ? x.w : x.z) * inv);
+    if constexpr (FOUR) {
+      *reinterpret_cast<uint32_t*>(dst + 32 * (c / 2) + 4 * g + 2 * (c & 1)) = v;
+    } else {
+      dst[16 * c + g] = static_cast<unsigned short>(v);
+      dst[16 * c + 8 + g] = static_cast<unsigned short>(v >> 16);
+    }
+  }
+}
+__device__ __forceinline__ void store_lse(const PagedArgs& a, const PgSeq& seq, int r0, int n, int hk, const float (&m)[2], const float (&l)[2]) {
+  const int t = threadIdx.x & 3;
+  if (a.lse == nullptr) return;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    if (2 * t + e >= n) continue;
+    const int r = r0 + 2 * t + e;
+    a.lse[static_cast<int64_t>(hk * a.group + r % a.group) * a.total_rows + seq.row0 + r / a.group] =
+        l[e] == 0.f ? -INFINITY : (m[e] + fast_log2(l[e])) * kPgLn2;
+  }
+}
+
 }  // namespace
 
 template <int D, bool BF16, bool FOUR, int NQ>
@@ -255,8 +284,11 @@ __global__ void __launch_bounds__(kPgThreads, 2) fmha_paged_kernel(const __grid_
   constexpr int ST = L::kStages, UN = L::kUnits, KEYS = L::kKeys, ROWS = 8 * NQ;
   constexpr bool MMA_BF16 = BF16 && !FOUR;
   constexpr float kLazy = FOUR ? 0.f : 8.f;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if (smem_u32(smem) & 1023) {
+    if (threadIdx.x == 0 && a.status != nullptr) atomicCAS(a.status, 0, kPgSmemBase);
+    return;
+  }
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kOffBar);   // [ST] a step has landed
   uint64_t* empty = full + ST;                                       // [ST] ... and the four consumer warps are done with it
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kOffMisc);
@@ -348,9 +380,16 @@ __global__ void __launch_bounds__(kPgThreads, 2) fmha_paged_kernel(const __grid_
     // ============================ consumers =========================================
     const int g = lane >> 2, t = lane & 3;   // this thread's MMA rows are g and g + 8, its columns (query rows) 2t and 2t + 1
     const int tid = threadIdx.x;
-    float* share = reinterpret_cast<float*>(smem + L::kOffShare);
+    float4* share = reinterpret_cast<float4*>(smem + L::kOffShare);   // [4][kBlocks][32]
     float2* stats = reinterpret_cast<float2*>(smem + L::kOffStats);   // [4][ROWS] (maximum, sum)
     const int mi = lane >> 3, r8 = lane & 7;   // ldmatrix: lane (mi, r8) addresses row r8 of 8x8 block mi
+    const int kw = warp * 16 * UN;             // this warp's keys in a step
+    // 4 bits: where this lane's row of a ldmatrix lies for groups 0 and 1, and for 2 and 3; blocks: (keys 0-7, group c), (keys 8-15, group c),
+    // (keys 0-7, group c + 1), (keys 8-15, group c + 1); the swizzle goes by the row within 8
+    [[maybe_unused]] const uint32_t ld_key = (kw + (mi & 1) * 8 + r8) * L::kRowBytes;
+    [[maybe_unused]] const uint32_t ld_at[2] = {ld_key + (D == 128 ? ((mi >> 1) ^ (r8 >> 1)) << 4 : ((mi >> 1) ^ (r8 >> 2)) << 4),
+                                                ld_key + (((2 + (mi >> 1)) ^ (r8 >> 1)) << 4)};
+    [[maybe_unused]] const float inv_sl2 = 1.0f / a.scale_log2;
     int i = 0;   // steps so far
     do {
       const PgSeq seq = sequence(a, w.b);
@@ -425,13 +464,15 @@ __global__ void __launch_bounds__(kPgThreads, 2) fmha_paged_kernel(const __grid_
         }
       }
 
-      float m[NQ][2], l[NQ][2];
+      // running maximum of the unscaled scores; what exponents are shifted by (minus the scaled maximum; 0 before the first key); running sum
+      float m[NQ][2];
+      float2 shift[NQ], l[NQ];
       float o[NQ][D / 16][4];   // 16 bits: dimensions 16 mt + g and + 8; 4 bits: block 2 c + e has 32 c + 4 g + 2 e and + 1
       [[maybe_unused]] float ob[NQ][4];   // 4 bits: rows are scales and bases
 #pragma unroll
       for (int nq = 0; nq < NQ; ++nq) {
         m[nq][0] = m[nq][1] = -INFINITY;
-        l[nq][0] = l[nq][1] = 0.f;
+        shift[nq] = l[nq] = make_float2(0.f, 0.f);
 #pragma unroll
         for (int c = 0; c < D / 16; ++c) o[nq][c][0] = o[nq][c][1] = o[nq][c][2] = o[nq][c][3] = 0.f;
         ob[nq][0] = ob[nq][1] = ob[nq][2] = ob[nq][3] = 0.f;
@@ -439,7 +480,7 @@ __global__ void __launch_bounds__(kPgThreads, 2) fmha_paged_kernel(const __grid_
 
       for (int j = w.j0; j < w.j1; ++j, ++i) {
         const int s = i % ST;
-        const int kw = warp * 16 * UN, key0 = j * KEYS + kw;   // this warp's keys in the step, in the sequence
+        const int key0 = j * KEYS + kw;   // this warp's first key
         mbar_wait(full + s, (i / ST) & 1, wctx, kPgFull);
         if (key0 < k_limit) {
           const uint32_t sk = smem_u32(smem + s * L::kStage), sv = sk + L::kTile;
@@ -467,15 +508,13 @@ __global__ void __launch_bounds__(kPgThreads, 2) fmha_paged_kernel(const __grid_
                 }
                 pw[e] = pw[2 + e] = lds32(at + (t % (D / 32)) * 4);
               }
-              float acc[NQ][4];
+              float2 acc[NQ][2];
 #pragma unroll
-              for (int nq = 0; nq < NQ; ++nq) acc[nq][0] = acc[nq][1] = acc[nq][2] = acc[nq][3] = 0.f;
+              for (int nq = 0; nq < NQ; ++nq) acc[nq][0] = acc[nq][1] = make_float2(0.f, 0.f);
 #pragma unroll
               for (int c = 0; c < D / 32; c += 2) {
-                // blocks: (keys 0-7, group c), (keys 8-15, group c), (keys 0-7, group c + 1), (keys 8-15, group c + 1): word t of key g
-                const int key = kb + (mi & 1) * 8 + r8, ch = c + (mi >> 1);
-                uint32_t wd[4];
-                ldmatrix_x4<false>(wd, sk + key * L::kRowBytes + ((D == 128 ? ch ^ ((key >> 1) & 3) : ch ^ ((key >> 2) & 1)) << 4));
+                uint32_t wd[4];   // word t of key g of each block
+                ldmatrix_x4<false>(wd, sk + ld_at[c / 2] + un * 16 * L::kRowBytes);
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                   uint32_t v0[4], v1[4];
@@ -487,10 +526,8 @@ __global__ void __launch_bounds__(kPgThreads, 2) fmha_paged_kernel(const __grid_
                     float mm[4], m2[4];
                     mma_16816<false>(mm, a0, qf[nq][2 * (c + e)][0], qf[nq][2 * (c + e)][1], zero);
                     mma_16816<false>(m2, a1, qf[nq][2 * (c + e) + 1][0], qf[nq][2 * (c + e) + 1][1], mm);
-                    acc[nq][0] = fmaf(ks[0][c + e], m2[0], acc[nq][0]);
-                    acc[nq][1] = fmaf(ks[0][c + e], m2[1], acc[nq][1]);
-                    acc[nq][2] = fmaf(ks[1][c + e], m2[2], acc[nq][2]);
-                    acc[nq][3] = fmaf(ks[1][c + e], m2[3], acc[nq][3]);
+                    acc[nq][0] = __ffma2_rn(make_float2(ks[0][c + e], ks[0][c + e]), make_float2(m2[0], m2[1]), acc[nq][0]);
+                    acc[nq][1] = __ffma2_rn(make_float2(ks[1][c + e], ks[1][c + e]), make_float2(m2[2], m2[3]), acc[nq][1]);
                   }
                 }
               }
@@ -499,7 +536,11 @@ __global__ void __launch_bounds__(kPgThreads, 2) fmha_paged_kernel(const __grid_
                 float base[4];
                 mma_16816<false>(base, pw, af[nq][0], af[nq][1], zero);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sc[un][nq][e] = fmaf(acc[nq][e], 65536.f, base[e]);   // c 2^-20 times 2^16 is c / 16
+                for (int e = 0; e < 2; ++e) {   // c 2^-20 times 2^16 is c / 16
+                  const float2 x = __ffma2_rn(acc[nq][e], make_float2(65536.f, 65536.f), make_float2(base[2 * e], base[2 * e + 1]));
+                  sc[un][nq][2 * e] = x.x;
+                  sc[un][nq][2 * e + 1] = x.y;
+                }
               }
             } else {
 #pragma unroll
@@ -532,24 +573,28 @@ __global__ void __launch_bounds__(kPgThreads, 2) fmha_paged_kernel(const __grid_
               float x = fmaxf(sc[0][nq][e], sc[0][nq][2 + e]);
 #pragma unroll
               for (int un = 1; un < UN; ++un) x = fmax3(x, sc[un][nq][e], sc[un][nq][2 + e]);
-              mx[nq][e] = x * sl2[nq][e];
-              more |= mx[nq][e] > m[nq][e] + kLazy;
+              mx[nq][e] = x;
+              more |= x > (FOUR ? m[nq][e] : fmaf(kLazy, inv_sl2, m[nq][e]));
             }
           if (__any_sync(0xffffffffu, more)) {   // the maximum of a row has moved
 #pragma unroll
             for (int nq = 0; nq < NQ; ++nq) {
-              float alpha[2];
+              float alpha[2], new_shift[2];
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
                 float x = mx[nq][e];
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                const float m_new = x > m[nq][e] + kLazy ? x : m[nq][e];
-                alpha[e] = m_new == m[nq][e] ? 1.0f : fast_exp2(m[nq][e] - m_new);
-                m[nq][e] = m_new;
-                l[nq][e] *= alpha[e];
+                const bool moved = x > (FOUR ? m[nq][e] : fmaf(kLazy, inv_sl2, m[nq][e]));
+                const float old = e ? shift[nq].y : shift[nq].x;
+                new_shift[e] = moved ? -x * sl2[nq][e] : old;
+                alpha[e] = !moved ? 1.0f : m[nq][e] == -INFINITY ? 0.f : fast_exp2(new_shift[e] - old);
+                if (moved) m[nq][e] = x;
               }
+              shift[nq] = make_float2(new_shift[0], new_shift[1]);
+              l[nq].x *= alpha[0];
+              l[nq].y *= alpha[1];
 #pragma unroll
               for (int c = 0; c < D / 16; ++c) {
                 o[nq][c][0] *= alpha[0];
@@ -565,18 +610,16 @@ __global__ void __launch_bounds__(kPgThreads, 2) fmha_paged_kernel(const __grid_
           }
           uint32_t p[UN][NQ][2];   // P^T as the second operand: keys 2t, 2t + 1 (and 8 further on) of row g
 #pragma unroll
-          for (int nq = 0; nq < NQ; ++nq) {
-            const float n0 = m[nq][0] == -INFINITY ? 0.f : -m[nq][0], n1 = m[nq][1] == -INFINITY ? 0.f : -m[nq][1];   // no key seen so far
+          for (int nq = 0; nq < NQ; ++nq)
 #pragma unroll
             for (int un = 0; un < UN; ++un)
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
-                const float e0 = fast_exp2(fmaf(sc[un][nq][2 * e], sl2[nq][0], n0)), e1 = fast_exp2(fmaf(sc[un][nq][2 * e + 1], sl2[nq][1], n1));
-                l[nq][0] += e0;
-                l[nq][1] += e1;
-                p[un][nq][e] = transpose_8x8(pack2<MMA_BF16>(e0, e1));
+                const float2 x = __ffma2_rn(make_float2(sc[un][nq][2 * e], sc[un][nq][2 * e + 1]), make_float2(sl2[nq][0], sl2[nq][1]), shift[nq]);
+                const float2 y = make_float2(fast_exp2(x.x), fast_exp2(x.y));
+                l[nq] = __fadd2_rn(l[nq], y);
+                p[un][nq][e] = transpose_8x8(pack2<MMA_BF16>(y.x, y.y));
               }
-          }
           // ---- O^T --------------------------------------------------------------------------------
           // What lies behind the last key is not a number that a zero probability could be trusted with: keys 16 un + 8 e + 2t and the next
           auto keep = [&](int un, int e) {
@@ -616,10 +659,8 @@ __global__ void __launch_bounds__(kPgThreads, 2) fmha_paged_kernel(const __grid_
               for (int nq = 0; nq < NQ; ++nq) mma_16816<false>(ob[nq], pt, p[un][nq][0], p[un][nq][1], ob[nq]);
 #pragma unroll
               for (int c = 0; c < D / 32; c += 2) {
-                // as for K, transposed: four codes (4g and on of the group) of keys 2t and 2t + 1
-                const int key = kb + (mi & 1) * 8 + r8, ch = c + (mi >> 1);
-                uint32_t wd[4];
-                ldmatrix_x4<true>(wd, sv + key * L::kRowBytes + ((D == 128 ? ch ^ ((key >> 1) & 3) : ch ^ ((key >> 2) & 1)) << 4));
+                uint32_t wd[4];   // as for K, transposed: four codes (4g and on of the group) of keys 2t and 2t + 1
+                ldmatrix_x4<true>(wd, sv + ld_at[c / 2] + un * 16 * L::kRowBytes);
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                   uint32_t v0[4], v1[4];
@@ -661,75 +702,64 @@ __global__ void __launch_bounds__(kPgThreads, 2) fmha_paged_kernel(const __grid_
       for (int nq = 0; nq < NQ; ++nq)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
+          float sum = e ? l[nq].y : l[nq].x;
 #pragma unroll
-          for (int k = 4; k < 32; k *= 2) l[nq][e] += __shfl_xor_sync(0xffffffffu, l[nq][e], k);
-          if (g == 0) stats[warp * ROWS + nq * 8 + 2 * t + e] = make_float2(m[nq][e], l[nq][e]);
+          for (int k = 4; k < 32; k *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+          // (the maximum in the log2 domain, as the exponents were shifted by it)
+          if (g == 0) stats[warp * ROWS + nq * 8 + 2 * t + e] = make_float2(m[nq][e] == -INFINITY ? -INFINITY : -(e ? shift[nq].y : shift[nq].x), sum);
         }
       const bool done = w.first && w.last;
       const int place = 2 * blockIdx.x + (w.n == 0 ? 0 : 1);
 #pragma unroll
-      for (int rd = 0; rd < ROWS / L::kRows; ++rd) {
-        const int rows_from = rd * L::kRows;
-        if (rows_from >= n_rows) break;
-        const int nq = rows_from / 8;
-        float* mine = share + warp * (L::kShare / 4);
-        if constexpr (FOUR) {
-          static_assert(L::kRows == 8, "a round is a column of rows");
+      for (int nq = 0; nq < NQ; ++nq) {
+        if (nq * 8 >= n_rows) break;
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float* dst = mine + (2 * t + e) * L::kRowFloats + 4 * g;
-#pragma unroll
-            for (int c = 0; c < D / 32; ++c) {
-              // the sum of P (b + s) of the group is in lanes 2c and 2c + 1 of the rows of scales and bases
-              const float both = __shfl_sync(0xffffffffu, ob[nq][e], 8 * c + t) + __shfl_sync(0xffffffffu, ob[nq][e], 8 * c + 4 + t);
-              *reinterpret_cast<float4*>(dst + 32 * c) =
-                  make_float4(fmaf(o[nq][2 * c][e], 1048576.f, both), fmaf(o[nq][2 * c][2 + e], 65536.f, both),
-                              fmaf(o[nq][2 * c + 1][e], 1048576.f, both), fmaf(o[nq][2 * c + 1][2 + e], 65536.f, both));
-            }
+        for (int c = 0; c < L::kBlocks; ++c) {
+          float4 x = make_float4(o[nq][c][0], o[nq][c][1], o[nq][c][2], o[nq][c][3]);
+          if constexpr (FOUR) {
+            // the sum of P (b + s) of the group is in lanes 2 (c/2) and 2 (c/2) + 1 of the rows of scales and bases
+            const int at = 8 * (c / 2) + t;
+            const float b0 = __shfl_sync(0xffffffffu, ob[nq][0], at) + __shfl_sync(0xffffffffu, ob[nq][0], at + 4);
+            const float b1 = __shfl_sync(0xffffffffu, ob[nq][1], at) + __shfl_sync(0xffffffffu, ob[nq][1], at + 4);
+            x = make_float4(fmaf(x.x, 1048576.f, b0), fmaf(x.y, 1048576.f, b1), fmaf(x.z, 65536.f, b0), fmaf(x.w, 65536.f, b1));
           }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-            if ((2 * t + e) / L::kRows == rd % (8 / L::kRows)) {
-              float* dst = mine + ((2 * t + e) % L::kRows) * L::kRowFloats + g;
-#pragma unroll
-              for (int mt = 0; mt < D / 16; ++mt) {
-                dst[16 * mt] = o[nq][mt][e];
-                dst[16 * mt + 8] = o[nq][mt][2 + e];
-              }
-            }
+          share[(warp * L::kBlocks + c) * 32 + lane] = x;
         }
         named_bar_sync(1, 32 * kPgWarps);
-        const int items = *abort_flag ? 0 : min(L::kRows, n_rows - rows_from) * (D / 8);   // (row, 8 columns)
-        for (int x = tid; x < items; x += 32 * kPgWarps) {
-          const int row = rows_from + x / (D / 8), ch = x % (D / 8);
-          float m_all = -INFINITY, l_all = 0.f, acc[8] = {};
+        // a warp takes a quarter of the blocks: the rows' factors first
+        float f[kPgWarps][2], m_all[2], l_all[2] = {0.f, 0.f};
+        {
+          float4 st[kPgWarps];   // (maximum, sum) of rows 2t and 2t + 1
 #pragma unroll
-          for (int k = 0; k < kPgWarps; ++k) m_all = fmaxf(m_all, stats[k * ROWS + row].x);
+          for (int k = 0; k < kPgWarps; ++k) st[k] = *reinterpret_cast<const float4*>(stats + k * ROWS + nq * 8 + 2 * t);
+          m_all[0] = fmaxf(fmaxf(st[0].x, st[1].x), fmaxf(st[2].x, st[3].x));
+          m_all[1] = fmaxf(fmaxf(st[0].z, st[1].z), fmaxf(st[2].z, st[3].z));
 #pragma unroll
-          for (int k = 0; k < kPgWarps; ++k) {
-            const float2 st = stats[k * ROWS + row];
-            const float f = st.x == -INFINITY ? 0.f : fast_exp2(st.x - m_all);   // a warp without keys
-            l_all = fmaf(f, st.y, l_all);
-            const float4* src = reinterpret_cast<const float4*>(share + k * (L::kShare / 4) + (row - rows_from) * L::kRowFloats + ch * 8);
-            const float4 x0 = src[0], x1 = src[1];
-            acc[0] = fmaf(f, x0.x, acc[0]); acc[1] = fmaf(f, x0.y, acc[1]); acc[2] = fmaf(f, x0.z, acc[2]); acc[3] = fmaf(f, x0.w, acc[3]);
-            acc[4] = fmaf(f, x1.x, acc[4]); acc[5] = fmaf(f, x1.y, acc[5]); acc[6] = fmaf(f, x1.z, acc[6]); acc[7] = fmaf(f, x1.w, acc[7]);
+          for (int k = 0; k < kPgWarps; ++k) {   // (a warp without keys counts nothing)
+            f[k][0] = st[k].x == -INFINITY ? 0.f : fast_exp2(st[k].x - m_all[0]);
+            f[k][1] = st[k].z == -INFINITY ? 0.f : fast_exp2(st[k].z - m_all[1]);
+            l_all[0] = fmaf(f[k][0], st[k].y, l_all[0]);
+            l_all[1] = fmaf(f[k][1], st[k].w, l_all[1]);
           }
-          if (done) {
-            const int64_t at = seq.row0 + (r0 + row) / a.group;
-            const int h = w.hk * a.group + (r0 + row) % a.group;
-            const float inv = l_all > 0.f ? 1.0f / l_all : 0.f;   // no key: zeros (a NaN among the scores stays one: its accumulator is)
-            *reinterpret_cast<uint4*>(static_cast<unsigned short*>(a.o_ptr) + at * a.o_ss + h * a.o_sh + ch * 8) =
-                make_uint4(pack2<BF16>(acc[0] * inv, acc[1] * inv), pack2<BF16>(acc[2] * inv, acc[3] * inv), pack2<BF16>(acc[4] * inv, acc[5] * inv),
-                           pack2<BF16>(acc[6] * inv, acc[7] * inv));
-            if (ch == 0 && a.lse != nullptr)
-              a.lse[static_cast<int64_t>(h) * a.total_rows + at] = l_all == 0.f ? -INFINITY : (m_all + fast_log2(l_all)) * kPgLn2;
-          } else {
-            float4* dst = reinterpret_cast<float4*>(a.part_o + (static_cast<int64_t>(place) * ROWS + row) * D + ch * 8);
-            dst[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-            dst[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
-            if (ch == 0) a.part_ml[place * ROWS + row] = make_float2(m_all, l_all);
+        }
+        if (*abort_flag == 0) {
+#pragma unroll
+          for (int c = warp; c < L::kBlocks; c += kPgWarps) {
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int k = 0; k < kPgWarps; ++k) {
+              const float4 y = share[(k * L::kBlocks + c) * 32 + lane];
+              x.x = fmaf(f[k][0], y.x, x.x);
+              x.y = fmaf(f[k][1], y.y, x.y);
+              x.z = fmaf(f[k][0], y.z, x.z);
+              x.w = fmaf(f[k][1], y.w, x.w);
+            }
+            if (done) store_block<BF16, FOUR>(a, seq, r0 + nq * 8, n_rows - nq * 8, w.hk, c, x, l_all);
+            else a.part_o[(static_cast<int64_t>(place * NQ + nq) * L::kBlocks + c) * 32 + lane] = x;
+          }
+          if (warp == 0 && g == 0) {
+            if (done) store_lse(a, seq, r0 + nq * 8, n_rows - nq * 8, w.hk, m_all, l_all);
+            else a.part_ml[(place * NQ + nq) * 4 + t] = make_float4(m_all[0], l_all[0], m_all[1], l_all[1]);
           }
         }
         named_bar_sync(1, 32 * kPgWarps);   // the shares (and at the end the statistics) may be overwritten
@@ -744,62 +774,78 @@ __global__ void __launch_bounds__(kPgThreads, 2) fmha_paged_kernel(const __grid_
   }
 }
 
-// Joins the pieces of a unit that was cut: block c takes the unit that CTA c begins in the middle of, if CTA c - 1 began elsewhere; the
-// pieces are the last part of CTA c - 1 and the first ones of CTA c and all after it that begin in the same unit.
-template <int D, bool BF16>
+// Joins the pieces of a unit that was cut: block c - 1 takes the unit that CTA c begins in the middle of, if CTA c - 1 began elsewhere; the
+// pieces are the last part of CTA c - 1 and the first ones of CTA c and all after it that begin in the same unit.  A warp takes a quarter of the
+// blocks of O^T.  A chain of a few loads, whose latency is all there is to it (the launch itself is hidden under the kernel before): so those that
+// can be are made together.
+template <int D, bool BF16, bool FOUR>
 __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__ PagedArgs a) {
   griddep_wait();
-  const int c = blockIdx.x + 1;   // of a.ctas CTAs
-  const int unit = a.part_info[c].x;
-  const int2 before = a.part_info[c - 1];
+  constexpr int kBlocks = D / 16, kAhead = 4;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = lane & 3, g = lane >> 2;
+  const int c = blockIdx.x + 1, nqs = a.tile_rows / 8, nq = blockIdx.y;
+  const int2 here = a.part_info[c], before = a.part_info[c - 1];
+  int follow = -2;
+  if (c + 1 + lane < a.ctas) follow = a.part_info[c + 1 + lane].x;
+  const int unit = here.x;
   if (unit < 0 || before.x == unit) return;
   int n = 2;   // pieces
-  while (c + n - 1 < a.ctas && a.part_info[c + n - 1].x == unit) ++n;
+  for (int k0 = c + 1;;) {
+    const uint32_t same = __ballot_sync(0xffffffffu, follow == unit);
+    n += same == 0xffffffffu ? 32 : __ffs(~same) - 1;
+    if (same != 0xffffffffu) break;
+    k0 += 32;
+    follow = k0 + lane < a.ctas ? a.part_info[k0 + lane].x : -2;
+  }
   const int hk = unit % a.H_kv, tile = unit / a.H_kv % a.row_tiles, b = unit / a.H_kv / a.row_tiles;
   const PgSeq seq = sequence(a, b);
-  const int r0 = tile * a.tile_rows, n_rows = min(a.tile_rows, seq.n_new * a.group - r0);
-  constexpr int V = D / 32;   // values of a lane; a warp per row
-  const int lane = threadIdx.x & 31;
-  auto place = [&](int k) { return k == 0 ? before.y : 2 * (c + k - 1); };
-  for (int row = threadIdx.x >> 5; row < n_rows; row += 4) {
-    float m_all = -INFINITY;
-    for (int k = lane; k < n; k += 32) m_all = fmaxf(m_all, a.part_ml[place(k) * a.tile_rows + row].x);
+  auto place = [&](int k) { return (k == 0 ? before.y : 2 * (c + k - 1)) * nqs + nq; };
+  // the rows' maxima over all pieces: lane (g, t) looks at every eighth piece
+  float m_all[2] = {-INFINITY, -INFINITY}, l_all[2] = {0.f, 0.f};
+  for (int k = g; k < n; k += 8) {
+    const float4 x = a.part_ml[place(k) * 4 + t];
+    m_all[0] = fmaxf(m_all[0], x.x);
+    m_all[1] = fmaxf(m_all[1], x.z);
+  }
 #pragma unroll
-    for (int k = 16; k > 0; k /= 2) m_all = fmaxf(m_all, __shfl_xor_sync(0xffffffffu, m_all, k));
-    float l_all = 0.f;
-    float acc[V] = {};
-    for (int k0 = 0; k0 < n; k0 += 32) {
-      float f = 0.f;
-      if (k0 + lane < n) {
-        const float2 x = a.part_ml[place(k0 + lane) * a.tile_rows + row];
-        f = x.x == -INFINITY ? 0.f : fast_exp2(x.x - m_all);   // a piece without keys that this row sees
-        l_all = fmaf(f, x.y, l_all);
-      }
-      const int some = min(32, n - k0);
-#pragma unroll 8
-      for (int k = 0; k < some; ++k) {
-        const float fk = __shfl_sync(0xffffffffu, f, k);
-        const float* src = a.part_o + (static_cast<int64_t>(place(k0 + k)) * a.tile_rows + row) * D + lane * V;
-        if constexpr (V == 4) {
-          const float4 x = *reinterpret_cast<const float4*>(src);
-          acc[0] = fmaf(fk, x.x, acc[0]); acc[1] = fmaf(fk, x.y, acc[1]); acc[2] = fmaf(fk, x.z, acc[2]); acc[3] = fmaf(fk, x.w, acc[3]);
-        } else {
-          const float2 x = *reinterpret_cast<const float2*>(src);
-          acc[0] = fmaf(fk, x.x, acc[0]); acc[1] = fmaf(fk, x.y, acc[1]);
-        }
+  for (int k = 4; k < 32; k *= 2) {
+    m_all[0] = fmaxf(m_all[0], __shfl_xor_sync(0xffffffffu, m_all[0], k));
+    m_all[1] = fmaxf(m_all[1], __shfl_xor_sync(0xffffffffu, m_all[1], k));
+  }
+  float4 acc[kBlocks / 4];
+#pragma unroll
+  for (int i = 0; i < kBlocks / 4; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k0 = 0; k0 < n; k0 += kAhead) {
+    float4 st[kAhead], x[kAhead][kBlocks / 4];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      st[k] = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
+      if (k0 + k < n) st[k] = a.part_ml[place(k0 + k) * 4 + t];
+#pragma unroll
+      for (int i = 0; i < kBlocks / 4; ++i) {
+        x[k][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (k0 + k < n) x[k][i] = a.part_o[(static_cast<int64_t>(place(k0 + k)) * kBlocks + warp + 4 * i) * 32 + lane];
       }
     }
 #pragma unroll
-    for (int k = 16; k > 0; k /= 2) l_all += __shfl_xor_sync(0xffffffffu, l_all, k);
-    const float inv = l_all > 0.f ? 1.0f / l_all : 0.f;
-    const int64_t at = seq.row0 + (r0 + row) / a.group;
-    const int h = hk * a.group + (r0 + row) % a.group;
-    unsigned short* dst = static_cast<unsigned short*>(a.o_ptr) + at * a.o_ss + h * a.o_sh + lane * V;
-    if constexpr (V == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<BF16>(acc[0] * inv, acc[1] * inv), pack2<BF16>(acc[2] * inv, acc[3] * inv));
-    else *reinterpret_cast<uint32_t*>(dst) = pack2<BF16>(acc[0] * inv, acc[1] * inv);
-    if (lane == 0 && a.lse != nullptr)
-      a.lse[static_cast<int64_t>(h) * a.total_rows + at] = l_all == 0.f ? -INFINITY : (m_all + fast_log2(l_all)) * kPgLn2;
+    for (int k = 0; k < kAhead; ++k) {
+      const float f0 = st[k].x == -INFINITY ? 0.f : fast_exp2(st[k].x - m_all[0]);   // a piece without keys that this row sees counts nothing
+      const float f1 = st[k].z == -INFINITY ? 0.f : fast_exp2(st[k].z - m_all[1]);
+      l_all[0] = fmaf(f0, st[k].y, l_all[0]);
+      l_all[1] = fmaf(f1, st[k].w, l_all[1]);
+#pragma unroll
+      for (int i = 0; i < kBlocks / 4; ++i) {
+        acc[i].x = fmaf(f0, x[k][i].x, acc[i].x);
+        acc[i].y = fmaf(f1, x[k][i].y, acc[i].y);
+        acc[i].z = fmaf(f0, x[k][i].z, acc[i].z);
+        acc[i].w = fmaf(f1, x[k][i].w, acc[i].w);
+      }
+    }
   }
+  const int r0 = tile * a.tile_rows + nq * 8, n_rows = min(8, seq.n_new * a.group - r0);
+#pragma unroll
+  for (int i = 0; i < kBlocks / 4; ++i) store_block<BF16, FOUR>(a, seq, r0, n_rows, hk, warp + 4 * i, acc[i], l_all);
+  if (warp == 0 && g == 0) store_lse(a, seq, r0, n_rows, hk, m_all, l_all);
 }
 
 // Where no sequence can have more keys than a CTA takes at the least, units stay whole (no workspace, no second kernel).  Else two CTAs per SM, but no
@@ -823,9 +869,9 @@ void paged_places(PagedArgs& a, void* workspace, const PagedGrid& g, int D) {
   a.row_tiles = static_cast<int>(g.row_tiles);
   if (g.whole) return;
   const size_t rows = static_cast<size_t>(g.ctas) * 2 * g.tile_rows;
-  a.part_o = static_cast<float*>(workspace);
-  a.part_ml = reinterpret_cast<float2*>(a.part_o + rows * D);
-  a.part_info = reinterpret_cast<int2*>(a.part_ml + rows);
+  a.part_o = static_cast<float4*>(workspace);
+  a.part_ml = a.part_o + rows * D / 4;
+  a.part_info = reinterpret_cast<int2*>(a.part_ml + rows / 2);
 }
 
 template <int D, bool BF16, bool FOUR, int NQ>
@@ -841,7 +887,7 @@ static int launch_paged_impl(const PagedArgs& a, cudaStream_t stream) {
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
   cudaError_t e = launch_overlapped(kfn, dim3(a.ctas), dim3(kPgThreads), L::kDynBytes, stream, a);
-  if (e == cudaSuccess && !a.whole && a.ctas > 1) e = launch_overlapped(paged_join_kernel<D, BF16>, dim3(a.ctas - 1), dim3(128), 0, stream, a);
+  if (e == cudaSuccess && !a.whole && a.ctas > 1) e = launch_overlapped(paged_join_kernel<D, BF16, FOUR>, dim3(a.ctas - 1, NQ), dim3(128), 0, stream, a);
   return static_cast<int>(e != cudaSuccess ? e : cudaGetLastError());
 }
 
