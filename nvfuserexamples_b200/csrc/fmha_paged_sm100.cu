@@ -40,6 +40,7 @@ namespace {
 constexpr int kPgWarps = 4;   // consumer warps
 constexpr int kPgThreads = 32 * (kPgWarps + 1);
 constexpr int kPgMinKeys = 256;   // a CTA's piece of the line holds at least so many
+constexpr int kPgUnitCost = 2;    // what a unit counts in the line beside its steps: its queries, its write-out
 constexpr float kPgLn2 = 0.6931471805599453f;
 
 enum PgWaitSite { kPgFull = 191, kPgEmpty = 192, kPgSmemBase = 193 };
@@ -145,7 +146,8 @@ __device__ __forceinline__ int keys_of(const PagedArgs& a, const PgSeq& s, int r
   const int64_t most = static_cast<int64_t>(a.table_width) * a.page_rows;
   return static_cast<int>(max(min(static_cast<int64_t>(s.len) - s.n_all + row + 1, most), static_cast<int64_t>(0)));
 }
-// A group of units: the key heads of a tile of query rows.
+// A group of units: the key heads of a tile of query rows.  A unit's place in the line is its steps and kPgUnitCost more in front of them (without which
+// CTAs with many short units were the last by far: B=16, 200 to 4000 keys, a CTA's switch from unit to unit takes as long as two steps).
 struct PgGroup {
   int n_rows, k_limit, steps, weight;   // rows that exist; keys that the last of them sees; what a unit of it counts in the line
 };
@@ -157,7 +159,7 @@ __device__ __forceinline__ PgGroup group_of(const PagedArgs& a, int b, int tile,
   if (u.n_rows <= 0) return u;
   u.k_limit = keys_of(a, s, (r0 + u.n_rows - 1) / a.group);
   u.steps = (u.k_limit + keys - 1) / keys;
-  u.weight = a.whole ? 1 : max(1, u.steps);   // rows that see no key are written as well
+  u.weight = a.whole ? 1 : u.steps + kPgUnitCost;   // rows that see no key are written as well
   return u;
 }
 
@@ -175,33 +177,39 @@ __device__ __forceinline__ void way_part(const PagedArgs& a, PgWay& w, int off) 
   const int take = min(w.u.weight - off, w.left);
   w.first = off == 0;
   w.last = off + take == w.u.weight;
-  w.j0 = a.whole ? 0 : min(off, w.u.steps);
-  w.j1 = a.whole ? w.u.steps : min(off + take, w.u.steps);
+  w.j0 = a.whole ? 0 : max(off - kPgUnitCost, 0);
+  w.j1 = a.whole ? w.u.steps : max(off + take - kPgUnitCost, 0);
   w.left -= take;
 }
-// False: nothing for this CTA.
+// False: nothing for this CTA.  Lanes look at 32 groups together; up to 32 of them the lengths are read once.
 template <int KEYS>
 __device__ __forceinline__ bool way_begin(const PagedArgs& a, PgWay& w) {
   const int lane = threadIdx.x & 31;
   w.tiles = a.row_tiles;
   w.groups = a.B * w.tiles;
+  auto look = [&](int g) {
+    PgGroup u = {0, 0, 0, 0};
+    if (g < w.groups) u = w.tiles == 1 ? group_of(a, g, 0, KEYS) : group_of(a, g / w.tiles, g % w.tiles, KEYS);
+    return u;
+  };
+  PgGroup u = look(lane);
   long long total = 0;
-  int mine = 0;   // weight of the lane's group among the first 32
-  for (int g0 = 0; g0 < w.groups; g0 += 32) {
-    const int g = g0 + lane, x = g < w.groups ? group_of(a, g / w.tiles, g % w.tiles, KEYS).weight : 0;
-    if (g0 == 0) mine = x;
-    total += __reduce_add_sync(0xffffffffu, x);
+  for (int g0 = 0;;) {
+    total += __reduce_add_sync(0xffffffffu, u.weight);
+    if ((g0 += 32) >= w.groups) break;
+    u = look(g0 + lane);
   }
   total *= a.H_kv;
-  const long long least = a.whole ? 1 : kPgMinKeys / KEYS;
-  const long long chunk = max(least, (total + gridDim.x - 1) / gridDim.x);
+  const int least = a.whole ? 1 : kPgMinKeys / KEYS + kPgUnitCost, ctas = gridDim.x;
+  // a piece of the line (in 32 bits, where a division takes a third of the time, if the line is that short)
+  const long long chunk = max(static_cast<long long>(least), total < (1ll << 30) ? (static_cast<int>(total) + ctas - 1) / ctas : (total + ctas - 1) / ctas);
   const long long w0 = chunk * blockIdx.x;
   if (w0 >= total) return false;
   w.left = static_cast<int>(min(chunk, total - w0));
   long long before = 0;   // of the groups passed
-  for (int g0 = 0;; g0 += 32) {
-    const int g = g0 + lane, x = g0 == 0 ? mine : g < w.groups ? group_of(a, g / w.tiles, g % w.tiles, KEYS).weight : 0;
-    int sum = x;   // inclusive
+  if (w.groups > 32) u = look(lane);
+  for (int g0 = 0;; u = look(g0 + lane)) {
+    int sum = u.weight;   // inclusive
 #pragma unroll
     for (int m = 1; m < 32; m *= 2) {
       const int y = __shfl_up_sync(0xffffffffu, sum, m);
@@ -211,18 +219,22 @@ __device__ __forceinline__ bool way_begin(const PagedArgs& a, PgWay& w) {
     if (beyond != 0u) {
       const int at = __ffs(beyond) - 1;
       w.g = g0 + at;
-      before += __shfl_sync(0xffffffffu, sum - x, at);
+      before += __shfl_sync(0xffffffffu, sum - u.weight, at);
+      w.u.n_rows = __shfl_sync(0xffffffffu, u.n_rows, at);
+      w.u.k_limit = __shfl_sync(0xffffffffu, u.k_limit, at);
+      w.u.steps = __shfl_sync(0xffffffffu, u.steps, at);
+      w.u.weight = __shfl_sync(0xffffffffu, u.weight, at);
       break;
     }
     before += __shfl_sync(0xffffffffu, sum, 31);
+    g0 += 32;
   }
-  w.b = w.g / w.tiles;
-  w.tile = w.g % w.tiles;
-  w.u = group_of(a, w.b, w.tile, KEYS);
+  w.b = w.tiles == 1 ? w.g : w.g / w.tiles;
+  w.tile = w.g - w.b * w.tiles;
   const int within = static_cast<int>(w0 - before * a.H_kv);
   w.hk = within / w.u.weight;
   w.n = 0;
-  way_part<KEYS>(a, w, within % w.u.weight);
+  way_part<KEYS>(a, w, within - w.hk * w.u.weight);
   return true;
 }
 template <int KEYS>
@@ -304,26 +316,12 @@ __global__ void __launch_bounds__(kPgThreads, 2) fmha_paged_kernel(const __grid_
     }
     mbar_fence_init();
   }
-  // Rows that no unit stands for: outside the sequences, or past max_rows of theirs.
-  {
-    auto zero = [&](int64_t from, int64_t to) {
-      from = max(from, static_cast<int64_t>(0));
-      to = min(to, static_cast<int64_t>(a.total_rows));
-      const int per_row = a.H * (D / 8);
-      for (int64_t i = threadIdx.x; i < (to - from) * per_row; i += kPgThreads) {
-        const int64_t row = from + i / per_row;
-        const int h = static_cast<int>(i % per_row) / (D / 8), ch = static_cast<int>(i % (D / 8));
-        *reinterpret_cast<uint4*>(static_cast<unsigned short*>(a.o_ptr) + row * a.o_ss + h * a.o_sh + ch * 8) = make_uint4(0u, 0u, 0u, 0u);
-        if (ch == 0 && a.lse != nullptr) a.lse[static_cast<int64_t>(h) * a.total_rows + row] = -INFINITY;
-      }
-    };
-    if (a.cu != nullptr) {
-      for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
-        const int64_t from = a.cu[b], to = a.cu[b + 1];
-        if (to - from > a.max_rows) zero(from + a.max_rows, to);
-        if (b == 0) zero(0, from);
-        if (b == a.B - 1) zero(max(from, to), a.total_rows);
-      }
+  if (threadIdx.x == 32) {
+    tma_prefetch_desc(&a.tm_k);
+    tma_prefetch_desc(&a.tm_v);
+    if constexpr (FOUR) {
+      tma_prefetch_desc(&a.tm_kp);
+      tma_prefetch_desc(&a.tm_vp);
     }
   }
   PgWay w;
@@ -331,9 +329,10 @@ __global__ void __launch_bounds__(kPgThreads, 2) fmha_paged_kernel(const __grid_
   // What the second kernel needs to know: the unit that this CTA begins in the middle of, and which of its two places its last part is in.
   if (threadIdx.x == 0 && a.part_info != nullptr) a.part_info[blockIdx.x] = make_int2(any && !w.first ? w.g * a.H_kv + w.hk : -1, -1);
   __syncthreads();
-  if (!any) return;
 
-  if (warp == kPgWarps) {
+  if (!any) {
+    // nothing of the line
+  } else if (warp == kPgWarps) {
     // ============================ TMA producer ======================================
     // Lane i brings piece i of the step: the page number of the next step is read while this one's buffers are waited for.
     const int pieces = KEYS / a.piece;   // up to 8
@@ -767,6 +766,28 @@ __global__ void __launch_bounds__(kPgThreads, 2) fmha_paged_kernel(const __grid_
       if (tid == 0 && !w.last) a.part_info[blockIdx.x].y = place;   // the CTA's last part, whose unit goes on in the next CTA
     } while (way_next<KEYS>(a, w));
   }
+  // Rows that no unit stands for: outside the sequences, or past max_rows of theirs.
+  {
+    auto zero = [&](int64_t from, int64_t to) {
+      from = max(from, static_cast<int64_t>(0));
+      to = min(to, static_cast<int64_t>(a.total_rows));
+      const int per_row = a.H * (D / 8);
+      for (int64_t i = threadIdx.x; i < (to - from) * per_row; i += kPgThreads) {
+        const int64_t row = from + i / per_row;
+        const int h = static_cast<int>(i % per_row) / (D / 8), ch = static_cast<int>(i % (D / 8));
+        *reinterpret_cast<uint4*>(static_cast<unsigned short*>(a.o_ptr) + row * a.o_ss + h * a.o_sh + ch * 8) = make_uint4(0u, 0u, 0u, 0u);
+        if (ch == 0 && a.lse != nullptr) a.lse[static_cast<int64_t>(h) * a.total_rows + row] = -INFINITY;
+      }
+    };
+    if (a.cu != nullptr) {
+      for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
+        const int64_t from = a.cu[b], to = a.cu[b + 1];
+        if (to - from > a.max_rows) zero(from + a.max_rows, to);
+        if (b == 0) zero(0, from);
+        if (b == a.B - 1) zero(max(from, to), a.total_rows);
+      }
+    }
+  }
   __syncthreads();
   if (*abort_flag) {
     for (int k = 0; k < 20; ++k) __nanosleep(1000000);   // copies in flight end before the CTA does
@@ -775,14 +796,14 @@ __global__ void __launch_bounds__(kPgThreads, 2) fmha_paged_kernel(const __grid_
 }
 
 // Joins the pieces of a unit that was cut: block c - 1 takes the unit that CTA c begins in the middle of, if CTA c - 1 began elsewhere; the
-// pieces are the last part of CTA c - 1 and the first ones of CTA c and all after it that begin in the same unit.  A warp takes a quarter of the
-// blocks of O^T.  A chain of a few loads, whose latency is all there is to it (the launch itself is hidden under the kernel before): so those that
-// can be are made together.
+// pieces are the last part of CTA c - 1 and the first ones of CTA c and all after it that begin in the same unit.  A warp takes a block of O^T (16
+// dimensions).  All there is to it is a chain of loads, so those that can be are made together: which pieces there are, then the first eight of them and
+// their statistics (its launch is hidden under the kernel before it).
 template <int D, bool BF16, bool FOUR>
-__global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__ PagedArgs a) {
+__global__ void __launch_bounds__(2 * D) paged_join_kernel(const __grid_constant__ PagedArgs a) {
   griddep_wait();
-  constexpr int kBlocks = D / 16, kAhead = 4;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = lane & 3, g = lane >> 2;
+  constexpr int kBlocks = D / 16, kAhead = 8;
+  const int lane = threadIdx.x & 31, block = threadIdx.x >> 5, t = lane & 3, g = lane >> 2;
   const int c = blockIdx.x + 1, nqs = a.tile_rows / 8, nq = blockIdx.y;
   const int2 here = a.part_info[c], before = a.part_info[c - 1];
   int follow = -2;
@@ -797,55 +818,63 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
     k0 += 32;
     follow = k0 + lane < a.ctas ? a.part_info[k0 + lane].x : -2;
   }
+  auto place = [&](int k) { return (k == 0 ? before.y : 2 * (c + k - 1)) * nqs + nq; };
+  float4 x[kAhead];
+  auto load = [&](int k0) {
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (k0 + k < n) x[k] = a.part_o[(static_cast<int64_t>(place(k0 + k)) * kBlocks + block) * 32 + lane];
+    }
+  };
+  load(0);
+  // maxima and sums of rows 2t and 2t + 1: lane (g, t) looks at pieces g, g + 8, ...; up to 32 of them are read once
+  float4 st[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    st[k] = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
+    if (8 * k + g < n) st[k] = a.part_ml[place(8 * k + g) * 4 + t];
+  }
   const int hk = unit % a.H_kv, tile = unit / a.H_kv % a.row_tiles, b = unit / a.H_kv / a.row_tiles;
   const PgSeq seq = sequence(a, b);
-  auto place = [&](int k) { return (k == 0 ? before.y : 2 * (c + k - 1)) * nqs + nq; };
-  // the rows' maxima over all pieces: lane (g, t) looks at every eighth piece
-  float m_all[2] = {-INFINITY, -INFINITY}, l_all[2] = {0.f, 0.f};
-  for (int k = g; k < n; k += 8) {
-    const float4 x = a.part_ml[place(k) * 4 + t];
-    m_all[0] = fmaxf(m_all[0], x.x);
-    m_all[1] = fmaxf(m_all[1], x.z);
+  float m_all[2] = {fmaxf(fmaxf(st[0].x, st[1].x), fmaxf(st[2].x, st[3].x)), fmaxf(fmaxf(st[0].z, st[1].z), fmaxf(st[2].z, st[3].z))};
+  for (int k = 32 + g; k < n; k += 8) {
+    const float4 y = a.part_ml[place(k) * 4 + t];
+    m_all[0] = fmaxf(m_all[0], y.x);
+    m_all[1] = fmaxf(m_all[1], y.z);
   }
 #pragma unroll
   for (int k = 4; k < 32; k *= 2) {
     m_all[0] = fmaxf(m_all[0], __shfl_xor_sync(0xffffffffu, m_all[0], k));
     m_all[1] = fmaxf(m_all[1], __shfl_xor_sync(0xffffffffu, m_all[1], k));
   }
-  float4 acc[kBlocks / 4];
-#pragma unroll
-  for (int i = 0; i < kBlocks / 4; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  float l_all[2] = {0.f, 0.f};
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int k0 = 0; k0 < n; k0 += kAhead) {
-    float4 st[kAhead], x[kAhead][kBlocks / 4];
+    // factors of the eight pieces, of this lane's one: a piece without keys that a row sees counts nothing
+    float4 s = st[0];
+    if (k0 > 0) s = k0 + g < n ? a.part_ml[place(k0 + g) * 4 + t] : make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
+    const float f0 = s.x == -INFINITY ? 0.f : fast_exp2(s.x - m_all[0]), f1 = s.z == -INFINITY ? 0.f : fast_exp2(s.z - m_all[1]);
+    l_all[0] = fmaf(f0, s.y, l_all[0]);
+    l_all[1] = fmaf(f1, s.w, l_all[1]);
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
-      st[k] = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
-      if (k0 + k < n) st[k] = a.part_ml[place(k0 + k) * 4 + t];
-#pragma unroll
-      for (int i = 0; i < kBlocks / 4; ++i) {
-        x[k][i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (k0 + k < n) x[k][i] = a.part_o[(static_cast<int64_t>(place(k0 + k)) * kBlocks + warp + 4 * i) * 32 + lane];
-      }
+      const float k_f0 = __shfl_sync(0xffffffffu, f0, 4 * k + t), k_f1 = __shfl_sync(0xffffffffu, f1, 4 * k + t);
+      acc.x = fmaf(k_f0, x[k].x, acc.x);
+      acc.y = fmaf(k_f1, x[k].y, acc.y);
+      acc.z = fmaf(k_f0, x[k].z, acc.z);
+      acc.w = fmaf(k_f1, x[k].w, acc.w);
     }
+    if (k0 + kAhead < n) load(k0 + kAhead);
+  }
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      const float f0 = st[k].x == -INFINITY ? 0.f : fast_exp2(st[k].x - m_all[0]);   // a piece without keys that this row sees counts nothing
-      const float f1 = st[k].z == -INFINITY ? 0.f : fast_exp2(st[k].z - m_all[1]);
-      l_all[0] = fmaf(f0, st[k].y, l_all[0]);
-      l_all[1] = fmaf(f1, st[k].w, l_all[1]);
-#pragma unroll
-      for (int i = 0; i < kBlocks / 4; ++i) {
-        acc[i].x = fmaf(f0, x[k][i].x, acc[i].x);
-        acc[i].y = fmaf(f1, x[k][i].y, acc[i].y);
-        acc[i].z = fmaf(f0, x[k][i].z, acc[i].z);
-        acc[i].w = fmaf(f1, x[k][i].w, acc[i].w);
-      }
-    }
+  for (int k = 4; k < 32; k *= 2) {
+    l_all[0] += __shfl_xor_sync(0xffffffffu, l_all[0], k);
+    l_all[1] += __shfl_xor_sync(0xffffffffu, l_all[1], k);
   }
   const int r0 = tile * a.tile_rows + nq * 8, n_rows = min(8, seq.n_new * a.group - r0);
-#pragma unroll
-  for (int i = 0; i < kBlocks / 4; ++i) store_block<BF16, FOUR>(a, seq, r0, n_rows, hk, warp + 4 * i, acc[i], l_all);
-  if (warp == 0 && g == 0) store_lse(a, seq, r0, n_rows, hk, m_all, l_all);
+  store_block<BF16, FOUR>(a, seq, r0, n_rows, hk, block, acc, l_all);
+  if (block == 0 && g == 0) store_lse(a, seq, r0, n_rows, hk, m_all, l_all);
 }
 
 // Where no sequence can have more keys than a CTA takes at the least, units stay whole (no workspace, no second kernel).  Else two CTAs per SM, but no
@@ -887,7 +916,7 @@ static int launch_paged_impl(const PagedArgs& a, cudaStream_t stream) {
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
   cudaError_t e = launch_overlapped(kfn, dim3(a.ctas), dim3(kPgThreads), L::kDynBytes, stream, a);
-  if (e == cudaSuccess && !a.whole && a.ctas > 1) e = launch_overlapped(paged_join_kernel<D, BF16, FOUR>, dim3(a.ctas - 1, NQ), dim3(128), 0, stream, a);
+  if (e == cudaSuccess && !a.whole && a.ctas > 1) e = launch_overlapped(paged_join_kernel<D, BF16, FOUR>, dim3(a.ctas - 1, NQ), dim3(2 * D), 0, stream, a);
   return static_cast<int>(e != cudaSuccess ? e : cudaGetLastError());
 }
 
