@@ -718,7 +718,8 @@ static int launch_dq_impl(const BwdArgs& a, cudaStream_t stream) {
   // matters: forward and backward fused / separate, 768 keys 276.6 / 280.1, with lengths 247.6 / 249.3, 1024 keys 310 / 315, with
   // dropout 364.5 / 368.6, 1280 keys 404.8 / 409.6, 487.7 / 495.0 with dropout, where runs of one side differ by up to 4 %.
   args.persist = static_cast<int64_t>(grid.x) * grid.y * grid.z > sm_count();
-  if (args.persist && a.S_k <= kDeltaPassKeys) {
+  // Causal items have half as many key tiles on the average, and the first of a sequence one or two.
+  if (args.persist && (CAUSAL || a.S_k <= kDeltaPassKeys)) {
     const cudaError_t e = launch_overlapped(bwd_delta_kernel<BF16>, dim3(static_cast<unsigned>(a.B) * a.H, (a.S_q + 63) / 64), dim3(256), 0,
                                             stream, a);
     if (e != cudaSuccess) return static_cast<int>(e);

@@ -315,7 +315,8 @@ struct BwdItem {
 // 16.6 -> 13.0, B=32 H=16 S=128 27.8 -> 19.5 / 29.1 -> 23.0, B=128 H=16 94.4 -> 68.3 / 97.8 -> 75.7; packed, B=32 H=16 of 64 to 128 rows 34.2 -> 27.7 / 36.1 -> 31.2).
 // CAUSAL: a packed batch whose rows see the keys up to their own position, with a.kv_group query heads to a key head.  An item is a key tile of
 // a KEY head: its query tiles are those from the diagonal on of every query head of the group, one head after the other, so dK and dV are summed
-// over the group in tensor memory, always in the same order.  Items count heads and sequences first and key tiles, longest first, last.
+// over the group in tensor memory, always in the same order.  Items count heads and sequences first and, last, the number of query tiles from the
+// diagonal on, most first: an item that begins late must not be a long one.
 // Rows of Q, dO and K behind the end of the sequence are zeroed in shared memory: they are contracted over.
 template <int D, bool BF16, bool KEYADD, bool DROP, bool PACKED = false, bool ONE_KV = false, bool CAUSAL = false>
 __global__ void __launch_bounds__(kBwdThreads, 1) fmha_bwd_kernel(const __grid_constant__ BwdArgs a) {
@@ -438,7 +439,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) fmha_bwd_kernel(const __grid_c
     it.row_base = 0;
     if (id >= 0) {
       const int heads = CAUSAL ? a.H_kv : a.H;
-      const int kv_tile = CAUSAL ? id / (heads * a.B) : id % kv_tiles;
+      int kv_tile = CAUSAL ? 0 : id % kv_tiles;
       const int bh = CAUSAL ? id % (heads * a.B) : id / kv_tiles;
       it.h = bh % heads;   // CAUSAL: the key head
       it.b = bh / heads;
@@ -454,6 +455,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1) fmha_bwd_kernel(const __grid_c
         // head's rows of the dQ accumulator and of delta
         k_limit = it.q_limit = packed_rows(it.row_base, cu[it.b + 1], a.S_q, a.total_rows);
         it.n_q = (it.q_limit + kTileM - 1) / kTileM;
+        if constexpr (CAUSAL) {   // the key tile with kv_tiles - level query tiles from its diagonal on, if the sequence has as many
+          kv_tile = it.n_q - kv_tiles + id / (heads * a.B);
+          it.k0 = kv_tile * kTileN;
+          if (kv_tile < 0) k_limit = it.k0;
+        }
       }
       it.n_cols = min(kTileN, k_limit - it.k0);
       if constexpr (CAUSAL) it.n_q = (it.n_q - kv_tile) * a.kv_group;
@@ -498,7 +504,13 @@ __global__ void __launch_bounds__(kBwdThreads, 1) fmha_bwd_kernel(const __grid_c
       int next = static_cast<int>(blockIdx.x);
       for (int n = 0;; ++n) {
         const int slot = n & 1;
-        const BwdItem it = decode(next < num_items && !*abort_flag ? next : -1);
+        BwdItem it = decode(next < num_items && !*abort_flag ? next : -1);
+        if constexpr (CAUSAL) {   // tiles that a sequence does not have are passed over here: published, they would keep the producer from running ahead
+          while (it.id >= 0 && it.n_cols <= 0) {
+            next = atomicAdd(a.work_counter, 1) + static_cast<int>(gridDim.x);
+            it = decode(next < num_items && !*abort_flag ? next : -1);
+          }
+        }
         if (n >= 2) mbar_wait(item_empty + slot, ((n >> 1) - 1) & 1, wctx, kSiteItemEmpty);
         sts128(ring + slot * 32, static_cast<uint32_t>(it.id), static_cast<uint32_t>(it.b), static_cast<uint32_t>(it.h),
                static_cast<uint32_t>(it.k0));

@@ -40,7 +40,7 @@ namespace {
 constexpr int kPgWarps = 4;   // consumer warps
 constexpr int kPgThreads = 32 * (kPgWarps + 1);
 constexpr int kPgMinKeys = 256;   // a CTA's piece of the line holds at least so many
-constexpr int kPgUnitCost = 2;    // what a unit counts in the line beside its steps: its queries, its write-out
+constexpr int kPgUnitCost = 4;    // what a unit counts in the line beside its steps: its queries, its write-out
 constexpr float kPgLn2 = 0.6931471805599453f;
 
 enum PgWaitSite { kPgFull = 191, kPgEmpty = 192, kPgSmemBase = 193 };
@@ -147,7 +147,8 @@ __device__ __forceinline__ int keys_of(const PagedArgs& a, const PgSeq& s, int r
   return static_cast<int>(max(min(static_cast<int64_t>(s.len) - s.n_all + row + 1, most), static_cast<int64_t>(0)));
 }
 // A group of units: the key heads of a tile of query rows.  A unit's place in the line is its steps and kPgUnitCost more in front of them (without which
-// CTAs with many short units were the last by far: B=16, 200 to 4000 keys, a CTA's switch from unit to unit takes as long as two steps).
+// CTAs with many short units were the last by far, for a switch from unit to unit takes as long as two to four steps: B=16, 200 to 4000 keys 45.6 us, with
+// 2 more 36.2, 3 34.9, 4 34.9, 6 35.0; B=32, 1000 to 8192 keys in 4 bits 52.4, 48.2, 47.7, 46.8, 48.9).
 struct PgGroup {
   int n_rows, k_limit, steps, weight;   // rows that exist; keys that the last of them sees; what a unit of it counts in the line
 };
@@ -291,13 +292,13 @@ __device__ __forceinline__ void store_lse(const PagedArgs& a, const PgSeq& seq, 
 
 template <int D, bool BF16, bool FOUR, int NQ>
 __global__ void __launch_bounds__(kPgThreads, 2) fmha_paged_kernel(const __grid_constant__ PagedArgs a) {
-  griddep_wait();
   using L = PgSmem<D, FOUR, NQ>;
   constexpr int ST = L::kStages, UN = L::kUnits, KEYS = L::kKeys, ROWS = 8 * NQ;
   constexpr bool MMA_BF16 = BF16 && !FOUR;
   constexpr float kLazy = FOUR ? 0.f : 8.f;
   extern __shared__ __align__(1024) uint8_t smem[];
   if (smem_u32(smem) & 1023) {
+    griddep_wait();
     if (threadIdx.x == 0 && a.status != nullptr) atomicCAS(a.status, 0, kPgSmemBase);
     return;
   }
@@ -324,6 +325,7 @@ __global__ void __launch_bounds__(kPgThreads, 2) fmha_paged_kernel(const __grid_
       tma_prefetch_desc(&a.tm_vp);
     }
   }
+  griddep_wait();   // up to here nothing of global memory has been touched
   PgWay w;
   const bool any = way_begin<KEYS>(a, w);
   // What the second kernel needs to know: the unit that this CTA begins in the middle of, and which of its two places its last part is in.
