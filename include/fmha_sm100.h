@@ -308,6 +308,7 @@ int fmha_sm100_bwd_static_scratch(const fmha_bwd_params* p, void* stream);
 /* Causal attention of packed sequences with grouped heads, and its gradients. */
 int fmha_sm100_causal_fwd(const fmha_causal_fwd_params* p, void* stream);
 int fmha_sm100_causal_bwd(const fmha_causal_bwd_params* p, void* stream);
+/* (depends on the sizes, total_rows among them, and on the current device) */
 int fmha_sm100_causal_bwd_workspace_bytes(const fmha_causal_bwd_params* p, size_t* bytes);
 
 /* Paged caches: appending rows, reading rows back, attention of a few new rows.  fmha_sm100_paged_workspace_bytes may give 0 (no sequence's

@@ -290,7 +290,8 @@ __global__ void __launch_bounds__(kDqThreads, 1) fmha_bwd_dq_kernel(const __grid
           for (int c = 0; c < 2; ++c) tma_load_4d(sV + c * 16384, &a.tm_v, v_full, c * 64, it.row_base + j * kTileN, hk, it.tb);
           // Early, for the statistics warps need the next item's rows in time; but the first time not at once: on a chip
           // that is still filling up, the CTA asked for may be about to start on an idle SM.
-          if (persist && j == (w == 0 ? min(2, it.n_kv - 1) : 0)) request_item(n + 1);
+          // (causal items differ in length: as late as the loads allow)
+          if (persist && j == (CAUSAL ? it.n_kv - 1 : w == 0 ? min(2, it.n_kv - 1) : 0)) request_item(n + 1);
         }
         __syncwarp();
         if constexpr (KEYADD) {   // the slot is free: its K stage was

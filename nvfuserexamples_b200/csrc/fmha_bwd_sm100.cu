@@ -316,7 +316,8 @@ struct BwdItem {
 // CAUSAL: a packed batch whose rows see the keys up to their own position, with a.kv_group query heads to a key head.  An item is a key tile of
 // a KEY head: its query tiles are those from the diagonal on of every query head of the group, one head after the other, so dK and dV are summed
 // over the group in tensor memory, always in the same order.  Items count heads and sequences first and, last, the number of query tiles from the
-// diagonal on, most first: an item that begins late must not be a long one.
+// diagonal on, most first: an item that begins late must not be a long one.  Where one item would outlast all the others (few key heads, long sequences), the
+// query heads of a key head are dealt out over a.kv_parts items, which leave their fp32 sums in the workspace for bwd_join_kernel (bwd_causal_parts).
 // Rows of Q, dO and K behind the end of the sequence are zeroed in shared memory: they are contracted over.
 template <int D, bool BF16, bool KEYADD, bool DROP, bool PACKED = false, bool ONE_KV = false, bool CAUSAL = false>
 __global__ void __launch_bounds__(kBwdThreads, 1) fmha_bwd_kernel(const __grid_constant__ BwdArgs a) {
@@ -376,7 +377,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1) fmha_bwd_kernel(const __grid_c
   const int kv_tiles = (a.S_k + kTileN - 1) / kTileN;
   const int n_q_all = (a.S_q + kTileM - 1) / kTileM;
   static_assert(!CAUSAL || (PACKED && !KEYADD && !DROP && !ONE_KV), "causal: packed batches without dropout");
-  const int num_items = kv_tiles * (CAUSAL ? a.H_kv : a.H) * a.B;
+  const int item_heads = CAUSAL ? a.H_kv * a.kv_parts : a.H, item_group = CAUSAL ? a.kv_group / a.kv_parts : 1;
+  const int num_items = kv_tiles * item_heads * a.B;
   constexpr bool packed = PACKED;
 
   if (threadIdx.x == 0) {
@@ -438,10 +440,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1) fmha_bwd_kernel(const __grid_c
     it.q_limit = a.S_q;
     it.row_base = 0;
     if (id >= 0) {
-      const int heads = CAUSAL ? a.H_kv : a.H;
+      const int heads = item_heads;
       int kv_tile = CAUSAL ? 0 : id % kv_tiles;
       const int bh = CAUSAL ? id % (heads * a.B) : id / kv_tiles;
-      it.h = bh % heads;   // CAUSAL: the key head
+      it.h = bh % heads;   // CAUSAL: key head and part
       it.b = bh / heads;
       it.k0 = kv_tile * kTileN;
       int k_limit = a.S_k;
@@ -462,7 +464,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) fmha_bwd_kernel(const __grid_c
         }
       }
       it.n_cols = min(kTileN, k_limit - it.k0);
-      if constexpr (CAUSAL) it.n_q = (it.n_q - kv_tile) * a.kv_group;
+      if constexpr (CAUSAL) it.n_q = (it.n_q - kv_tile) * item_group;
     }
     return it;
   };
@@ -470,7 +472,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) fmha_bwd_kernel(const __grid_c
   struct QTile {
     int tile, h;
   };
-  auto first_q = [&](const BwdItem& it) { return CAUSAL ? QTile{it.k0 / kTileN, it.h * a.kv_group} : QTile{0, it.h}; };
+  auto first_q = [&](const BwdItem& it) { return CAUSAL ? QTile{it.k0 / kTileN, it.h * item_group} : QTile{0, it.h}; };
   auto next_q = [&](const BwdItem& it, QTile& x) {
     ++x.tile;
     if constexpr (CAUSAL) {
@@ -519,16 +521,16 @@ __global__ void __launch_bounds__(kBwdThreads, 1) fmha_bwd_kernel(const __grid_c
         mbar_arrive(item_full + slot);
         if (it.id < 0) break;
         if constexpr (ONE_KV) next += static_cast<int>(gridDim.x);
-        else next = atomicAdd(a.work_counter, 1) + static_cast<int>(gridDim.x);   // not looked at before this item's loads are out
+        else if constexpr (!CAUSAL) next = atomicAdd(a.work_counter, 1) + static_cast<int>(gridDim.x);   // not looked at before this item's loads are out
         const int tb = packed ? 0 : it.b;
         if (it.n_cols <= 0) continue;
-        const int kvb = w % KV;
+        const int kvb = w % KV, hk = CAUSAL ? it.h / a.kv_parts : it.h;
         const uint32_t kvp = (w / KV - 1) & 1;
         if (w >= KV) mbar_wait(k_empty + kvb, kvp, wctx, kSiteKEmpty);
         mbar_arrive_expect_tx(k_full + kvb, L::kTileBytes);
 #pragma unroll
         for (int c = 0; c < D / 64; ++c)
-          tma_load_4d(sK + kvb * L::kTileBytes + c * 16384, &a.tm_k, k_full + kvb, c * 64, it.row_base + it.k0, it.h, tb);
+          tma_load_4d(sK + kvb * L::kTileBytes + c * 16384, &a.tm_k, k_full + kvb, c * 64, it.row_base + it.k0, hk, tb);
         QTile q = first_q(it);
         for (int i = 0; i < it.n_q; ++i, ++g, next_q(it, q)) {
           const int qs = g % QS, os = g % OS;
@@ -542,7 +544,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) fmha_bwd_kernel(const __grid_c
             mbar_arrive_expect_tx(v_full + kvb, L::kTileBytes);
 #pragma unroll
             for (int c = 0; c < D / 64; ++c)
-              tma_load_4d(sV + kvb * L::kTileBytes + c * 16384, &a.tm_v, v_full + kvb, c * 64, it.row_base + it.k0, it.h, tb);
+              tma_load_4d(sV + kvb * L::kTileBytes + c * 16384, &a.tm_v, v_full + kvb, c * 64, it.row_base + it.k0, hk, tb);
           }
           if (g >= OS) mbar_wait(do_empty + os, ((g / OS) - 1) & 1, wctx, kSiteDoEmpty);
           mbar_arrive_expect_tx(do_full + os, L::kTileBytes);
@@ -551,6 +553,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1) fmha_bwd_kernel(const __grid_c
             tma_load_4d(sdO + os * L::kTileBytes + c * 16384, &a.tm_do, do_full + os, c * 64, it.row_base + q.tile * kTileM, q.h, tb);
         }
         ++w;
+        // Items of unequal length: the next one is taken when this one's last loads are out, two query tiles before its end, and not at its start, or
+        // the CTA with the longest item would take the longest but 148 as well.
+        if constexpr (CAUSAL) next = atomicAdd(a.work_counter, 1) + static_cast<int>(gridDim.x);
       }
     }
   } else if (warp == 1) {
@@ -829,6 +834,25 @@ __global__ void __launch_bounds__(kBwdThreads, 1) fmha_bwd_kernel(const __grid_c
       // rows, so its rows are written one by one from registers.
       const int key = k0 + quad * 32 + lane;
       const bool edge = packed && (k0 + quad * 32 + 32 > q_limit);
+      if constexpr (CAUSAL) {
+        if (a.kv_parts > 1) {   // fp32 sums of this part's query heads: whole sectors, 512 consecutive bytes of a warp's store
+          float* dst = a.kv_partial + (static_cast<int64_t>(b * item_heads + h) * kv_tiles + k0 / kTileN) * (2 * kTileN * D) + dq_accum_index<D>(row, cq * DQ);
+#pragma unroll
+          for (int which = 0; which < 2; ++which)
+#pragma unroll
+            for (int c = 0; c < DQ / 16; ++c) {
+              uint32_t r[16];
+              tmem_ld16(tmem_base + lane_addr + (which == 0 ? kColdV : kColdK) + cq * DQ + c * 16, r);
+              tmem_wait_ld();
+              if (*abort_flag == 0) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                  *reinterpret_cast<uint4*>(dst + which * (kTileN * D) + (c * 4 + q) * 128) = make_uint4(r[q * 4], r[q * 4 + 1], r[q * 4 + 2], r[q * 4 + 3]);
+              }
+            }
+          return;
+        }
+      }
       stage_free();
 #pragma unroll
       for (int which = 0; which < 2; ++which) {
@@ -1083,6 +1107,67 @@ bool bwd_one_kv(int D, int64_t heads, int S_q, int S_k) {
   return D == 64 && S_k <= kTileN && (S_q <= 3 * kTileM || heads >= 12 * ((S_q + kTileM - 1) / kTileM));
 }
 
+// Causal, kv_parts > 1: sums the parts' dK and dV and rounds them.  A block takes 32 rows of a key tile, by way of shared memory to whole rows; bound by
+// its reads, which mostly find the L2 cache.
+template <int D, bool BF16>
+__global__ void __launch_bounds__(256) bwd_join_kernel(const __grid_constant__ BwdArgs a) {
+  griddep_wait();
+  constexpr int kStride = D * 2 + 8, N = 8 * D / 256;   // bytes of a staged row; float4 of a thread
+  __shared__ __align__(16) uint8_t tile[32 * kStride];
+  const int kv_tile = blockIdx.x / 4, r0 = (blockIdx.x % 4) * 32, hk = blockIdx.y >> 1, which = blockIdx.y & 1, b = blockIdx.z;   // which: 0 dV, 1 dK
+  const int* cu = static_cast<const int*>(a.mask);
+  const int base = cu[b], limit = packed_rows(base, cu[b + 1], a.S_q, a.total_rows) - kv_tile * kTileN - r0;
+  if (limit <= 0) return;
+  const int kv_tiles = (a.S_k + kTileN - 1) / kTileN;
+  float4 x[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int p = 0; p < a.kv_parts; ++p) {   // in this order, whatever order the parts were done in
+    const int64_t item = static_cast<int64_t>(b * a.H_kv * a.kv_parts + hk * a.kv_parts + p) * kv_tiles + kv_tile;
+    const float4* src = reinterpret_cast<const float4*>(a.kv_partial + (item * 2 + which) * (kTileN * D) + r0 * D);
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const float4 y = src[k * 256 + threadIdx.x];
+      x[k] = make_float4(x[k].x + y.x, x[k].y + y.y, x[k].z + y.z, x[k].w + y.w);
+    }
+  }
+  const float mul = which == 0 ? 1.0f : a.scale;
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const int i = k * 256 + threadIdx.x, row = i & 31, c4 = i >> 5;   // see dq_accum_index
+    *reinterpret_cast<uint2*>(tile + row * kStride + c4 * 8) =
+        make_uint2(pack2<BF16>(x[k].x * mul, x[k].y * mul), pack2<BF16>(x[k].z * mul, x[k].w * mul));
+  }
+  __syncthreads();
+  unsigned short* dst = static_cast<unsigned short*>(which == 0 ? a.dv_ptr : a.dk_ptr) + hk * (which == 0 ? a.dv_sh : a.dk_sh);
+  const int64_t ss = which == 0 ? a.dv_ss : a.dk_ss;
+#pragma unroll
+  for (int i = threadIdx.x; i < 32 * (D / 8); i += 256) {
+    const int row = i / (D / 8), ch = i % (D / 8);
+    const uint2 lo = *reinterpret_cast<const uint2*>(tile + row * kStride + ch * 16), hi = *reinterpret_cast<const uint2*>(tile + row * kStride + ch * 16 + 8);
+    if (row < limit) *reinterpret_cast<uint4*>(dst + (base + kv_tile * kTileN + r0 + row) * ss + ch * 8) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+  }
+}
+
+// Causal: over how many items the query heads of a key head are dealt out.  The first key tile of the longest sequence takes group x tiles steps, the
+// average multiprocessor as many as there are divided by their number (by the average length): where the former is the larger by more than the join costs
+// (some five steps' time), the least number of parts, 2 or 4, that makes it no larger, or the most there is.
+int bwd_causal_parts(int64_t sms, int64_t B, int64_t H, int64_t H_kv, int64_t max_len, int64_t total_rows) {
+  if (sms <= 0 || B <= 0 || H_kv <= 0 || H_kv > 32767) return 1;   // (two blocks of the join per key head along a grid axis)
+  const int64_t group = H / H_kv, tiles = (max_len + kTileM - 1) / kTileM, avg = (std::min(max_len, (total_rows + B - 1) / B) + kTileM - 1) / kTileM;
+  const int64_t mean = B * H * avg * (avg + 1) / 2 / sms, longest = group * tiles;
+  int parts = 1;
+  while (parts < 4 && group % (2 * parts) == 0 && longest / parts > mean + 5 && longest - std::max(mean, longest / (2 * parts)) > 5) parts *= 2;
+  return parts;
+}
+
+int launch_bwd_causal_join(const BwdArgs& a, int D, int dtype, cudaStream_t stream) {
+  const bool bf = dtype == FMHA_DTYPE_BF16;
+  auto kfn = D == 64 ? (bf ? bwd_join_kernel<64, true> : bwd_join_kernel<64, false>) : bf ? bwd_join_kernel<128, true> : bwd_join_kernel<128, false>;
+  const cudaError_t e = launch_overlapped(kfn, dim3((a.S_k + kTileN - 1) / kTileN * 4, 2 * a.H_kv, a.B), dim3(256), 0, stream, a);
+  return static_cast<int>(e != cudaSuccess ? e : cudaGetLastError());
+}
+
 template <int D, bool BF16, bool KEYADD, bool DROP, bool PACKED = false, bool ONE_KV = false, bool CAUSAL = false>
 static int launch_bwd_impl(const BwdArgs& a, cudaStream_t stream) {
   using L = BwdSmem<D>;
@@ -1095,7 +1180,7 @@ static int launch_bwd_impl(const BwdArgs& a, cudaStream_t stream) {
     if (e != cudaSuccess) return static_cast<int>(e);
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
-  const int64_t items = static_cast<int64_t>((a.S_k + kTileN - 1) / kTileN) * (CAUSAL ? a.H_kv : a.H) * a.B;
+  const int64_t items = static_cast<int64_t>((a.S_k + kTileN - 1) / kTileN) * (CAUSAL ? a.H_kv * a.kv_parts : a.H) * a.B;
   const int grid = static_cast<int>(std::min<int64_t>(items, sm_count()));   // one persistent CTA per SM
   const cudaError_t e = launch_overlapped(kfn, dim3(grid), dim3(kBwdThreads), L::kDynBytes, stream, a);
   return static_cast<int>(e != cudaSuccess ? e : cudaGetLastError());

@@ -507,6 +507,10 @@ int fmha_sm100_causal_bwd_workspace_bytes(const fmha_causal_bwd_params* p, size_
   if (rc != FMHA_OK) return rc;
   const size_t bh = static_cast<size_t>(p->B) * p->H, pad = (static_cast<size_t>(p->max_seqlen) + kTileM - 1) / kTileM * kTileM;
   *bytes = align256(bwd_accum_bytes(bh, pad, p->D)) + align256(bh * p->max_seqlen * sizeof(float)) + 256;
+  if (p->H > 0) {
+    const int parts = bwd_causal_parts(sm_count(), p->B, p->H, p->H_kv, p->max_seqlen, p->total_rows);
+    if (parts > 1) *bytes += static_cast<size_t>(p->B) * p->H_kv * parts * pad * p->D * 2 * sizeof(float);
+  }
   return FMHA_OK;
 }
 
@@ -544,6 +548,8 @@ int fmha_sm100_causal_bwd(const fmha_causal_bwd_params* p, void* stream_) {
   a.total_rows = rows;
   a.H_kv = Hk;
   a.kv_group = H / Hk;
+  a.kv_parts = bwd_causal_parts(sm_count(), p->B, H, Hk, p->max_seqlen, rows);
+  a.kv_partial = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(a.work_counter) + 256);
   a.dk_ptr = tdk.ptr; a.dk_ss = tdk.stride_s; a.dk_sh = tdk.stride_h;
   a.dv_ptr = tdv.ptr; a.dv_ss = tdv.stride_s; a.dv_sh = tdv.stride_h;
   a.B = p->B; a.H = H; a.S_q = a.S_k = p->max_seqlen;
@@ -572,6 +578,7 @@ int fmha_sm100_causal_bwd(const fmha_causal_bwd_params* p, void* stream_) {
     e = launch_bwd_prepare(to, tdo, a, p->dtype, stream);
   }
   if (e == 0) e = launch_bwd(a, D, p->dtype, stream);
+  if (e == 0 && a.kv_parts > 1) e = launch_bwd_causal_join(a, D, p->dtype, stream);
   if (e == 0 && D == 64)
     e = launch_bwd_finish(a.dq_accum, tdq, p->B, H, p->max_seqlen, pad, p->dtype, p->scale, p->cu_seqlens, rows, stream);
   return e != 0 ? cuda_fail(static_cast<cudaError_t>(e)) : FMHA_OK;

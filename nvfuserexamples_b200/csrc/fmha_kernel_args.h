@@ -96,6 +96,8 @@ struct BwdArgs {
   UncoveredRows zero;
   int persist;   // a CTA takes further work items of the grid when it has done its own
   int H_kv, kv_group;   // causal variants: key heads, query heads per key head (else 0)
+  int kv_parts;         // ... and over how many items of the dK / dV kernel the query heads of a key head are dealt out (bwd_causal_parts)
+  float* kv_partial;    // [B, H_kv * kv_parts, key tiles, 2, 128 * D] fp32 dK and dV of the items in the order of dq_accum_index, if kv_parts > 1
   int B, H, S_q, S_k;
   float scale;       // softmax scale
   float scale_log2;  // softmax scale * log2(e)
@@ -151,6 +153,10 @@ bool fwd_dense_applies(const FwdArgs& a, int D);
 int launch_fwd_dense(const FwdArgs& a, int dtype, cudaStream_t stream);
 int launch_bwd_dq(const BwdArgs& a, int dtype, cudaStream_t stream);   // head dimension 128: dQ, delta, work counter
 int launch_bwd(const BwdArgs& a, int D, int dtype, cudaStream_t stream);
+// causal: kv_parts for these sizes
+int bwd_causal_parts(int64_t sms, int64_t B, int64_t H, int64_t H_kv, int64_t max_len, int64_t total_rows);
+// ... and dK and dV of the parts' sum
+int launch_bwd_causal_join(const BwdArgs& a, int D, int dtype, cudaStream_t stream);
 // head dimension 64, one key tile: whether the main kernel is all there is (ONE_KV in fmha_bwd_sm100.cu)
 bool bwd_one_kv(int D, int64_t heads, int S_q, int S_k);
 // head dimension 64: the passes before and after the main kernel
