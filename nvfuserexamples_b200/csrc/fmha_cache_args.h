@@ -70,16 +70,29 @@ void paged_places(PagedArgs& a, void* workspace, const PagedGrid& g, int D);   /
 int launch_paged(const PagedArgs& a, int dtype, int D, int bits, cudaStream_t stream);
 
 #ifdef __CUDACC__
-// The sequence that packed row `row` belongs to, by a whole warp: how many sequences end at or before it.  -1 in front of the first, B behind the last.
-__device__ __forceinline__ int sequence_of_row(const int* cu, int B, int row) {
+// The sequence that packed row `row` belongs to, by a whole warp: b (-1: none), its first row, how many it has, and its entry of `lens`.  Lanes look at a
+// sequence each, and everything about it comes with the same round of loads.
+struct RowSequence {
+  int b, first, n, len;
+};
+__device__ __forceinline__ RowSequence sequence_of_row(const int* cu, const int* lens, int B, int row) {
   const int lane = threadIdx.x & 31;
-  if (row < cu[0]) return -1;
-  int n = 0;
-  for (int i = 0; i < B; i += 32) {
-    const bool ended = i + lane < B && cu[i + lane + 1] <= row;
-    n += __popc(__ballot_sync(0xffffffffu, ended));
+  RowSequence s = {-1, 0, 0, 0};
+#pragma unroll 4
+  for (int i0 = 0; i0 < B; i0 += 32) {   // (no early end, so that the loads of a large batch are in flight together)
+    const int i = i0 + lane;
+    int lo = 0, hi = 0, len = 0;
+    if (i < B) {
+      lo = cu[i];
+      hi = cu[i + 1];
+      if (lens != nullptr) len = lens[i];
+    }
+    if (lo <= row && row < hi) s = {i, lo, hi - lo, len};
   }
-  return n;
+  const uint32_t found = __ballot_sync(0xffffffffu, s.b >= 0);
+  const int at = found != 0u ? __ffs(found) - 1 : 0;
+  return {__shfl_sync(0xffffffffu, s.b, at), __shfl_sync(0xffffffffu, s.first, at), __shfl_sync(0xffffffffu, s.n, at),
+          __shfl_sync(0xffffffffu, s.len, at)};
 }
 #endif
 

@@ -422,3 +422,89 @@ def test_prompt_then_decoding(cuda_device, bits):
         r += n
         # two roundings of P and two of O on either side, of values of a few units; in 4 bits also those of the cache's values to fp16
         assert (got.double() - want.double()).abs().max() <= (4 if bits == 16 else 16) * 2.0 ** -11 * 3
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_other_layouts_of_the_arguments(cuda_device, bits):
+    """Lines of a wider page table, int64 lengths and offsets, q and k as slices of one projection or with heads outermost, one head, one page."""
+    lens, new, D = [45, 20, 64], [2, 1, 2], 64
+    c = filled(lens, 2, D, 32, torch.float16, bits, cuda_device)
+    wide = torch.full((3, 7), -5, dtype=torch.int32, device=cuda_device)
+    wide[:, 2:4] = c.table
+    x = randn(5, 10, D, dtype=torch.float16, device=cuda_device)
+    q, k, v = x[:, :6], x[:, 6:8], x[:, 8:]
+    args = (wide[:, 2:4], ints(lens, cuda_device, torch.int64), offsets(new, cuda_device).long())
+    turned = ops.kv_append(k, v, c.k, c.v, *args, q=q, inv_freq=inv_freq(32, cuda_device), **c.params)
+    heads_first = turned.transpose(0, 1).contiguous().transpose(0, 1)
+    o, lse = ops.fmha_paged_fwd(heads_first, c.k, c.v, *args, 2, **c.params)
+    want_o, want_lse = ref.attention(c, turned, lens, new)
+    check(o, want_o, "o")
+    check(lse, want_lse, "lse")
+    kk, vv = ops.kv_read(c.k, c.v, wide[:, 2:4], offsets(lens, cuda_device).long(), sum(lens), **c.params)
+    plain = ops.kv_read(c.k, c.v, c.table, offsets(lens, cuda_device), sum(lens), **c.params)
+    assert torch.equal(kk, plain[0]) and torch.equal(vv, plain[1])
+    one = filled([30], 1, D, 32, torch.float16, bits, cuda_device)
+    one.k, one.v, page = one.k[one.table[0, 0]:][:1], one.v[one.table[0, 0]:][:1], one.table[0, 0].item()
+    one.params = {n: p[page:page + 1] for n, p in one.params.items()}
+    one.table = torch.zeros_like(one.table)
+    q1 = randn(1, 1, D, dtype=torch.float16, device=cuda_device)
+    o, lse = attend(one, q1, [30], [1], cuda_device, cu=False)
+    want_o, want_lse = ref.attention(one, q1, [30], [1])
+    check(o, want_o, "o")
+    check(lse, want_lse, "lse")
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_no_pages_and_no_rows(cuda_device, bits):
+    c = filled([30, 10], 2, 64, 16, torch.float16, bits, cuda_device)
+    q = randn(2, 4, 64, dtype=torch.float16, device=cuda_device)
+    o, lse = ops.fmha_paged_fwd(q, c.k, c.v, c.table[:, :0], ints([30, 10], cuda_device), **c.params)   # a table without entries: no keys
+    assert (o == 0).all() and torch.isneginf(lse).all()
+    o, lse = ops.fmha_paged_fwd(q, c.k, c.v, c.table, ints([-3, 0], cuda_device), **c.params)
+    assert (o == 0).all() and torch.isneginf(lse).all()
+    o, lse = ops.fmha_paged_fwd(q[:0], c.k, c.v, c.table, ints([30, 10], cuda_device), **c.params)
+    assert o.shape == (0, 4, 64) and lse.shape == (4, 0)
+    k = randn(0, 2, 64, dtype=torch.float16, device=cuda_device)
+    out = ops.kv_append(k, k, c.k, c.v, c.table, ints([30, 10], cuda_device), q=q[:0], inv_freq=inv_freq(32, cuda_device), **c.params)
+    assert out.shape == (0, 4, 64)
+    assert ops.kv_read(c.k, c.v, c.table, ints([0, 0, 0], cuda_device), 0, **c.params)[0].shape == (0, 2, 64)
+
+
+def test_many_sequences(cuda_device):
+    """More sequences than lanes, several row tiles each, lengths of all kinds: the line of units is cut anywhere."""
+    g = torch.Generator().manual_seed(8)
+    lens = torch.randint(0, 700, (150,), generator=g).tolist()
+    new = torch.randint(0, 6, (150,), generator=g).tolist()
+    c = filled(lens, 2, 64, 16, torch.float16, 4, cuda_device)
+    q, k = (randn(sum(new), h, 64, dtype=torch.float16, device=cuda_device, seed=h) for h in (10, 2))
+    o, lse = attend(c, q, lens, new, cuda_device)
+    ops.check_status()
+    want_o, want_lse = ref.attention(c, q, lens, new)
+    check(o, want_o, "o")
+    check(lse, want_lse, "lse")
+    live = [n >= m for n, m in zip(lens, new)]
+    rows = torch.tensor([x for x, m in zip(live, new) for _ in range(m)], device=cuda_device)
+    ops.kv_append(k, k, c.k, c.v, c.table, ints(lens, cuda_device), offsets(new, cuda_device), **c.params)
+    pos = torch.cat([torch.arange(n - m, n) for n, m in zip(lens, new)]).to(cuda_device)
+    seq = torch.tensor([b for b, m in enumerate(new) for _ in range(m)], device=cuda_device)
+    at = (c.table[seq[rows], pos[rows] // 16].long(), slice(None), pos[rows] % 16)
+    assert torch.equal(c.v[at], ref.encode(k[rows])[0])
+    # offsets that decrease, lengths past everything: nothing outside the tensors is touched, and the call returns
+    ops.fmha_paged_fwd(q, c.k, c.v, c.table, ints([2 ** 31 - 1] * 150, cuda_device), ints(list(range(150, -1, -1)), cuda_device), 5, **c.params)
+    ops.kv_append(k, k, c.k.clone(), c.v.clone(), c.table, ints([2 ** 31 - 1] * 150, cuda_device), ints(list(range(150, -1, -1)), cuda_device),
+                  **{n: p.clone() for n, p in c.params.items()})
+    ops.kv_read(c.k, c.v, c.table, ints(list(range(150, -1, -1)), cuda_device), 200, **c.params)
+    ops.check_status()
+
+
+def test_operators_refuse_other_devices_and_types(cuda_device):
+    c = filled([30], 2, 64, 16, torch.float16, 16, cuda_device)
+    q = randn(1, 4, 64, dtype=torch.float16, device=cuda_device)
+    lens = ints([30], cuda_device)
+    for bad in (dict(block_table=c.table.cpu()), dict(seqlens=lens.cpu()), dict(v_cache=c.v.cpu()), dict(k_cache=c.k[..., :32], v_cache=c.v[..., :32]),
+                dict(q=q[:, :, :32]), dict(q=randn(3, 2, 64, dtype=torch.float16, device=cuda_device).as_strided((1, 4, 64), (260, 65, 1))),
+                dict(k_cache=c.k.transpose(2, 3)), dict(scale=-1.0)):
+        args = dict(q=q, k_cache=c.k, v_cache=c.v, block_table=c.table, seqlens=lens)
+        args.update(bad)
+        with pytest.raises(RuntimeError):
+            ops.fmha_paged_fwd(**args)
