@@ -1151,7 +1151,10 @@ __global__ void __launch_bounds__(256) bwd_join_kernel(const __grid_constant__ B
 
 // Causal: over how many items the query heads of a key head are dealt out.  The first key tile of the longest sequence takes group x tiles steps, the
 // average multiprocessor as many as there are divided by their number (by the average length): where the former is the larger by more than the join costs
-// (some five steps' time), the least number of parts, 2 or 4, that makes it no larger, or the most there is.
+// (some five steps' time), the least number of parts, 2 or 4, that makes it no larger, or the most there is.  The whole backward pass measured with 1, 2
+// and 4 parts (us; the rule's choice in brackets), D = 128: 6 sequences of 300-2048, 16/4 heads: 304 [276] 296; one of 2000, 32/8: 254 [196] 204; 2 of
+// 1000-1500, 16/2: 279 181 [134]; one of 700, 8/1: 137 88 [63]; 4 of 1500-4096, 32/8: [1475] 1539 1651; 32 of 100-500, 16/4: [198] 222 252; D = 64: one of 4000,
+// 16/4: 305 [200] 201; 13 of 61-1021, 16/4: [117] 118 128.
 int bwd_causal_parts(int64_t sms, int64_t B, int64_t H, int64_t H_kv, int64_t max_len, int64_t total_rows) {
   if (sms <= 0 || B <= 0 || H_kv <= 0 || H_kv > 32767) return 1;   // (two blocks of the join per key head along a grid axis)
   const int64_t group = H / H_kv, tiles = (max_len + kTileM - 1) / kTileM, avg = (std::min(max_len, (total_rows + B - 1) / B) + kTileM - 1) / kTileM;

@@ -591,11 +591,14 @@ bool fwd_pair_applies(const FwdArgs& a, int head_dim) {
   return fwd_pair_pays(sm_count(), a.B, a.H, a.S_q, a.S_k, packed || a.mask_kind == FMHA_MASK_SEQLEN, packed ? a.total_rows : 0);
 }
 
-// Causal: grids of at least a pair of tiles per SM by the average length.
+// Causal: pairs of tiles where sequences pass three tiles and there is a pair for every multiprocessor by the average length.  Measured, 16-bit (pair /
+// one tile at a time, us), B, query / key heads, lengths: 1, 32/8, 2000: 41.9 / 46.3; 4, 32/8, 1500-4096: 283 / 329; 6, 16/4, 300-2048: 61.9 / 70.0;
+// 8, 8/1, 500-2000: 45.4 / 48.0; 32, 16/16, 500: 76.9 / 87.8; 30, 32/8, 100-600: 119 / 119.  The other way, too few pairs: 1, 32/8, 1000: 21.3 / 18.5;
+// 1, 8/8, 4000: 63.6 / 59.3; 4, 8/2, 500-1500: 27.6 / 25.5; 3, 16/16, 640: 15.4 / 14.3; and too short: 32, 16/4, 384: 62.0 / 53.6; 64, 16/4, 250: 82.4 / 75.2.
 bool fwd_pair_causal_pays(int64_t sms, int64_t B, int64_t H, int64_t max_len, int64_t total_rows) {
   if (sms <= 0) return false;
   const int64_t n_avg = (std::min(max_len, (total_rows + B - 1) / B) + kTileM - 1) / kTileM;
-  return max_len > 256 && B * H * ((n_avg + 1) / 2) >= sms;
+  return max_len > 3 * kTileM && B * H * ((n_avg + 1) / 2) >= sms;
 }
 
 template <bool BF16, bool KEYADD, bool PACKED, bool CAUSAL = false>

@@ -292,7 +292,7 @@ template <int D, bool BF16, bool FOUR, bool INTER>
 static int append_impl(const KvAppendArgs& a, cudaStream_t stream) {
   KvAppendArgs args = a;
   const int steps = (a.H + 2 * a.cache.H_kv + 512 / D - 1) / (512 / D);
-  const int64_t fill = static_cast<int64_t>(sm_count()) * 16;   // warps that keep the memory busy
+  const int64_t fill = static_cast<int64_t>(sm_count()) * 16;   // warps that keep the memory busy (rows of 32/8 heads, 4 / 8 / 16 / 32 per SM: 64 rows 3.2 3.0 3.0 3.0 us, 512 rows 8.2 5.7 4.8 5.3)
   args.parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(steps, fill / std::max(a.total_rows, 1))));
   const int64_t warps = static_cast<int64_t>(a.total_rows) * args.parts;
   const cudaError_t e = launch_overlapped(kv_append_kernel<D, BF16, FOUR, INTER>, dim3(static_cast<unsigned>((warps + kKvWarps - 1) / kKvWarps)),

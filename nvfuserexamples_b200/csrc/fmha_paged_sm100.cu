@@ -39,8 +39,9 @@ namespace {
 
 constexpr int kPgWarps = 4;   // consumer warps
 constexpr int kPgThreads = 32 * (kPgWarps + 1);
-constexpr int kPgMinKeys = 256;   // a CTA's piece of the line holds at least so many
-constexpr int kPgUnitCost = 4;    // what a unit counts in the line beside its steps: its queries, its write-out
+constexpr int kPgMinKeys = 64;     // a CTA's piece of the line holds at least so many
+constexpr int kPgWholeKeys = 512;  // units stay whole where no sequence can have more
+constexpr int kPgUnitCost = 4;     // what a unit counts in the line beside its steps: its queries, its write-out
 constexpr float kPgLn2 = 0.6931471805599453f;
 
 enum PgWaitSite { kPgFull = 191, kPgEmpty = 192, kPgSmemBase = 193 };
@@ -201,7 +202,7 @@ __device__ __forceinline__ bool way_begin(const PagedArgs& a, PgWay& w) {
     u = look(g0 + lane);
   }
   total *= a.H_kv;
-  const int least = a.whole ? 1 : kPgMinKeys / KEYS + kPgUnitCost, ctas = gridDim.x;
+  const int least = a.whole ? 1 : max(1, kPgMinKeys / KEYS) + kPgUnitCost, ctas = gridDim.x;
   // a piece of the line (in 32 bits, where a division takes a third of the time, if the line is that short)
   const long long chunk = max(static_cast<long long>(least), total < (1ll << 30) ? (static_cast<int>(total) + ctas - 1) / ctas : (total + ctas - 1) / ctas);
   const long long w0 = chunk * blockIdx.x;
@@ -879,13 +880,20 @@ __global__ void __launch_bounds__(2 * D) paged_join_kernel(const __grid_constant
   if (block == 0 && g == 0) store_lse(a, seq, r0, n_rows, hk, m_all, l_all);
 }
 
-// Where no sequence can have more keys than a CTA takes at the least, units stay whole (no workspace, no second kernel).  Else two CTAs per SM, but no
-// more than the most keys that there can be would occupy.
+// The rules, each with both sides measured (us, 32/8 heads of 128, one new row if not said; 16 bits if not said):
+// - 8 query rows as one column where a unit has no more, else tiles of 16.  Four rows of a group: 54.3 against 55.4 with tiles of 16 (32 sequences of
+//   500-4000), in 4 bits 30.3 against 44.2.  Twelve rows: 60.2 with a tile of 16, 87.3 with two of 8, which read the cache twice.
+// - Units whole (no workspace, no second kernel) up to 512 keys.  One sequence of 250 keys: 6.9, cut 9.1; of 512: 9.3, cut 9.4, in 4 bits 8.5 and 10.0;
+//   64 of 100-512: 23.7 and 25.8; but one of 700: 11.2 and 8.9, of 1000: 14.2 and 9.8.
+// - Pieces of at least 64 keys.  At least 128 and 256: one sequence of 700 keys 9.8 and 11.4 against 8.9, of 2000: 10.0 and 11.2 against 9.8; of 30 000
+//   every CTA has more than that.
+// - Two CTAs per SM (what shared memory takes), but no more than the most keys that there can be would occupy.  In 4 bits three, of fewer stages, took
+//   51.2 instead of 55.3 at 32 sequences of 1000-8192 and 74.2 instead of 71.5 at two of 90 001-131 072, before other steps.
 PagedGrid paged_grid(int64_t sms, int64_t max_rows, int64_t group, int64_t heads, int64_t max_keys) {
   PagedGrid g;
   g.tile_rows = max_rows * group <= 8 ? 8 : 16;
   g.row_tiles = (max_rows * group + g.tile_rows - 1) / g.tile_rows;
-  g.whole = max_keys <= kPgMinKeys;
+  g.whole = max_keys <= kPgWholeKeys;
   const int64_t units = g.row_tiles * heads, most = units * std::max<int64_t>(1, (max_keys + kPgMinKeys - 1) / kPgMinKeys);
   g.ctas = static_cast<int>(std::max<int64_t>(1, std::min(2 * sms, most)));
   return g;
