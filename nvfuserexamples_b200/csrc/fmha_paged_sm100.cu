@@ -887,8 +887,9 @@ __global__ void __launch_bounds__(2 * D) paged_join_kernel(const __grid_constant
 //   64 of 100-512: 23.7 and 25.8; but one of 700: 11.2 and 8.9, of 1000: 14.2 and 9.8.
 // - Pieces of at least 64 keys.  At least 128 and 256: one sequence of 700 keys 9.8 and 11.4 against 8.9, of 2000: 10.0 and 11.2 against 9.8; of 30 000
 //   every CTA has more than that.
-// - Two CTAs per SM (what shared memory takes), but no more than the most keys that there can be would occupy.  In 4 bits three, of fewer stages, took
-//   51.2 instead of 55.3 at 32 sequences of 1000-8192 and 74.2 instead of 71.5 at two of 90 001-131 072, before other steps.
+// - Two CTAs per SM, but no more than the most keys that there can be would occupy.  Three, of fewer stages, against two: D = 128, 4 bits, 32 sequences of
+//   1000-8192 48.7 and 46.7, two of 90 001-131 072 64.2 and 60.8; D = 64, 16/4 heads, 4 bits: 64 of 500-4000 22.7 and 27.0, one of 60 000 19.1 and 17.8;
+//   16 bits: 32.3 and 32.2, 24.6 and 21.9.  What a CTA costs at its start and at the join outweighs the warps that it adds, but for one of these.
 PagedGrid paged_grid(int64_t sms, int64_t max_rows, int64_t group, int64_t heads, int64_t max_keys) {
   PagedGrid g;
   g.tile_rows = max_rows * group <= 8 ? 8 : 16;

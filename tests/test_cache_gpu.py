@@ -247,6 +247,21 @@ def test_long_sequences_are_dealt_out(cuda_device, D, bits):
     assert torch.equal(o, again[0]) and torch.equal(lse, again[1])
 
 
+@pytest.mark.parametrize("D,dtype", [(64, torch.float16), (128, torch.bfloat16)])
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("lens", [[512], [513], [641], [1000, 0, 64], [1, 1, 700, 1]])
+def test_few_keys_in_small_pieces(cuda_device, D, dtype, bits, lens):
+    """Around the length up to which units stay whole, and pieces of hardly more than their start."""
+    new = [min(n, 1) for n in lens]
+    c = filled(lens, 3, D, 16, dtype, bits, cuda_device)
+    q = randn(sum(new), 6, D, dtype=dtype, device=cuda_device)
+    o, lse = attend(c, q, lens, new, cuda_device)
+    ops.check_status()
+    want_o, want_lse = ref.attention(c, q, lens, new)
+    check(o, want_o, "o")
+    check(lse, want_lse, "lse")
+
+
 @pytest.mark.parametrize("bits", [16, 4])
 def test_rows_outside_sequences_and_past_max_rows(cuda_device, bits):
     lens, new = [50, 90], [3, 20]
