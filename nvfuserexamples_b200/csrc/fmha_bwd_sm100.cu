@@ -313,6 +313,12 @@ struct BwdItem {
 // counter.  A packed batch has the pass before it, to zero rows.  The accumulator, its clearing and conversion and the launches around
 // this one took 14 to 30 % of the time (whole backward, without / with dropout: B=2 H=4 S=128 10.6 -> 7.8 / 10.9 -> 8.4 us, B=13 H=12 S=100 15.1 -> 11.2 /
 // 16.6 -> 13.0, B=32 H=16 S=128 27.8 -> 19.5 / 29.1 -> 23.0, B=128 H=16 94.4 -> 68.3 / 97.8 -> 75.7; packed, B=32 H=16 of 64 to 128 rows 34.2 -> 27.7 / 36.1 -> 31.2).
+// Place of a sequence's key tile in kv_partial, by the row it begins at: with sequences one after the other none shares its place with another, whatever
+// their lengths, and there are no more than total_rows / 128 + B (places for the longest one's tiles in every sequence took 17 GB for one of 8192 rows
+// among 64 of 14 000 rows together, 8 key heads of 128; these take 0.7).
+int64_t kv_partial_tiles(int64_t total_rows, int64_t B) { return total_rows / kTileN + B; }
+__device__ __forceinline__ int64_t kv_partial_tile(int row_base, int b, int tile) { return static_cast<int64_t>(row_base / kTileN) + b + tile; }
+
 // CAUSAL: a packed batch whose rows see the keys up to their own position, with a.kv_group query heads to a key head.  An item is a key tile of
 // a KEY head: its query tiles are those from the diagonal on of every query head of the group, one head after the other, so dK and dV are summed
 // over the group in tensor memory, always in the same order.  Items count heads and sequences first and, last, the number of query tiles from the
@@ -836,7 +842,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) fmha_bwd_kernel(const __grid_c
       const bool edge = packed && (k0 + quad * 32 + 32 > q_limit);
       if constexpr (CAUSAL) {
         if (a.kv_parts > 1) {   // fp32 sums of this part's query heads: whole sectors, 512 consecutive bytes of a warp's store
-          float* dst = a.kv_partial + (static_cast<int64_t>(b * item_heads + h) * kv_tiles + k0 / kTileN) * (2 * kTileN * D) + dq_accum_index<D>(row, cq * DQ);
+          float* dst = a.kv_partial + (kv_partial_tile(row_base, b, k0 / kTileN) * item_heads + h) * (2 * kTileN * D) + dq_accum_index<D>(row, cq * DQ);
 #pragma unroll
           for (int which = 0; which < 2; ++which)
 #pragma unroll
@@ -1118,12 +1124,11 @@ __global__ void __launch_bounds__(256) bwd_join_kernel(const __grid_constant__ B
   const int* cu = static_cast<const int*>(a.mask);
   const int base = cu[b], limit = packed_rows(base, cu[b + 1], a.S_q, a.total_rows) - kv_tile * kTileN - r0;
   if (limit <= 0) return;
-  const int kv_tiles = (a.S_k + kTileN - 1) / kTileN;
   float4 x[N];
 #pragma unroll
   for (int k = 0; k < N; ++k) x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int p = 0; p < a.kv_parts; ++p) {   // in this order, whatever order the parts were done in
-    const int64_t item = static_cast<int64_t>(b * a.H_kv * a.kv_parts + hk * a.kv_parts + p) * kv_tiles + kv_tile;
+    const int64_t item = (kv_partial_tile(base, b, kv_tile) * a.H_kv + hk) * a.kv_parts + p;
     const float4* src = reinterpret_cast<const float4*>(a.kv_partial + (item * 2 + which) * (kTileN * D) + r0 * D);
 #pragma unroll
     for (int k = 0; k < N; ++k) {

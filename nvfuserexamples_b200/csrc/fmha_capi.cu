@@ -509,7 +509,7 @@ int fmha_sm100_causal_bwd_workspace_bytes(const fmha_causal_bwd_params* p, size_
   *bytes = align256(bwd_accum_bytes(bh, pad, p->D)) + align256(bh * p->max_seqlen * sizeof(float)) + 256;
   if (p->H > 0) {
     const int parts = bwd_causal_parts(sm_count(), p->B, p->H, p->H_kv, p->max_seqlen, p->total_rows);
-    if (parts > 1) *bytes += static_cast<size_t>(p->B) * p->H_kv * parts * pad * p->D * 2 * sizeof(float);
+    if (parts > 1) *bytes += static_cast<size_t>(kv_partial_tiles(p->total_rows, p->B)) * p->H_kv * parts * kTileN * p->D * 2 * sizeof(float);
   }
   return FMHA_OK;
 }

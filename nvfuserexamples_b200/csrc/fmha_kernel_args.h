@@ -97,7 +97,7 @@ struct BwdArgs {
   int persist;   // a CTA takes further work items of the grid when it has done its own
   int H_kv, kv_group;   // causal variants: key heads, query heads per key head (else 0)
   int kv_parts;         // ... and over how many items of the dK / dV kernel the query heads of a key head are dealt out (bwd_causal_parts)
-  float* kv_partial;    // [B, H_kv * kv_parts, key tiles, 2, 128 * D] fp32 dK and dV of the items in the order of dq_accum_index, if kv_parts > 1
+  float* kv_partial;    // [kv_partial_tiles, H_kv * kv_parts, 2, 128 * D] fp32 dV and dK of the items in the order of dq_accum_index, if kv_parts > 1
   int B, H, S_q, S_k;
   float scale;       // softmax scale
   float scale_log2;  // softmax scale * log2(e)
@@ -153,6 +153,7 @@ bool fwd_dense_applies(const FwdArgs& a, int D);
 int launch_fwd_dense(const FwdArgs& a, int dtype, cudaStream_t stream);
 int launch_bwd_dq(const BwdArgs& a, int dtype, cudaStream_t stream);   // head dimension 128: dQ, delta, work counter
 int launch_bwd(const BwdArgs& a, int D, int dtype, cudaStream_t stream);
+int64_t kv_partial_tiles(int64_t total_rows, int64_t B);   // places of key tiles in kv_partial
 // causal: kv_parts for these sizes
 int bwd_causal_parts(int64_t sms, int64_t B, int64_t H, int64_t H_kv, int64_t max_len, int64_t total_rows);
 // ... and dK and dV of the parts' sum

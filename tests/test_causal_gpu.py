@@ -56,6 +56,24 @@ def test_many_heads_and_long_sequences(cuda_device, D):
         assert torch.equal(dq, dq2)
 
 
+@pytest.mark.parametrize("D,H,H_kv", [(64, 8, 1), (128, 8, 1), (128, 12, 2)])
+def test_few_key_heads_and_one_long_sequence(cuda_device, D, H, H_kv):
+    """Query heads of a key head dealt out over items; their sums' places, and the scratch, go by rows and not by sequences times the longest."""
+    lens = [3, 700, 1, 129, 0, 128, 40] + [5] * 40
+    q, k, v, d_o, cu = batch(lens, H, H_kv, D, torch.bfloat16, cuda_device, before=7, behind=3)
+    o, lse = ops.fmha_causal_varlen_fwd(q, k, v, cu, 700)
+    torch.cuda.reset_peak_memory_stats()
+    held = torch.cuda.memory_allocated()
+    dq, dk, dv = ops.fmha_causal_varlen_bwd(d_o, q, k, v, o, lse, cu, 700)
+    used = torch.cuda.max_memory_allocated() - held
+    ops.check_status()
+    ref = ref64.causal(q, k, v, lens, d_o, offsets=cu[:-1].tolist())
+    for name, x in dict(dq=dq, dk=dk, dv=dv).items():
+        ref64.check(x[7:-3], (ref[name][0][7:-3], ref[name][1][7:-3]), name)
+    tiles, rows = q.shape[0] // 128 + len(lens), 768 * len(lens)   # (rows: as many as the longest of every sequence, of dQ's sums at 64 and delta)
+    assert used <= 4 * tiles * H_kv * 128 * D * 8 + rows * H * 4 * (1 + (D if D == 64 else 0)) + 3 * q.nbytes + (4 << 20)
+
+
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("lens", [[200, 77], [900, 40, 1300, 650] * 3], ids=["small", "large"])
 def test_rows_outside_the_sequences_do_not_matter(cuda_device, D, lens):
