@@ -169,7 +169,7 @@ typedef struct {
    owns rows [cu_seqlens[b], cu_seqlens[b+1]) of all of them (stride_b is not used), as with FMHA_MASK_CU_SEQLENS; one that is longer than
    max_seqlen is cut there.  Rows outside the sequences are neither read into a result nor, without FMHA_FLAG_ZERO_UNCOVERED, written: what
    they hold, an infinity or NaN included, does not matter.  Within a sequence an infinite or NaN value in V of a LATER row can reach rows
-   of the same 128 (a zero probability times it). */
+   of the same 128 (a zero probability times it), and in the backward pass one of an EARLIER row of q, o, d_o the keys' gradients there. */
 typedef struct {
   int32_t struct_bytes; /* sizeof(fmha_causal_fwd_params) */
   int32_t dtype;        /* FMHA_DTYPE_* */
@@ -258,7 +258,8 @@ typedef struct {
   int32_t struct_bytes; /* sizeof(fmha_paged_params) */
   int32_t dtype;        /* of q, o and a 16-bit cache */
   int32_t B, H, total_rows;
-  int32_t max_rows;     /* most new rows of a sequence (it sizes the grid) */
+  int32_t max_rows;     /* most new rows of a sequence (it sizes the grid); without cu_rows at least total_rows / B;
+                           (max_rows * H / H_kv, rounded up to 8) * H_kv: at most 2^22 */
   float scale;
   fmha_tensor4 q, o;    /* [total_rows, H, D] views (stride_h, stride_s) */
   float* lse;           /* optional [H, total_rows] */

@@ -88,7 +88,7 @@ static int validate_paged(const fmha_paged_params* p) {
   if (!(p->scale > 0.f) || !std::isfinite(p->scale)) return FMHA_ERR_BAD_ARG;
   // units are counted in 32 bits
   const int64_t tiles = (static_cast<int64_t>(p->max_rows) * (p->H / p->cache.H_kv) + 7) / 8;
-  if (p->H > 65535 || tiles * p->cache.H_kv > (1 << 20) || tiles * p->cache.H_kv * p->B > 0x7fffffffll) return FMHA_ERR_TOO_LARGE;
+  if (p->H > 65535 || tiles * p->cache.H_kv > (1 << 19) || tiles * p->cache.H_kv * p->B > 0x7fffffffll) return FMHA_ERR_TOO_LARGE;
   return FMHA_OK;
 }
 static PagedGrid grid_of(const fmha_paged_params* p) {
@@ -161,6 +161,7 @@ int fmha_sm100_paged_fwd(const fmha_paged_params* p, void* stream) {
   std::memset(&a, 0, sizeof(a));
   const fmha_kv_cache& c = p->cache;
   if (p->B == 0 || p->max_rows == 0 || p->seqlens == nullptr || !rows_each(p->total_rows, p->B, p->cu_rows, &a.rows_each)) return FMHA_ERR_BAD_ARG;
+  if (p->cu_rows == nullptr && p->max_rows < a.rows_each) return FMHA_ERR_BAD_ARG;
   if (!rows_ok(p->q, p->H) || !rows_ok(p->o, p->H) || c.pages == 0) return FMHA_ERR_BAD_ARG;
   rc = check_device();
   if (rc != FMHA_OK) return rc;

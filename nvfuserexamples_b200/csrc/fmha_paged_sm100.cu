@@ -246,7 +246,7 @@ __device__ __forceinline__ bool way_next(const PagedArgs& a, PgWay& w) {
   if (++w.hk == a.H_kv) {
     w.hk = 0;
     do {
-      ++w.g;
+      if (++w.g >= w.groups) return false;   // (the line's length says that there is one: if offsets are changed meanwhile, none is looked for behind them)
       if (++w.tile == w.tiles) {
         w.tile = 0;
         ++w.b;
@@ -391,7 +391,7 @@ __global__ void __launch_bounds__(kPgThreads, 2) fmha_paged_kernel(const __grid_
     [[maybe_unused]] const uint32_t ld_key = (kw + (mi & 1) * 8 + r8) * L::kRowBytes;
     [[maybe_unused]] const uint32_t ld_at[2] = {ld_key + (D == 128 ? ((mi >> 1) ^ (r8 >> 1)) << 4 : ((mi >> 1) ^ (r8 >> 2)) << 4),
                                                 ld_key + (((2 + (mi >> 1)) ^ (r8 >> 1)) << 4)};
-    [[maybe_unused]] const float inv_sl2 = 1.0f / a.scale_log2;
+    [[maybe_unused]] const float inv_sl2 = fminf(1.0f / a.scale_log2, 1e30f);   // (a subnormal scale: finite, as -infinity may be added to 8 times it)
     int i = 0;   // steps so far
     do {
       const PgSeq seq = sequence(a, w.b);

@@ -161,6 +161,11 @@ def test_argument_checks_of_attention(over, code):
     assert capi.load().fmha_sm100_paged_fwd(C.byref(paged_params(**over)), None) == code
 
 
+def test_without_offsets_all_rows_take_part():
+    assert capi.load().fmha_sm100_paged_fwd(C.byref(paged_params(max_rows=1)), None) == capi.FMHA_ERR_BAD_ARG   # two rows each
+    assert capi.load().fmha_sm100_paged_fwd(C.byref(paged_params(max_rows=1, cu_rows=0x5000)), None) != capi.FMHA_ERR_BAD_ARG
+
+
 @pytest.mark.parametrize("over,code", [
     (dict(struct_bytes=4), capi.FMHA_ERR_BAD_ARG), (dict(n_freq=65), capi.FMHA_ERR_UNSUPPORTED), (dict(n_freq=12), capi.FMHA_ERR_UNSUPPORTED),
     (dict(inv_freq=None), capi.FMHA_ERR_BAD_ARG), (dict(flags=2), capi.FMHA_ERR_BAD_ARG), (dict(total_rows=7), capi.FMHA_ERR_BAD_ARG),

@@ -263,6 +263,19 @@ def test_few_keys_in_small_pieces(cuda_device, D, dtype, bits, lens):
 
 
 @pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("scale", [1e-42, 1e-38, 1e-4])
+def test_small_scales(cuda_device, bits, scale):
+    """Down to subnormal numbers: means of the values."""
+    lens = [40, 600]
+    c = filled(lens, 2, 64, 16, torch.float16, bits, cuda_device)
+    q = randn(2, 4, 64, dtype=torch.float16, device=cuda_device)
+    o, lse = attend(c, q, lens, [1, 1], cuda_device, scale=scale)
+    want_o, want_lse = ref.attention(c, q, lens, [1, 1], scale=scale)
+    check(o, want_o, "o")
+    check(lse, want_lse, "lse")
+
+
+@pytest.mark.parametrize("bits", [16, 4])
 def test_rows_outside_sequences_and_past_max_rows(cuda_device, bits):
     lens, new = [50, 90], [3, 20]
     c = filled(lens, 2, 64, 16, torch.float16, bits, cuda_device)
