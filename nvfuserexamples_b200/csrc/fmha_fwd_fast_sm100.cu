@@ -91,7 +91,10 @@ struct FastSmem {
 // combines them through distributed shared memory.
 // CAUSAL: a packed batch whose rows see the keys up to their own position, with a.kv_group query heads to a key head.  The grid counts
 // heads, sequences and, longest first, query tiles: with one tile of every head before the next shorter ones the last CTAs to start are short,
-// and the query heads of a key head, which are neighbours, find its keys and values in the L2 cache.
+// and the query heads of a key head, which are neighbours, find its keys and values in the L2 cache.  Short grids end with the longest sequence's last
+// tile, a chain of its key steps (D = 64: some 1.2 us each with four CTAs on an SM): 11 sequences of 33-900, 16/4 heads of 64: 23.5 us, where the operations
+// take 4.  Steps of 128 keys at D = 64 halve their number but leave two CTAs on an SM: 31.2 us there, 203 / 283 at 4 of 1500-4096 of 32/8 heads, and less
+// (16.4 / 14.8) only where the grid does not fill the chip (one of 1000, 16/4): not used.  P is rounded to 16 bits for its product, as in the full form.
 template <int D, bool BF16, bool KEYADD, bool DROP, bool PACKED = false, bool SPLIT = false, bool CAUSAL = false>
 __global__ void __launch_bounds__(fast_threads<D>(), FastSmem<D, DROP>::kCtasPerSm) fmha_fwd_fast_kernel(const __grid_constant__ FwdArgs a) {
   griddep_wait();

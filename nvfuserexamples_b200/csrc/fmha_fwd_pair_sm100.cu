@@ -118,7 +118,8 @@ __device__ __forceinline__ void o_warp_out(uint32_t tO, float out_scale, uint32_
 
 // CAUSAL: a packed batch whose rows see the keys up to their own position, with a.kv_group query heads to a key head.  The second tile of a
 // pair has one key step more than the first; in that step nothing takes turns, and the first tile's MMA warp passes its K and V on unread.  The
-// grid counts heads, sequences and, longest first, pairs.
+// grid counts heads, sequences and, longest first, pairs.  4 sequences of 1500-4096, 32/8 heads: 281 us in short bursts, 1.02 PFLOP/s of the scores that there
+// are; 320 after a second of them, at the power limit's clock.
 template <bool BF16, bool KEYADD, bool PACKED, bool CAUSAL>
 __global__ void __launch_bounds__(kPairThreads, 1) fmha_fwd_pair_kernel(const __grid_constant__ FwdArgs a) {
   griddep_wait();
