@@ -24,8 +24,8 @@
 //
 // Measured (device time, 32/8 heads of 128; bytes of the cache once).  16 bits: 32 sequences of 8000 rows, one new row: 157 us, 6.7 TB/s; 16 of 200-4000, four new
 // rows: 34.6 us, 4.0 TB/s.  4 bits: two of 90 001-131 072: 60.5 us, 4.7 TB/s; 32 of 1000-8192: 46.5 us, 4.1 TB/s.  Of a short run some 4.5 us pass before the
-// first keys have landed and 3 at the join; in 4 bits the steady state is bound by issue and latency (1.9 instructions a cycle and SM; ALU 46 %, tensor
-// pipe 27 %, DRAM 56 %).  Before: tiles of 16 query rows and a grid of splits 39 / 107 / 122 us (four new rows / batch / long), a line of work 46 / 86 / 117,
+// first keys have landed and 3 at the join; in 4 bits the steady state is bound by issue and latency (1.8 instructions a cycle and SM; ALU 43 %, tensor
+// pipe 24 %, DRAM 50 %).  Before: tiles of 16 query rows and a grid of splits 39 / 107 / 122 us (four new rows / batch / long), a line of work 46 / 86 / 117,
 // the cache as the operand of 16 rows 48 / 55 / 71, shares in the accumulators' order 45 / 54 / 69, starts counted in the line 35 / 47 / 61.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
