@@ -327,7 +327,7 @@ __device__ __forceinline__ int64_t kv_partial_tile(int row_base, int b, int tile
 // Rows of Q, dO and K behind the end of the sequence are zeroed in shared memory: they are contracted over.  Bound by the chain of a tile (scores,
 // exponentials, dS, its products), of which one CTA per SM has one or two under way: B = 4, S = 2048, 16 heads of 128, causal 154 us, full 255; 6 sequences of
 // 300-2048, 16/4 heads: 195 us with longest key tiles first, 180 with tiles that do not exist passed over, 151 with heads dealt out, 124 with items claimed
-// late (and 14 for the join).
+// late (and 13 for the join).
 template <int D, bool BF16, bool KEYADD, bool DROP, bool PACKED = false, bool ONE_KV = false, bool CAUSAL = false>
 __global__ void __launch_bounds__(kBwdThreads, 1) fmha_bwd_kernel(const __grid_constant__ BwdArgs a) {
   griddep_wait();
@@ -1127,17 +1127,22 @@ __global__ void __launch_bounds__(256) bwd_join_kernel(const __grid_constant__ B
   const int* cu = static_cast<const int*>(a.mask);
   const int base = cu[b], limit = packed_rows(base, cu[b + 1], a.S_q, a.total_rows) - kv_tile * kTileN - r0;
   if (limit <= 0) return;
+  // (2 or 4 parts: two at a time, so that all their loads are in flight; added up in this order, whatever order the parts were done in)
+  const float4* src = reinterpret_cast<const float4*>(a.kv_partial + ((kv_partial_tile(base, b, kv_tile) * a.H_kv + hk) * a.kv_parts * 2 + which) * (kTileN * D) + r0 * D) +
+                      threadIdx.x;
   float4 x[N];
 #pragma unroll
   for (int k = 0; k < N; ++k) x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int p = 0; p < a.kv_parts; ++p) {   // in this order, whatever order the parts were done in
-    const int64_t item = (kv_partial_tile(base, b, kv_tile) * a.H_kv + hk) * a.kv_parts + p;
-    const float4* src = reinterpret_cast<const float4*>(a.kv_partial + (item * 2 + which) * (kTileN * D) + r0 * D);
+  for (int p = 0; p < a.kv_parts; p += 2) {
+    float4 y[2][N];
 #pragma unroll
-    for (int k = 0; k < N; ++k) {
-      const float4 y = src[k * 256 + threadIdx.x];
-      x[k] = make_float4(x[k].x + y.x, x[k].y + y.y, x[k].z + y.z, x[k].w + y.w);
-    }
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+      for (int k = 0; k < N; ++k) y[e][k] = src[(p + e) * (2 * kTileN * D / 4) + k * 256];
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+      for (int k = 0; k < N; ++k) x[k] = make_float4(x[k].x + y[e][k].x, x[k].y + y[e][k].y, x[k].z + y[e][k].z, x[k].w + y[e][k].w);
   }
   const float mul = which == 0 ? 1.0f : a.scale;
 #pragma unroll
