@@ -64,7 +64,7 @@ struct PagedGrid {
   bool whole;          // no unit is cut
   int ctas;
 };
-PagedGrid paged_grid(int64_t sms, int64_t max_rows, int64_t group, int64_t heads, int64_t max_keys);   // heads: key heads of all sequences
+PagedGrid paged_grid(int64_t sms, int64_t max_rows, int64_t group, int64_t heads, int64_t max_keys, int D, int bits);   // heads: key heads of all sequences
 size_t paged_workspace(const PagedGrid& g, int D);
 void paged_places(PagedArgs& a, void* workspace, const PagedGrid& g, int D);   // lays the workspace out
 int launch_paged(const PagedArgs& a, int dtype, int D, int bits, cudaStream_t stream);

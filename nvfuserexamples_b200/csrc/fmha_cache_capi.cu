@@ -93,7 +93,7 @@ static int validate_paged(const fmha_paged_params* p) {
 }
 static PagedGrid grid_of(const fmha_paged_params* p) {
   return paged_grid(sm_count(), p->max_rows, p->H / p->cache.H_kv, static_cast<int64_t>(p->cache.H_kv) * p->B,
-                    static_cast<int64_t>(p->cache.table_width) * p->cache.page_rows);
+                    static_cast<int64_t>(p->cache.table_width) * p->cache.page_rows, p->cache.D, p->cache.bits);
 }
 
 }  // namespace fmha

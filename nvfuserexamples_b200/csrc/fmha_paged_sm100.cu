@@ -63,7 +63,8 @@ struct PgSmem {
   static constexpr int kParTile = kKeys * kParBytes;           // its scales and bases
   static constexpr int kSub = kKeys * 128;                     // 16 bits: a 64-column sub-tile (128-byte swizzle)
   static constexpr int kStage = 2 * (kTile + kParTile);        // K, V, parameters of K, of V
-  static constexpr int kStages = FOUR ? (D == 128 ? 4 : 7) : D == 128 ? 3 : 6;
+  static constexpr int kCtas = FOUR && D == 64 && NQ == 1 ? 3 : 2;   // of an SM, at the most (paged_grid)
+  static constexpr int kStages = FOUR ? (D == 128 ? 4 : NQ == 1 ? 5 : 7) : D == 128 ? 3 : 6;
   // O of the four warps on its way to be added up, a column of 8 rows at a time, in the accumulators' order (16 bytes of a lane), and statistics
   static constexpr int kBlocks = D / 16;
   static constexpr int kOffShare = kStages * kStage;
@@ -71,7 +72,7 @@ struct PgSmem {
   static constexpr int kOffBar = kOffStats + kPgWarps * 8 * NQ * 8;
   static constexpr int kOffMisc = kOffBar + 2 * kStages * 8;
   static constexpr int kDynBytes = kOffMisc + 16;   // 1024-byte aligned base: checked by the kernel
-  static_assert(2 * (kDynBytes + 1024) <= 233472, "two CTAs share an SM");
+  static_assert(kCtas * (kDynBytes + 1024) <= 233472, "so many CTAs share an SM");
   static_assert(kStage % 1024 == 0 || (FOUR && kStage % 512 == 0), "swizzled tiles begin at multiples of 1024 bytes (64-byte rows: 512)");
 };
 
@@ -298,7 +299,7 @@ __device__ __forceinline__ void store_lse(const PagedArgs& a, const PgSeq& seq, 
 }  // namespace
 
 template <int D, bool BF16, bool FOUR, int NQ>
-__global__ void __launch_bounds__(kPgThreads, 2) fmha_paged_kernel(const __grid_constant__ PagedArgs a) {
+__global__ void __launch_bounds__(kPgThreads, PgSmem<D, FOUR, NQ>::kCtas) fmha_paged_kernel(const __grid_constant__ PagedArgs a) {
   using L = PgSmem<D, FOUR, NQ>;
   constexpr int ST = L::kStages, UN = L::kUnits, KEYS = L::kKeys, ROWS = 8 * NQ;
   constexpr bool MMA_BF16 = BF16 && !FOUR;
@@ -894,15 +895,19 @@ __global__ void __launch_bounds__(2 * D) paged_join_kernel(const __grid_constant
 // - Pieces of at least 64 keys.  At least 128 and 256: one sequence of 700 keys 9.8 and 11.4 against 8.9, of 2000: 10.0 and 11.2 against 9.8; of 30 000
 //   every CTA has more than that.
 // - Two CTAs per SM, but no more than the most keys that there can be would occupy.  Three, of fewer stages, against two: D = 128, 4 bits, 32 sequences of
-//   1000-8192 48.7 and 46.7, two of 90 001-131 072 64.2 and 60.8; D = 64, 16/4 heads, 4 bits: 64 of 500-4000 22.7 and 27.0, one of 60 000 19.1 and 17.8;
-//   16 bits: 32.3 and 32.2, 24.6 and 21.9.  What a CTA costs at its start and at the join outweighs the warps that it adds, but for one of these.
-PagedGrid paged_grid(int64_t sms, int64_t max_rows, int64_t group, int64_t heads, int64_t max_keys) {
+//   1000-8192 48.7 and 46.7, two of 90 001-131 072 64.2 and 60.8; D = 64, 16/4 heads, 16 bits: 64 of 500-4000 32.3 and 32.2, one of 60 000 24.6 and 21.9; 4 bits,
+//   tiles of 16: 22.1 and 21.4.  What a CTA costs at its start and at the join outweighs the warps that it adds, but for D = 64 in 4 bits with one
+//   column, where a step is mostly instructions: three from 2/3 of a unit per SM on.  64 sequences of 500-4000, 16/4 heads (256 units): 23.3 and 27.1; 64 of
+//   100-3000, 12/12: 42.6 and 55.6; 128 of 300-2000, 32/8: 42.4 and 49.1; 16 of 500-4000, 32/8 (128 units): 15.1 and 16.1; 100 of 100-3000, 8/1: 18.2 and
+//   18.7; the other way 8 of 500-4000, 32/8 (64 units): 12.5 and 11.6; one of 60 000, 16/4: 19.1 and 18.0; units that stay whole, 512 of up to 200 keys: 11.6 and 10.8.
+PagedGrid paged_grid(int64_t sms, int64_t max_rows, int64_t group, int64_t heads, int64_t max_keys, int D, int bits) {
   PagedGrid g;
   g.tile_rows = max_rows * group <= 8 ? 8 : 16;
   g.row_tiles = (max_rows * group + g.tile_rows - 1) / g.tile_rows;
   g.whole = max_keys <= kPgWholeKeys;
   const int64_t units = g.row_tiles * heads, most = units * std::max<int64_t>(1, (max_keys + kPgMinKeys - 1) / kPgMinKeys);
-  g.ctas = static_cast<int>(std::max<int64_t>(1, std::min(2 * sms, most)));
+  const bool three = D == 64 && bits == 4 && g.tile_rows == 8 && !g.whole && 3 * units >= 2 * sms;
+  g.ctas = static_cast<int>(std::max<int64_t>(1, std::min((three ? 3 : 2) * sms, most)));
   return g;
 }
 size_t paged_workspace(const PagedGrid& g, int D) {

@@ -262,6 +262,21 @@ def test_few_keys_in_small_pieces(cuda_device, D, dtype, bits, lens):
     check(lse, want_lse, "lse")
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("H,H_kv", [(8, 4), (6, 6)])
+def test_batches_in_four_bits(cuda_device, D, H, H_kv):
+    """Fewer units than, about as many as and more than fill the chip."""
+    for B in (20, 30, 70):
+        lens = [5 + (37 * b * b) % 900 for b in range(B)]
+        c = filled(lens, H_kv, D, 32, torch.float16, 4, cuda_device)
+        q = randn(B, H, D, dtype=torch.float16, device=cuda_device)
+        o, lse = attend(c, q, lens, [1] * B, cuda_device, cu=False)
+        ops.check_status()
+        want_o, want_lse = ref.attention(c, q, lens, [1] * B)
+        check(o, want_o, "o")
+        check(lse, want_lse, "lse")
+
+
 @pytest.mark.parametrize("bits", [16, 4])
 @pytest.mark.parametrize("scale", [1e-42, 1e-38, 1e-4])
 def test_small_scales(cuda_device, bits, scale):
