@@ -190,7 +190,9 @@ __device__ __forceinline__ void way_part(const PagedArgs& a, PgWay& w, int off) 
   w.j1 = a.whole ? w.u.steps : max(off + take - kPgUnitCost, 0);
   w.left -= take;
 }
-// False: nothing for this CTA.  Lanes look at 32 groups together; up to 32 of them the lengths are read once.
+// False: nothing for this CTA.  Lanes look at 32 groups together; up to 32 of them the lengths are read once.  With more, a lane sums a block of consecutive
+// groups, its loads in flight together, and only the block that holds the CTA's first unit is looked through (all of them, 32 at a time, twice: 1000 sequences of
+// up to 64 keys, 8/2 heads of 64, 41.0 us, 256 of 100-512, 32/8 heads of 128, 74.4 us, instead of 26.9 and 71.2).
 template <int KEYS>
 __device__ __forceinline__ bool way_begin(const PagedArgs& a, PgWay& w) {
   const int lane = threadIdx.x & 31;
@@ -201,12 +203,21 @@ __device__ __forceinline__ bool way_begin(const PagedArgs& a, PgWay& w) {
     if (g < w.groups) u = w.tiles == 1 ? group_of(a, g, 0, KEYS) : group_of(a, g / w.tiles, g % w.tiles, KEYS);
     return u;
   };
-  PgGroup u = look(lane);
-  long long total = 0;
-  for (int g0 = 0;;) {
-    total += __reduce_add_sync(0xffffffffu, u.weight);
-    if ((g0 += 32) >= w.groups) break;
-    u = look(g0 + lane);
+  PgGroup u;
+  const int block = (w.groups + 31) / 32;
+  long long total, blocks = 0, before = 0;   // of all groups; of those up to this lane's block; of the groups passed
+  if (block == 1) {
+    u = look(lane);
+    total = __reduce_add_sync(0xffffffffu, u.weight);
+  } else {
+#pragma unroll 8
+    for (int i = 0; i < block; ++i) blocks += look(lane * block + i).weight;
+#pragma unroll
+    for (int m = 1; m < 32; m *= 2) {
+      const long long y = __shfl_up_sync(0xffffffffu, blocks, m);
+      if (lane >= m) blocks += y;
+    }
+    total = __shfl_sync(0xffffffffu, blocks, 31);
   }
   total *= a.H_kv;
   const int least = a.whole ? 1 : max(1, kPgMinKeys / KEYS) + kPgUnitCost, ctas = gridDim.x;
@@ -215,9 +226,14 @@ __device__ __forceinline__ bool way_begin(const PagedArgs& a, PgWay& w) {
   const long long w0 = chunk * blockIdx.x;
   if (w0 >= total) return false;
   w.left = static_cast<int>(min(chunk, total - w0));
-  long long before = 0;   // of the groups passed
-  if (w.groups > 32) u = look(lane);
-  for (int g0 = 0;; u = look(g0 + lane)) {
+  int g0 = 0;
+  if (block > 1) {
+    const int at = __ffs(__ballot_sync(0xffffffffu, blocks * a.H_kv > w0)) - 1;   // (there is one: w0 < total)
+    if (at > 0) before = __shfl_sync(0xffffffffu, blocks, at - 1);
+    g0 = at * block;
+    u = look(g0 + lane);
+  }
+  for (;; u = look(g0 + lane)) {
     int sum = u.weight;   // inclusive
 #pragma unroll
     for (int m = 1; m < 32; m *= 2) {
@@ -252,14 +268,14 @@ __device__ __forceinline__ bool way_next(const PagedArgs& a, PgWay& w) {
   ++w.n;
   if (++w.hk == a.H_kv) {
     w.hk = 0;
-    do {
-      if (++w.g >= w.groups) return false;   // (the line's length says that there is one: if offsets are changed meanwhile, none is looked for behind them)
-      if (++w.tile == w.tiles) {
+    do {   // (a sequence's tiles without rows are its last ones)
+      if (w.u.weight == 0 || ++w.tile == w.tiles) {
         w.tile = 0;
-        ++w.b;
+        if (++w.b >= a.B) return false;   // (the line's length says that there is one: if offsets are changed meanwhile, none is looked for behind them)
       }
       w.u = group_of(a, w.b, w.tile, KEYS);
     } while (w.u.weight == 0);
+    w.g = w.b * w.tiles + w.tile;
   }
   way_part<KEYS>(a, w, 0);
   return true;
