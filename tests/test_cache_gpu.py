@@ -278,6 +278,20 @@ def test_batches_in_four_bits(cuda_device, D, H, H_kv):
 
 
 @pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("B", [3, 90])
+def test_a_loose_maximum_of_new_rows(cuda_device, bits, B):
+    """max_seqlen_q far above what any sequence has: tiles without rows."""
+    lens, new = [(61 * b * b + 9) % 700 for b in range(B)], [b % 4 for b in range(B)]
+    c = filled(lens, 2, 64, 32, torch.float16, bits, cuda_device)
+    q = randn(sum(new), 8, 64, dtype=torch.float16, device=cuda_device)
+    o, lse = ops.fmha_paged_fwd(q, c.k, c.v, c.table, ints(lens, cuda_device), offsets(new, cuda_device), 1000, **c.params)
+    ops.check_status()
+    want_o, want_lse = ref.attention(c, q, lens, new)
+    check(o, want_o, "o")
+    check(lse, want_lse, "lse")
+
+
+@pytest.mark.parametrize("bits", [16, 4])
 @pytest.mark.parametrize("scale", [1e-42, 1e-38, 1e-4])
 def test_small_scales(cuda_device, bits, scale):
     """Down to subnormal numbers: means of the values."""
