@@ -252,8 +252,9 @@ typedef struct {
 /* Attention of the last rows of sequences over all their rows in a paged cache.  q, o are packed like the rows of fmha_kv_append_params; the i-th of n
    new rows sees positions 0 to seqlens[b] - n + i, query head h reads key head h / (H / H_kv).  A row that sees no key gets zeros and a logsumexp of
    -infinity, as do rows outside the sequences and past max_rows of theirs.  What the cache holds behind a sequence's last row does not matter; an infinite or
-   NaN value in V of a LATER new row can reach the earlier ones.  From a 4-bit cache products are formed in fp16: q is rounded to it (finite
-   values stay finite). */
+   NaN value in V of a LATER new row can reach the earlier ones.  Scores count up to 2^24 in absolute value; the exponentials of larger ones are not to be told apart.
+   From a 4-bit cache products are formed in fp16: q is rounded to it, a row with values of 1024 and more divided by a power of two before; probabilities, in a scaled
+   form, and their products with the scales of V as well, each once.  Relative to a row's largest probability, one of 2^-25 still has 11 bits, and from 2^-36 on they end. */
 typedef struct {
   int32_t struct_bytes; /* sizeof(fmha_paged_params) */
   int32_t dtype;        /* of q, o and a 16-bit cache */

@@ -19,11 +19,14 @@
 // scale (the query's even values are taken 16-fold) are multiplied by it in 32 bits; what does not depend on codes, the sum of (b + s) times the query's
 // values, is one more MMA of the scales and bases as they lie in memory against those values' sums (in two parts of 11 bits).  So scores are as exact
 // as 32 bits allow.  V: P is multiplied by the key's scale of each 32 dimensions, the product with the codes is scaled at the end, and the sum of P (b + s)
-// is one more MMA of the transposed scales and bases (both products round P, or P times a scale, to 11 bits, as a 16-bit type would).  The row maximum is kept exactly here (16 bits: up to 2^8), for P times a scale of up to 65 504 has to fit
-// fp16.
+// is one more MMA of the transposed scales and bases.  P is rounded to 11 bits for both, and its product with a scale once more.  Both have to stay normal numbers of
+// fp16 for that, however small V's values or the probabilities of most keys are.  So the row maximum is kept exactly here (16 bits: up to 2^8), P is taken up to
+// 2^15-fold by way of the exponent, and each warp follows the largest scale it has seen, as it does the maximum: scales of 2 to 32 take so much of the factor of P,
+// and below 2^-7 or from 32 on the scales are multiplied by a power of two (p_top, v_factor).  (Without that, o was off by 2 % for values of 1e-4, and by more than itself
+// where the largest probability, 2^24 times the others, had a value of zero; it costs 3 %, a load and some ten instructions a step.)
 //
 // Measured (device time, 32/8 heads of 128; bytes of the cache once).  16 bits: 32 sequences of 8000 rows, one new row: 157 us, 6.7 TB/s; 16 of 200-4000, four new
-// rows: 34.6 us, 4.0 TB/s.  4 bits: two of 90 001-131 072: 60.5 us, 4.7 TB/s; 32 of 1000-8192: 46.5 us, 4.1 TB/s.  Of a short run some 4.5 us pass before the
+// rows: 34.6 us, 4.0 TB/s.  4 bits: two of 90 001-131 072: 63.5 us, 4.5 TB/s; 32 of 1000-8192: 48.5 us, 3.9 TB/s.  Of a short run some 4.5 us pass before the
 // first keys have landed and 3 at the join; in 4 bits the steady state is bound by issue and latency (1.8 instructions a cycle and SM; ALU 43 %, tensor
 // pipe 24 %, DRAM 50 %).  Before: tiles of 16 query rows and a grid of splits 39 / 107 / 122 us (four new rows / batch / long), a line of work 46 / 86 / 117,
 // the cache as the operand of 16 rows 48 / 55 / 71, shares in the accumulators' order 45 / 54 / 69, starts counted in the line 35 / 47 / 61.
@@ -131,6 +134,13 @@ __device__ __forceinline__ void code_pairs(uint32_t w, uint32_t (&v)[4]) {
   v[2] = (w >> 8) & 0x000F000Fu;
   v[3] = (w >> 8) & 0x00F000F0u;
 }
+
+// 4 bits, by the exponent field of V's largest scale (which is 2^(field - 15) to twice that; an infinity counts as the largest number): P is taken
+// 2^p_top-fold and the scales 2^v_factor-fold, so that P times a scale stays below 2^16.  Scales from 2^-7 to 32 are left as they are.
+__device__ __forceinline__ int p_top(int field) { return 15 - min(max(field - 15, 0), 4); }
+__device__ __forceinline__ int v_factor(int field) { return field >= 20 ? 19 - min(field, 30) : field >= 8 ? 0 : 15 - field; }
+// 2^k as a half, -14 <= k <= 15, twice
+__device__ __forceinline__ uint32_t half2_pow2(int k) { return (static_cast<uint32_t>(15 + k) << 10) * 0x00010001u; }
 
 // A sequence: its new rows and its keys.
 struct PgSeq {
@@ -494,6 +504,9 @@ __global__ void __launch_bounds__(kPgThreads, PgSmem<D, FOUR, NQ>::kCtas) fmha_p
       float2 shift[NQ], l[NQ];
       float o[NQ][D / 16][4];   // 16 bits: dimensions 16 mt + g and + 8; 4 bits: block 2 c + e has 32 c + 4 g + 2 e and + 1
       [[maybe_unused]] float ob[NQ][4];   // 4 bits: rows are scales and bases
+      // 4 bits: the first number above all with the exponent of V's largest scale so far; v_factor of that
+      [[maybe_unused]] uint32_t v_limit = 1u << 10;
+      [[maybe_unused]] int v_up = v_factor(0);
 #pragma unroll
       for (int nq = 0; nq < NQ; ++nq) {
         m[nq][0] = m[nq][1] = -INFINITY;
@@ -510,6 +523,19 @@ __global__ void __launch_bounds__(kPgThreads, PgSmem<D, FOUR, NQ>::kCtas) fmha_p
         if (key0 < k_limit) {
           const uint32_t sk = smem_u32(smem + s * L::kStage), sv = sk + L::kTile;
           const bool whole = key0 + 16 * UN <= k_limit;
+          // 4 bits: V's largest scale, of which the sums of products follow the exponent as they do the maximum; a lane looks at one key's
+          [[maybe_unused]] uint32_t v_scale = 0u;
+          if constexpr (FOUR) {
+            const uint32_t at = sv + L::kTile + L::kParTile + (kw + lane) * L::kParBytes;
+            if constexpr (D == 128) {
+              const uint4 x = lds128(at);
+              v_scale = max(max(x.x & 0x7fffu, x.y & 0x7fffu), max(x.z & 0x7fffu, x.w & 0x7fffu));
+            } else {
+              const uint2 x = lds64(at);
+              v_scale = max(x.x & 0x7fffu, x.y & 0x7fffu);
+            }
+            if (key0 + lane >= k_limit) v_scale = 0u;
+          }
           // ---- S^T ----------------------------------------------------------------------
           float sc[UN][NQ][4];   // keys 16 un + g (rows 2t, 2t + 1), + 8
 #pragma unroll
@@ -590,7 +616,7 @@ __global__ void __launch_bounds__(kPgThreads, PgSmem<D, FOUR, NQ>::kCtas) fmha_p
                   if (key0 + un * 16 + (e >> 1) * 8 + g >= limit[nq][e & 1]) sc[un][nq][e] = -INFINITY;
           }
           float mx[NQ][2];
-          bool more = false;
+          bool more = FOUR && v_scale >= v_limit;
 #pragma unroll
           for (int nq = 0; nq < NQ; ++nq)
 #pragma unroll
@@ -601,7 +627,16 @@ __global__ void __launch_bounds__(kPgThreads, PgSmem<D, FOUR, NQ>::kCtas) fmha_p
               mx[nq][e] = x;
               more |= x > (FOUR ? m[nq][e] : fmaf(kLazy, inv_sl2, m[nq][e]));
             }
-          if (__any_sync(0xffffffffu, more)) {   // the maximum of a row has moved
+          if (__any_sync(0xffffffffu, more)) {   // the maximum of a row has moved, or that of the scales
+            [[maybe_unused]] float top = 0.f, top_by = 0.f, v_by = 1.f;
+            if constexpr (FOUR) {
+              const int old = static_cast<int>(v_limit >> 10) - 1, field = max(old, static_cast<int>(__reduce_max_sync(0xffffffffu, v_scale) >> 10));
+              top = static_cast<float>(p_top(field));
+              top_by = static_cast<float>(p_top(old) - p_top(field));
+              v_by = __int_as_float((127 + v_factor(field) - v_up) << 23);
+              v_limit = static_cast<uint32_t>(field + 1) << 10;
+              v_up = v_factor(field);
+            }
 #pragma unroll
             for (int nq = 0; nq < NQ; ++nq) {
               float alpha[2], new_shift[2];
@@ -613,23 +648,27 @@ __global__ void __launch_bounds__(kPgThreads, PgSmem<D, FOUR, NQ>::kCtas) fmha_p
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
                 const bool moved = x > (FOUR ? m[nq][e] : fmaf(kLazy, inv_sl2, m[nq][e]));
                 const float old = e ? shift[nq].y : shift[nq].x;
-                new_shift[e] = moved ? -x * sl2[nq][e] : old;
-                alpha[e] = !moved ? 1.0f : m[nq][e] == -INFINITY ? 0.f : fast_exp2(new_shift[e] - old);
+                // (4 bits: rounded so that no exponent, a multiply-add rounded once, passes `top`, however large the scores are)
+                if constexpr (FOUR) new_shift[e] = moved ? __fsub_rd(top, __fmul_ru(x, sl2[nq][e])) : __fsub_rd(old, top_by);
+                else new_shift[e] = moved ? -x * sl2[nq][e] : old;
+                alpha[e] = !moved && (!FOUR || top_by == 0.f) ? 1.0f : m[nq][e] == -INFINITY ? 0.f : fast_exp2(new_shift[e] - old);
                 if (moved) m[nq][e] = x;
               }
               shift[nq] = make_float2(new_shift[0], new_shift[1]);
               l[nq].x *= alpha[0];
               l[nq].y *= alpha[1];
+              if constexpr (FOUR) {
+                ob[nq][0] *= alpha[0];
+                ob[nq][1] *= alpha[1];
+                alpha[0] *= v_by;
+                alpha[1] *= v_by;
+              }
 #pragma unroll
               for (int c = 0; c < D / 16; ++c) {
                 o[nq][c][0] *= alpha[0];
                 o[nq][c][1] *= alpha[1];
                 o[nq][c][2] *= alpha[0];
                 o[nq][c][3] *= alpha[1];
-              }
-              if constexpr (FOUR) {
-                ob[nq][0] *= alpha[0];
-                ob[nq][1] *= alpha[1];
               }
             }
           }
@@ -679,6 +718,13 @@ __global__ void __launch_bounds__(kPgThreads, PgSmem<D, FOUR, NQ>::kCtas) fmha_p
 #pragma unroll
                   for (int c = 0; c < D / 32; ++c) ss[e][c] &= kp;
                 }
+              }
+              if (v_up != 0) {
+                const uint32_t by = half2_pow2(v_up);
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                  for (int c = 0; c < D / 32; ++c) ss[e][c] = hmul2(ss[e][c], by);
               }
 #pragma unroll
               for (int nq = 0; nq < NQ; ++nq) mma_16816<false>(ob[nq], pt, p[un][nq][0], p[un][nq][1], ob[nq]);
@@ -746,7 +792,8 @@ __global__ void __launch_bounds__(kPgThreads, PgSmem<D, FOUR, NQ>::kCtas) fmha_p
             const int at = 8 * (c / 2) + t;
             const float b0 = __shfl_sync(0xffffffffu, ob[nq][0], at) + __shfl_sync(0xffffffffu, ob[nq][0], at + 4);
             const float b1 = __shfl_sync(0xffffffffu, ob[nq][1], at) + __shfl_sync(0xffffffffu, ob[nq][1], at + 4);
-            x = make_float4(fmaf(x.x, 1048576.f, b0), fmaf(x.y, 1048576.f, b1), fmaf(x.z, 65536.f, b0), fmaf(x.w, 65536.f, b1));
+            const float f20 = __int_as_float((127 + 20 - v_up) << 23), f16 = __int_as_float((127 + 16 - v_up) << 23);
+            x = make_float4(fmaf(x.x, f20, b0), fmaf(x.y, f20, b1), fmaf(x.z, f16, b0), fmaf(x.w, f16, b1));
           }
           share[(warp * L::kBlocks + c) * 32 + lane] = x;
         }
