@@ -783,6 +783,22 @@ void check_append_shapes(const at::Tensor& k, const at::Tensor& v, const at::Ten
     TORCH_CHECK(2 * n <= D && n % step == 0, "mha_manual: inv_freq must have a multiple of ", step, " pairs, at most D/2, got ", n);
   }
 }
+// Autograd learns of a write: the version counters move, and where gradients are on a cache that wants them is refused.
+void check_written(const at::Tensor& k_cache, const at::Tensor& v_cache, const OptTensor& k_params, const OptTensor& v_params) {
+  if (!at::GradMode::is_enabled()) return;
+  TORCH_CHECK(!k_cache.requires_grad() && !v_cache.requires_grad() && !(k_params.has_value() && k_params->requires_grad()) &&
+                  !(v_params.has_value() && v_params->requires_grad()),
+              "mha_manual: a cache that requires gradients cannot be appended to");
+}
+void count_writes(const at::Tensor& k_cache, const at::Tensor& v_cache, const OptTensor& k_params, const OptTensor& v_params) {
+  auto count = [](const at::Tensor& x) {
+    if (!x.is_inference()) x.unsafeGetTensorImpl()->bump_version();   // (a tensor made in inference mode has none)
+  };
+  count(k_cache);
+  count(v_cache);
+  if (k_params.has_value()) count(*k_params);
+  if (v_params.has_value()) count(*v_params);
+}
 OptTensor kv_append(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& block_table,
                     const at::Tensor& seqlens, const OptTensor& cu_seqlens, const OptTensor& q, const OptTensor& inv_freq, bool interleaved,
                     const OptTensor& k_params, const OptTensor& v_params) {
@@ -791,6 +807,7 @@ OptTensor kv_append(const at::Tensor& k, const at::Tensor& v, const at::Tensor& 
   fill_cache(p.cache, k, k_cache, v_cache, block_table, k_params, v_params);
   check_append_shapes(k, v, k_cache, p.cache.D, q, inv_freq);
   check_lens_shapes(block_table, seqlens, cu_seqlens, k.size(0));
+  check_written(k_cache, v_cache, k_params, v_params);
   const c10::cuda::CUDAGuard guard(k.device());
   const int dev = k.get_device();
   check_same(k, v, "v");
@@ -820,9 +837,22 @@ OptTensor kv_append(const at::Tensor& k, const at::Tensor& v, const at::Tensor& 
   }
   p.flags = interleaved ? FMHA_KV_INTERLEAVED : 0;
   finish_call(fmha_sm100_kv_append(&p, at::cuda::getCurrentCUDAStream(dev).stream()), "kv_append", dev);
+  count_writes(k_cache, v_cache, k_params, v_params);
   return out;
 }
 
+// torch.compile takes no operator that writes to its arguments and may return a tensor or none, so beneath kv_append there are two, with and without q, as
+// which it is traced.  Called otherwise it goes straight to the kernel (by way of the two a call takes the host 0.5 us more).
+void kv_append_kv(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& block_table,
+                  const at::Tensor& seqlens, const OptTensor& cu_seqlens, const OptTensor& inv_freq, bool interleaved, const OptTensor& k_params,
+                  const OptTensor& v_params) {
+  kv_append(k, v, k_cache, v_cache, block_table, seqlens, cu_seqlens, OptTensor(), inv_freq, interleaved, k_params, v_params);
+}
+at::Tensor kv_append_qkv(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                         const at::Tensor& block_table, const at::Tensor& seqlens, const OptTensor& cu_seqlens, const OptTensor& inv_freq,
+                         bool interleaved, const OptTensor& k_params, const OptTensor& v_params) {
+  return *kv_append(k, v, k_cache, v_cache, block_table, seqlens, cu_seqlens, q, inv_freq, interleaved, k_params, v_params);
+}
 at::ScalarType read_type(const at::Tensor& k_cache, bool bf16) {
   return k_cache.scalar_type() != at::kByte ? k_cache.scalar_type() : bf16 ? at::kBFloat16 : at::kHalf;
 }
@@ -1213,6 +1243,21 @@ at::Tensor fmha_causal_varlen_noautograd(const at::Tensor& q, const at::Tensor& 
                              int64_t, c10::optional<double>>("mha_manual::fmha_causal_varlen_fwd", q, k, v, cu_seqlens, max_seqlen, scale));
 }
 
+// kv_append as the two operators that torch.compile takes.
+OptTensor kv_append_traced(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& block_table,
+                           const at::Tensor& seqlens, const OptTensor& cu_seqlens, const OptTensor& q, const OptTensor& inv_freq, bool interleaved,
+                           const OptTensor& k_params, const OptTensor& v_params) {
+  if (q.has_value()) {
+    static auto op = find_op<at::Tensor, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                             const at::Tensor&, const OptTensor&, const OptTensor&, bool, const OptTensor&, const OptTensor&>("mha_manual::kv_append_qkv");
+    return op.call(*q, k, v, k_cache, v_cache, block_table, seqlens, cu_seqlens, inv_freq, interleaved, k_params, v_params);
+  }
+  static auto op = find_op<void, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                           const OptTensor&, const OptTensor&, bool, const OptTensor&, const OptTensor&>("mha_manual::kv_append_kv");
+  op.call(k, v, k_cache, v_cache, block_table, seqlens, cu_seqlens, inv_freq, interleaved, k_params, v_params);
+  return OptTensor();
+}
+
 // ---------------------------------------------------------------------------------------
 // shape-only kernels (Meta key): what fake-tensor tracing and torch.compile need.  They check the
 // same shape rules as the CUDA kernels' wrappers and allocate outputs of the same shapes.
@@ -1399,7 +1444,19 @@ OptTensor kv_append_meta(const at::Tensor& k, const at::Tensor& v, const at::Ten
                          const OptTensor& k_params, const OptTensor& v_params) {
   check_append_shapes(k, v, k_cache, check_cache_shapes(k_cache, v_cache, block_table, k_params, v_params), q, inv_freq);
   check_lens_shapes(block_table, seqlens, cu_seqlens, k.size(0));
+  check_written(k_cache, v_cache, k_params, v_params);
+  count_writes(k_cache, v_cache, k_params, v_params);
   return q.has_value() ? OptTensor(at::empty(q->sizes(), q->options())) : OptTensor();
+}
+void kv_append_kv_meta(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& block_table,
+                       const at::Tensor& seqlens, const OptTensor& cu_seqlens, const OptTensor& inv_freq, bool interleaved, const OptTensor& k_params,
+                       const OptTensor& v_params) {
+  kv_append_meta(k, v, k_cache, v_cache, block_table, seqlens, cu_seqlens, OptTensor(), inv_freq, interleaved, k_params, v_params);
+}
+at::Tensor kv_append_qkv_meta(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                              const at::Tensor& block_table, const at::Tensor& seqlens, const OptTensor& cu_seqlens, const OptTensor& inv_freq,
+                              bool interleaved, const OptTensor& k_params, const OptTensor& v_params) {
+  return *kv_append_meta(k, v, k_cache, v_cache, block_table, seqlens, cu_seqlens, q, inv_freq, interleaved, k_params, v_params);
 }
 Pair kv_read_meta(const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& block_table, const at::Tensor& cu_seqlens, int64_t total_rows,
                   const OptTensor& k_params, const OptTensor& v_params, bool bf16) {
@@ -1453,7 +1510,12 @@ TORCH_LIBRARY(mha_manual, m) {
         "float? scale=None) -> (Tensor, Tensor, Tensor)");
   m.def("fmha_causal_varlen(Tensor q, Tensor k, Tensor v, Tensor cu_seqlens, int max_seqlen, float? scale=None) -> Tensor");
   m.def("kv_append(Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor block_table, Tensor seqlens, Tensor? cu_seqlens=None, *, "
-        "Tensor? q=None, Tensor? inv_freq=None, bool interleaved=False, Tensor(c!)? k_params=None, Tensor(d!)? v_params=None) -> Tensor?");
+        "Tensor? q=None, Tensor? inv_freq=None, bool interleaved=False, Tensor(c!)? k_params=None, Tensor(d!)? v_params=None) -> Tensor?",
+        torch::dispatch(c10::DispatchKey::CompositeImplicitAutograd, TORCH_FN(kv_append_traced)));
+  m.def("kv_append_kv(Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor block_table, Tensor seqlens, Tensor? cu_seqlens=None, "
+        "Tensor? inv_freq=None, bool interleaved=False, Tensor(c!)? k_params=None, Tensor(d!)? v_params=None) -> ()");
+  m.def("kv_append_qkv(Tensor q, Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor block_table, Tensor seqlens, "
+        "Tensor? cu_seqlens=None, Tensor? inv_freq=None, bool interleaved=False, Tensor(c!)? k_params=None, Tensor(d!)? v_params=None) -> Tensor");
   m.def("kv_read(Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor cu_seqlens, int total_rows, *, Tensor? k_params=None, "
         "Tensor? v_params=None, bool bf16=False) -> (Tensor, Tensor)");
   m.def("fmha_paged_fwd(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor seqlens, Tensor? cu_seqlens=None, "
@@ -1476,6 +1538,8 @@ TORCH_LIBRARY_IMPL(mha_manual, CUDA, m) {
   m.impl("fmha_varlen_qkvpacked_fwd", fmha_varlen_qkvpacked_fwd);
   m.impl("fmha_varlen_qkvpacked_bwd", fmha_varlen_qkvpacked_bwd);
   m.impl("kv_append", kv_append);
+  m.impl("kv_append_kv", kv_append_kv);
+  m.impl("kv_append_qkv", kv_append_qkv);
   m.impl("kv_read", kv_read);
   m.impl("fmha_paged_fwd", fmha_paged_fwd);
   m.impl("fmha_causal_varlen_fwd", fmha_causal_varlen_fwd);
@@ -1500,6 +1564,8 @@ TORCH_LIBRARY_IMPL(mha_manual, Meta, m) {
   m.impl("fmha_varlen_qkvpacked_fwd", fmha_varlen_qkvpacked_fwd_meta);
   m.impl("fmha_varlen_qkvpacked_bwd", fmha_varlen_qkvpacked_bwd_meta);
   m.impl("kv_append", kv_append_meta);
+  m.impl("kv_append_kv", kv_append_kv_meta);
+  m.impl("kv_append_qkv", kv_append_qkv_meta);
   m.impl("kv_read", kv_read_meta);
   m.impl("fmha_paged_fwd", fmha_paged_fwd_meta);
   m.impl("fmha_causal_varlen_fwd", fmha_causal_varlen_fwd_meta);
