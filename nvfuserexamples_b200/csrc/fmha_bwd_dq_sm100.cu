@@ -420,7 +420,7 @@ __global__ void __launch_bounds__(kDqThreads, 1) fmha_bwd_dq_kernel(const __grid
         const int slot = w & 1;
         float* st = sStats + slot * 2 * kTileM;
         const float* lse = a.lse + (packed ? static_cast<int64_t>(it.h) * a.total_rows + it.row_base : static_cast<int64_t>(it.bh) * a.S_q);
-        float* delta = a.delta + static_cast<int64_t>(it.bh) * a.S_q;
+        float* delta = a.delta + (CAUSAL ? static_cast<int64_t>(it.h) * a.total_rows + it.row_base : static_cast<int64_t>(it.bh) * a.S_q);
         const int64_t b_o = packed ? static_cast<int64_t>(it.row_base) * a.o_ss : static_cast<int64_t>(it.b) * a.o_sb;
         const int64_t b_do = packed ? static_cast<int64_t>(it.row_base) * a.do_ss : static_cast<int64_t>(it.b) * a.do_sb;
         const unsigned short* po = static_cast<const unsigned short*>(a.o_ptr) + b_o + it.h * a.o_sh + part * 8;
@@ -568,7 +568,8 @@ __global__ void __launch_bounds__(kDqThreads, 1) fmha_bwd_dq_kernel(const __grid
         const int r = cw * 8 + 2 * k + (lane >> 4);
         if ((lane & 15) == 0) {
           sStats[kTileM + r] = sum * (DROP ? 1.0f / a.dropout_scale : 1.0f);
-          if (it.q0 + r < it.q_limit) a.delta[static_cast<int64_t>(it.bh) * a.S_q + it.q0 + r] = sum;
+          if (it.q0 + r < it.q_limit)
+            a.delta[(CAUSAL ? static_cast<int64_t>(it.h) * a.total_rows + it.row_base : static_cast<int64_t>(it.bh) * a.S_q) + it.q0 + r] = sum;
         }
       }
       named_bar_sync(1, kDqCompute);
@@ -673,12 +674,13 @@ __global__ void __launch_bounds__(256) bwd_delta_kernel(const __grid_constant__ 
   const int bh = blockIdx.x, h = bh % a.H, b = bh / a.H;
   const int part = threadIdx.x & 15;
   int q_limit = a.S_q;
-  int64_t base_o = static_cast<int64_t>(b) * a.o_sb, base_do = static_cast<int64_t>(b) * a.do_sb;
+  int64_t base_o = static_cast<int64_t>(b) * a.o_sb, base_do = static_cast<int64_t>(b) * a.do_sb, base_delta = static_cast<int64_t>(bh) * a.S_q;
   if (a.mask_kind == FMHA_MASK_CU_SEQLENS) {
     const int* cu = static_cast<const int*>(a.mask);
     q_limit = packed_rows(cu[b], cu[b + 1], a.S_q, a.total_rows);
     base_o = static_cast<int64_t>(cu[b]) * a.o_ss;
     base_do = static_cast<int64_t>(cu[b]) * a.do_ss;
+    if (a.kv_group > 0) base_delta = static_cast<int64_t>(h) * a.total_rows + cu[b];   // causal
   }
   const unsigned short* po = static_cast<const unsigned short*>(a.o_ptr) + base_o + h * a.o_sh + part * 8;
   const unsigned short* pd = static_cast<const unsigned short*>(a.do_ptr) + base_do + h * a.do_sh + part * 8;
@@ -696,7 +698,7 @@ __global__ void __launch_bounds__(256) bwd_delta_kernel(const __grid_constant__ 
   for (int k = 0; k < 4; ++k) {
     const float sum = row_dot16<BF16>(wo[k], wd[k]);
     const int q = blockIdx.y * 64 + k * 16 + (threadIdx.x >> 4);
-    if (part == 0 && q < q_limit) a.delta[static_cast<int64_t>(bh) * a.S_q + q] = sum;
+    if (part == 0 && q < q_limit) a.delta[base_delta + q] = sum;
   }
 }
 

@@ -175,6 +175,7 @@ __global__ void __launch_bounds__(256, PACKED ? 4 : 8) bwd_prepare_kernel(const 
   int64_t row_o = static_cast<int64_t>(b) * a.o_sb + static_cast<int64_t>(r) * a.o_ss;
   int64_t row_do = static_cast<int64_t>(b) * a.do_sb + static_cast<int64_t>(r) * a.do_ss;
   int q_limit = m.S_q;
+  int64_t at_acc = static_cast<int64_t>(bh) * m.S_q_pad + r0, at_delta = static_cast<int64_t>(bh) * m.S_q + r;   // rows of the scratch
   if constexpr (PACKED) {
     const int* cu = static_cast<const int*>(m.mask);
     const int base = cu[b];
@@ -189,6 +190,10 @@ __global__ void __launch_bounds__(256, PACKED ? 4 : 8) bwd_prepare_kernel(const 
     if (r0 >= q_limit || m.dq_accum == nullptr) return;   // nothing of the accumulator there is added to or read; or rows to zero are all there is to do
     row_o = static_cast<int64_t>(base + r) * a.o_ss;
     row_do = static_cast<int64_t>(base + r) * a.do_ss;
+    if (m.kv_group > 0) {   // causal
+      at_acc = (h * packed_tiles(m.total_rows, m.B) + packed_tile(base, b, 0)) * kTileM + r0;
+      at_delta = static_cast<int64_t>(h) * m.total_rows + base + r;
+    }
   }
   uint4 wo[R], wd[R];
 #pragma unroll
@@ -200,13 +205,13 @@ __global__ void __launch_bounds__(256, PACKED ? 4 : 8) bwd_prepare_kernel(const 
     }
   }
   // the accumulator's rows, a warp's store to 512 consecutive bytes (S_q_pad is a multiple of 128 rows)
-  float4* acc = reinterpret_cast<float4*>(m.dq_accum + (static_cast<int64_t>(bh) * m.S_q_pad + r0) * D) + threadIdx.x;
+  float4* acc = reinterpret_cast<float4*>(m.dq_accum + at_acc * D) + threadIdx.x;
 #pragma unroll
   for (int i = 0; i < 2 * R; ++i) acc[i * 256] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
   for (int k = 0; k < R; ++k) {
     const float sum = row_dot<BF16>(wo[k], wd[k]);
-    if (part == 0 && r + 32 * k < q_limit) m.delta[static_cast<int64_t>(bh) * m.S_q + r + 32 * k] = sum;
+    if (part == 0 && r + 32 * k < q_limit) m.delta[at_delta + 32 * k] = sum;
   }
 }
 
@@ -221,11 +226,13 @@ struct FinishArgs {
   float scale;
   const int* cu_seqlens;  // packed batch: row offsets into the [total_rows, H, D] dQ (sb unused), else null
   int total_rows;
+  bool by_rows;           // the accumulator's tiles have their places by packed_tile
 };
 
 // A block converts 128 rows of a head: coalesced 16-byte reads of the accumulator (eight in flight per thread),
 // through shared memory to coalesced 16-byte writes of the rows.
 constexpr int kFinishRows = 128;
+static_assert(kFinishRows == kTileM, "a block converts a tile of the accumulator");
 template <bool BF16>
 __global__ void __launch_bounds__(256) bwd_finish_kernel(const FinishArgs a) {
   griddep_wait();
@@ -238,13 +245,15 @@ __global__ void __launch_bounds__(256) bwd_finish_kernel(const FinishArgs a) {
   const int r0 = blockIdx.y * R;
   int64_t base = static_cast<int64_t>(b) * a.sb;
   int q_limit = a.S_q;
+  int64_t at = static_cast<int64_t>(bh) * a.S_q_pad + r0;
   if (a.cu_seqlens != nullptr) {
     const int first = a.cu_seqlens[b];
     q_limit = packed_rows(first, a.cu_seqlens[b + 1], a.S_q, a.total_rows);
     base = static_cast<int64_t>(first) * a.ss;
+    if (a.by_rows) at = (h * packed_tiles(a.total_rows, a.B) + packed_tile(first, b, 0)) * R + r0;
   }
   if (r0 >= q_limit) return;
-  const float4* src = reinterpret_cast<const float4*>(a.dq_accum + (static_cast<int64_t>(bh) * a.S_q_pad + r0) * D);
+  const float4* src = reinterpret_cast<const float4*>(a.dq_accum + at * D);
   float4 x[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) x[k] = src[k * 256 + threadIdx.x];
@@ -313,12 +322,7 @@ struct BwdItem {
 // counter.  A packed batch has the pass before it, to zero rows.  The accumulator, its clearing and conversion and the launches around
 // this one took 14 to 30 % of the time (whole backward, without / with dropout: B=2 H=4 S=128 10.6 -> 7.8 / 10.9 -> 8.4 us, B=13 H=12 S=100 15.1 -> 11.2 /
 // 16.6 -> 13.0, B=32 H=16 S=128 27.8 -> 19.5 / 29.1 -> 23.0, B=128 H=16 94.4 -> 68.3 / 97.8 -> 75.7; packed, B=32 H=16 of 64 to 128 rows 34.2 -> 27.7 / 36.1 -> 31.2).
-// Place of a sequence's key tile in kv_partial, by the row it begins at: with sequences one after the other none shares its place with another, whatever
-// their lengths, and there are no more than total_rows / 128 + B (places for the longest one's tiles in every sequence took 17 GB for one of 8192 rows
-// among 64 of 14 000 rows together, 8 key heads of 128; these take 0.7).
-int64_t kv_partial_tiles(int64_t total_rows, int64_t B) { return total_rows / kTileN + B; }
-__device__ __forceinline__ int64_t kv_partial_tile(int row_base, int b, int tile) { return static_cast<int64_t>(row_base / kTileN) + b + tile; }
-
+//
 // CAUSAL: a packed batch whose rows see the keys up to their own position, with a.kv_group query heads to a key head.  An item is a key tile of
 // a KEY head: its query tiles are those from the diagonal on of every query head of the group, one head after the other, so dK and dV are summed
 // over the group in tensor memory, always in the same order.  Items count heads and sequences first and, last, the number of query tiles from the
@@ -736,10 +740,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1) fmha_bwd_kernel(const __grid_c
       const BwdItem cur = fetch_item(n++, 0);
       if (cur.id < 0) break;
       if (cur.n_cols <= 0) continue;
-      // logsumexp rows: [B*H, S_q], or [H, total_rows] for a packed batch; delta is always [B*H, S_q]
+      // logsumexp rows: [B*H, S_q], or [H, total_rows] for a packed batch; delta is [B*H, S_q], or lies as the logsumexp does (CAUSAL)
       QTile q = first_q(cur);
       const float* lse = a.lse + (packed ? static_cast<int64_t>(q.h) * a.total_rows + cur.row_base : static_cast<int64_t>(cur.b * a.H + q.h) * a.S_q);
-      const float* delta = a.delta + static_cast<int64_t>(cur.b * a.H + q.h) * a.S_q;
+      const float* delta = a.delta + (CAUSAL ? static_cast<int64_t>(q.h) * a.total_rows + cur.row_base : static_cast<int64_t>(cur.b * a.H + q.h) * a.S_q);
       for (int i = 0; i < cur.n_q; ++i, ++t) {
         float x[4], d[4];
 #pragma unroll
@@ -766,7 +770,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) fmha_bwd_kernel(const __grid_c
         next_q(cur, q);
         if (CAUSAL && q.h != h) {
           lse += a.total_rows;
-          delta += a.S_q;
+          delta += a.total_rows;
         }
       }
     }
@@ -845,7 +849,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) fmha_bwd_kernel(const __grid_c
       const bool edge = packed && (k0 + quad * 32 + 32 > q_limit);
       if constexpr (CAUSAL) {
         if (a.kv_parts > 1) {   // fp32 sums of this part's query heads: whole sectors, 512 consecutive bytes of a warp's store
-          float* dst = a.kv_partial + (kv_partial_tile(row_base, b, k0 / kTileN) * item_heads + h) * (2 * kTileN * D) + dq_accum_index<D>(row, cq * DQ);
+          float* dst = a.kv_partial + (packed_tile(row_base, b, k0 / kTileN) * item_heads + h) * (2 * kTileN * D) + dq_accum_index<D>(row, cq * DQ);
 #pragma unroll
           for (int which = 0; which < 2; ++which)
 #pragma unroll
@@ -916,6 +920,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) fmha_bwd_kernel(const __grid_c
                  static_cast<int>(r.w), true);
       pending = false;
     };
+    [[maybe_unused]] const int acc_tiles = static_cast<int>(packed_tiles(a.total_rows, a.B));   // CAUSAL: tiles of a head in the accumulator
     [[maybe_unused]] int prev_tile = 0;       // D = 64: tile t-1 as dq_readout wants it,
     [[maybe_unused]] bool dq_out = true;      // and whether its dQ has been read out
 
@@ -939,6 +944,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) fmha_bwd_kernel(const __grid_c
         if (c < a.S_k) key_add = reinterpret_cast<const float*>(a.mask)[static_cast<size_t>(cur.b) * a.S_k + c] * kLog2eB;
       }
 
+      [[maybe_unused]] const int acc_tile0 = static_cast<int>(packed_tile(cur.row_base, cur.b, 0));
       QTile q = first_q(cur);
       for (int i = 0; i < n_q; ++i, ++t, next_q(cur, q)) {
         // ONE_KV: O and dO for delta of rows [8 cw, +8) of the tile, eight lanes a row, four rows an instruction.  (Its place among the
@@ -1076,7 +1082,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) fmha_bwd_kernel(const __grid_c
         if constexpr (D == 64) {
           if (!dq_out) dq_readout(t - 1, prev_tile);
           dq_out = false;
-          prev_tile = ONE_KV ? 2 * i + (w & 1) : CAUSAL ? (cur.b * a.H + q.h) * n_q_all + q.tile : bh * n_q_all + i;
+          prev_tile = ONE_KV ? 2 * i + (w & 1) : CAUSAL ? acc_tile0 + q.h * acc_tiles + q.tile : bh * n_q_all + i;
         }
       }
       pending = true;
@@ -1128,7 +1134,7 @@ __global__ void __launch_bounds__(256) bwd_join_kernel(const __grid_constant__ B
   const int base = cu[b], limit = packed_rows(base, cu[b + 1], a.S_q, a.total_rows) - kv_tile * kTileN - r0;
   if (limit <= 0) return;
   // (2 or 4 parts: two at a time, so that all their loads are in flight; added up in this order, whatever order the parts were done in)
-  const float4* src = reinterpret_cast<const float4*>(a.kv_partial + ((kv_partial_tile(base, b, kv_tile) * a.H_kv + hk) * a.kv_parts * 2 + which) * (kTileN * D) + r0 * D) +
+  const float4* src = reinterpret_cast<const float4*>(a.kv_partial + ((packed_tile(base, b, kv_tile) * a.H_kv + hk) * a.kv_parts * 2 + which) * (kTileN * D) + r0 * D) +
                       threadIdx.x;
   float4 x[N];
 #pragma unroll
@@ -1284,12 +1290,12 @@ int launch_bwd_prepare(const fmha_tensor4& ot, const fmha_tensor4& dot, const Bw
 }
 
 int launch_bwd_finish(const float* dq_accum, const fmha_tensor4& dq, int B, int H, int S_q, int S_q_pad, int dtype, float scale,
-                      const int* cu_seqlens, int total_rows, cudaStream_t stream) {
+                      const int* cu_seqlens, int total_rows, bool by_rows, cudaStream_t stream) {
   FinishArgs f;
   f.dq_accum = dq_accum; f.dq = dq.ptr;
   f.sb = dq.stride_b; f.sh = dq.stride_h; f.ss = dq.stride_s;
   f.B = B; f.H = H; f.S_q = S_q; f.S_q_pad = S_q_pad; f.scale = scale;
-  f.cu_seqlens = cu_seqlens; f.total_rows = total_rows;
+  f.cu_seqlens = cu_seqlens; f.total_rows = total_rows; f.by_rows = by_rows;
   const dim3 grid(static_cast<unsigned>(B) * H, static_cast<unsigned>((S_q + kFinishRows - 1) / kFinishRows));
   auto kfn = dtype == FMHA_DTYPE_BF16 ? bwd_finish_kernel<true> : bwd_finish_kernel<false>;
   const cudaError_t e = launch_overlapped(kfn, grid, dim3(256), 0, stream, f);

@@ -13,6 +13,7 @@
 
 #include "../../include/fmha_sm100.h"
 #include "fmha_capi_common.h"
+#include "fmha_device_utils.cuh"
 #include "fmha_kernel_args.h"
 #include "philox.cuh"
 #include "sm100_ptx.cuh"
@@ -442,7 +443,7 @@ int fmha_sm100_bwd(const fmha_bwd_params* p, void* stream_) {
   if (e != 0) return cuda_fail(static_cast<cudaError_t>(e));
   if (!two_pass && !(p->flags & FMHA_FLAG_BWD_SKIP_FINISH)) {
     // the main kernel leaves the dropout factor 1/(1-p) out of dS; it is applied here (and to dK, dV in its epilogue)
-    e = launch_bwd_finish(dq_accum, tdq, p->B, p->H, p->S_q, s_q_pad, p->dtype, p->scale * a.dropout_scale, cu_seqlens, p->total_rows, stream);
+    e = launch_bwd_finish(dq_accum, tdq, p->B, p->H, p->S_q, s_q_pad, p->dtype, p->scale * a.dropout_scale, cu_seqlens, p->total_rows, false, stream);
     if (e != 0) return cuda_fail(static_cast<cudaError_t>(e));
   }
   return FMHA_OK;
@@ -500,16 +501,21 @@ int fmha_sm100_causal_fwd(const fmha_causal_fwd_params* p, void* stream_) {
   return e != 0 ? cuda_fail(static_cast<cudaError_t>(e)) : FMHA_OK;
 }
 
+// By the rows that there are, not by sequences times the longest: see packed_tile.
+static size_t causal_accum_bytes(const fmha_causal_bwd_params* p) {
+  return bwd_accum_bytes(static_cast<size_t>(packed_tiles(p->total_rows, p->B)) * p->H, kTileM, p->D);
+}
+static size_t causal_delta_bytes(const fmha_causal_bwd_params* p) { return static_cast<size_t>(p->H) * p->total_rows * sizeof(float); }
+
 int fmha_sm100_causal_bwd_workspace_bytes(const fmha_causal_bwd_params* p, size_t* bytes) {
   if (p == nullptr || bytes == nullptr) return FMHA_ERR_BAD_ARG;
   const int rc = validate_causal(p->struct_bytes, sizeof(fmha_causal_bwd_params), p->dtype, p->B, p->H, p->H_kv, p->max_seqlen, p->D, p->scale,
                                  p->total_rows);
   if (rc != FMHA_OK) return rc;
-  const size_t bh = static_cast<size_t>(p->B) * p->H, pad = (static_cast<size_t>(p->max_seqlen) + kTileM - 1) / kTileM * kTileM;
-  *bytes = align256(bwd_accum_bytes(bh, pad, p->D)) + align256(bh * p->max_seqlen * sizeof(float)) + 256;
+  *bytes = align256(causal_accum_bytes(p)) + align256(causal_delta_bytes(p)) + 256;
   if (p->H > 0) {
     const int parts = bwd_causal_parts(sm_count(), p->B, p->H, p->H_kv, p->max_seqlen, p->total_rows);
-    if (parts > 1) *bytes += static_cast<size_t>(kv_partial_tiles(p->total_rows, p->B)) * p->H_kv * parts * kTileN * p->D * 2 * sizeof(float);
+    if (parts > 1) *bytes += static_cast<size_t>(packed_tiles(p->total_rows, p->B)) * p->H_kv * parts * kTileN * p->D * 2 * sizeof(float);
   }
   return FMHA_OK;
 }
@@ -540,11 +546,10 @@ int fmha_sm100_causal_bwd(const fmha_causal_bwd_params* p, void* stream_) {
   if ((rc = make_tmap(&a.tm_do, tdo, p->dtype, 1, H, rows, D, kTileM))) return rc;
   if ((rc = make_tmap(&a.tm_dk, tdk, p->dtype, 1, Hk, rows, D, 32, D / 4))) return rc;
   if ((rc = make_tmap(&a.tm_dv, tdv, p->dtype, 1, Hk, rows, D, 32, D / 4))) return rc;
-  const size_t bh = static_cast<size_t>(p->B) * H;
   const int pad = (p->max_seqlen + kTileM - 1) / kTileM * kTileM;
   a.dq_accum = static_cast<float*>(p->workspace);
-  a.delta = reinterpret_cast<float*>(static_cast<uint8_t*>(p->workspace) + align256(bwd_accum_bytes(bh, pad, D)));
-  a.work_counter = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(a.delta) + align256(bh * p->max_seqlen * sizeof(float)));
+  a.delta = reinterpret_cast<float*>(static_cast<uint8_t*>(p->workspace) + align256(causal_accum_bytes(p)));
+  a.work_counter = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(a.delta) + align256(causal_delta_bytes(p)));
   a.total_rows = rows;
   a.H_kv = Hk;
   a.kv_group = H / Hk;
@@ -580,7 +585,7 @@ int fmha_sm100_causal_bwd(const fmha_causal_bwd_params* p, void* stream_) {
   if (e == 0) e = launch_bwd(a, D, p->dtype, stream);
   if (e == 0 && a.kv_parts > 1) e = launch_bwd_causal_join(a, D, p->dtype, stream);
   if (e == 0 && D == 64)
-    e = launch_bwd_finish(a.dq_accum, tdq, p->B, H, p->max_seqlen, pad, p->dtype, p->scale, p->cu_seqlens, rows, stream);
+    e = launch_bwd_finish(a.dq_accum, tdq, p->B, H, p->max_seqlen, pad, p->dtype, p->scale, p->cu_seqlens, rows, true, stream);
   return e != 0 ? cuda_fail(static_cast<cudaError_t>(e)) : FMHA_OK;
 }
 

@@ -97,13 +97,13 @@ struct BwdArgs {
   int persist;   // a CTA takes further work items of the grid when it has done its own
   int H_kv, kv_group;   // causal variants: key heads, query heads per key head (else 0)
   int kv_parts;         // ... and over how many items of the dK / dV kernel the query heads of a key head are dealt out (bwd_causal_parts)
-  float* kv_partial;    // [kv_partial_tiles, H_kv * kv_parts, 2, 128 * D] fp32 dV and dK of the items in the order of dq_accum_index, if kv_parts > 1
+  float* kv_partial;    // [packed_tiles, H_kv * kv_parts, 2, 128 * D] fp32 dV and dK of the items in the order of dq_accum_index, if kv_parts > 1
   int B, H, S_q, S_k;
   float scale;       // softmax scale
   float scale_log2;  // softmax scale * log2(e)
   const float* lse;  // [B*H, S_q] natural log
-  float* delta;        // [B*H, S_q] rowsum(dO * O); not used with ONE_KV
-  float* dq_accum;     // head dimension 64: [B*H, S_q_pad, D] fp32 in the blocked order of dq_accum_index, zero on entry; null: not used
+  float* delta;        // [B*H, S_q] (causal variants: [H, total_rows]) rowsum(dO * O); not used with ONE_KV
+  float* dq_accum;     // head dimension 64: [B*H, S_q_pad, D] (causal: [H, packed_tiles, 128 * D]) fp32 in the blocked order of dq_accum_index, zero on entry; null: not used
   int* work_counter;   // zero on entry; the persistent CTAs draw their work items from it (not with ONE_KV: every grid-th item)
   // FMHA_MASK_CU_SEQLENS: mask = int32 [B+1] row offsets into the packed [total_rows, H, D] tensors; the raw
   // dK / dV pointers serve the row-wise stores of a sequence's last, partial key tile
@@ -153,7 +153,6 @@ bool fwd_dense_applies(const FwdArgs& a, int D);
 int launch_fwd_dense(const FwdArgs& a, int dtype, cudaStream_t stream);
 int launch_bwd_dq(const BwdArgs& a, int dtype, cudaStream_t stream);   // head dimension 128: dQ, delta, work counter
 int launch_bwd(const BwdArgs& a, int D, int dtype, cudaStream_t stream);
-int64_t kv_partial_tiles(int64_t total_rows, int64_t B);   // places of key tiles in kv_partial
 // causal: kv_parts for these sizes
 int bwd_causal_parts(int64_t sms, int64_t B, int64_t H, int64_t H_kv, int64_t max_len, int64_t total_rows);
 // ... and dK and dV of the parts' sum
@@ -164,7 +163,7 @@ bool bwd_one_kv(int D, int64_t heads, int S_q, int S_k);
 // `m`: the main kernel's arguments (sizes, mask, Philox, workspace)
 int launch_bwd_prepare(const fmha_tensor4& ot, const fmha_tensor4& dot, const BwdArgs& m, int dtype, cudaStream_t stream);
 int launch_bwd_finish(const float* dq_accum, const fmha_tensor4& dq, int B, int H, int S_q, int S_q_pad, int dtype, float scale,
-                      const int* cu_seqlens, int total_rows, cudaStream_t stream);
+                      const int* cu_seqlens, int total_rows, bool by_rows, cudaStream_t stream);
 
 // Multiprocessors of the current device, asked for once per device.
 inline int sm_count() {

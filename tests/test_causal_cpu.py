@@ -71,3 +71,20 @@ def test_workspace_and_checks_of_the_backward():
     p.struct_bytes -= 4
     assert lib.fmha_sm100_causal_bwd(C.byref(p), None) == capi.FMHA_ERR_BAD_ARG
     assert lib.fmha_sm100_causal_bwd(None, None) == capi.FMHA_ERR_BAD_ARG
+
+
+def workspace_bytes(lens, H, H_kv, D):
+    p = capi.CausalBwdParams()
+    p.struct_bytes, p.dtype, p.B, p.H, p.H_kv, p.max_seqlen, p.D, p.scale, p.total_rows = (
+        C.sizeof(p), capi.DTYPE_BF16, len(lens), H, H_kv, max(lens), D, 0.125, sum(lens))
+    n = C.c_size_t()
+    assert capi.load().fmha_sm100_causal_bwd_workspace_bytes(C.byref(p), C.byref(n)) == capi.FMHA_OK
+    return n.value
+
+
+@pytest.mark.parametrize("lens", [[16384] + [247] * 199, [8192] + [92] * 511, [1] * 4000, [5000]], ids=["200", "512", "short", "one"])
+@pytest.mark.parametrize("D,H", [(64, 16), (128, 16), (64, 32)])
+def test_workspace_goes_by_rows(lens, D, H):
+    """Whatever the longest sequence: dQ's sums (head dimension 64) and delta, a row of either per row and one tile more per sequence."""
+    rows = sum(lens) + 128 * len(lens)
+    assert workspace_bytes(lens, H, H, D) <= rows * H * 4 * (1 + (D if D == 64 else 0)) + 4096

@@ -246,3 +246,54 @@ def test_no_rows_and_no_grad(cuda_device):
     assert (o == 0).all()
     with torch.inference_mode():
         assert not ops.fmha_causal_varlen(q, k, v, cu, 5).requires_grad
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_one_long_document_among_many_short_ones(cuda_device, D):
+    """The backward pass's scratch goes by rows; gradients at sequences that begin anywhere within a tile's rows."""
+    lens, H, H_kv = [40] * 30 + [3001] + [1, 128, 127, 129, 256, 0, 60] * 8, 12, 6
+    q, k, v, d_o, cu = batch(lens, H, H_kv, D, torch.float16, cuda_device, before=50, behind=9)
+    o, lse = ops.fmha_causal_varlen_fwd(q, k, v, cu, max(lens))
+    for _ in range(2):   # (the scratch of the first call is the second one's, with what it left there)
+        torch.cuda.reset_peak_memory_stats()
+        held = torch.cuda.memory_allocated()
+        dq, dk, dv = ops.fmha_causal_varlen_bwd(d_o, q, k, v, o, lse, cu, max(lens))
+        used = torch.cuda.max_memory_allocated() - held
+        ops.check_status()
+        ref = ref64.causal(q, k, v, lens, d_o, offsets=cu[:-1].tolist())
+        for name, x in dict(dq=dq, dk=dk, dv=dv).items():
+            ref64.check(x[50:-9], (ref[name][0][50:-9], ref[name][1][50:-9]), name)
+            assert (x[:50] == 0).all() and (x[-9:] == 0).all()
+        rows = q.shape[0] + 128 * len(lens)
+        parts = 4 * rows * H_kv * D * 8   # at most, if a key head's query heads are dealt out
+        assert used <= rows * H * 4 * (1 + (D if D == 64 else 0)) + parts + 3 * q.nbytes + (4 << 20)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_replays_start_from_clear_sums(cuda_device, D):
+    """A captured forward and backward pass, replayed with other inputs: each replay's gradients, dq among them, are those of its inputs."""
+    lens = [150, 260, 900]
+    q, k, v, d_o, cu = batch(lens, 8, 4, D, torch.bfloat16, cuda_device)
+
+    def step():
+        o, lse = ops.fmha_causal_varlen_fwd(q, k, v, cu, 900)
+        return (o, *ops.fmha_causal_varlen_bwd(d_o, q, k, v, o, lse, cu, 900))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for seed in (11, 12, 13):
+        for x, y in zip((q, k, v, d_o), batch(lens, 8, 4, D, torch.bfloat16, cuda_device, seed=seed)):
+            x.copy_(y)
+        for x in got:
+            x.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        ref = ref64.causal(q, k, v, lens, d_o)
+        for name, x in zip(("o", "dq", "dk", "dv"), got):
+            ref64.check(x, ref[name], name)
