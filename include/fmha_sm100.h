@@ -180,7 +180,7 @@ typedef struct {
   float* lse;           /* optional [H, total_rows] natural-log logsumexp */
   const int32_t* cu_seqlens; /* device int32 [B+1] */
   int32_t total_rows;
-  int32_t flags;        /* FMHA_FLAG_ZERO_UNCOVERED */
+  int32_t flags;        /* FMHA_FLAG_ZERO_UNCOVERED (such rows have a logsumexp of -infinity then) */
   int32_t* status;      /* optional device int32[4] */
 } fmha_causal_fwd_params;
 

@@ -128,6 +128,7 @@ struct OutsideArgs {
   UncoveredRows u;
   int B, H, D;
   const int* cu;
+  float* lse;   // [H, total_rows], or null: such rows get -infinity
 };
 // Bound by its writes; kOutsideRows rows of all heads per block and step.
 constexpr int kOutsideRows = 8;
@@ -144,11 +145,13 @@ __global__ void __launch_bounds__(256) zero_outside_rows_kernel(const __grid_con
         const int k = k0 + i / per_row, piece = i % per_row;
         unsigned short* row = static_cast<unsigned short*>(u.grad[t].ptr) + (k < first ? k : last + static_cast<int64_t>(k - first)) * u.grad[t].stride_s;
         *reinterpret_cast<uint4*>(row + piece / (D / 8) * u.grad[t].stride_h + piece % (D / 8) * 8) = make_uint4(0u, 0u, 0u, 0u);
+        if (a.lse != nullptr && piece % (D / 8) == 0)
+          a.lse[static_cast<int64_t>(piece / (D / 8)) * u.total_rows + (k < first ? k : last + static_cast<int64_t>(k - first))] = -INFINITY;
       }
 }
-static int zero_outside_rows(const UncoveredRows& u, int B, int H, int D, const int* cu, cudaStream_t stream) {
+static int zero_outside_rows(const UncoveredRows& u, int B, int H, int D, const int* cu, cudaStream_t stream, float* lse = nullptr) {
   if (u.mode != kUncoveredCut) return 0;
-  const OutsideArgs a = {u, B, H, D, cu};
+  const OutsideArgs a = {u, B, H, D, cu, lse};
   const int blocks = std::min(u.total_rows / kOutsideRows + 1, 8 * sm_count());
   const cudaError_t e = launch_overlapped(zero_outside_rows_kernel, dim3(blocks), dim3(256), 0, stream, a);
   return static_cast<int>(e != cudaSuccess ? e : cudaGetLastError());
@@ -486,7 +489,7 @@ int fmha_sm100_causal_fwd(const fmha_causal_fwd_params* p, void* stream_) {
   if (p->flags & FMHA_FLAG_ZERO_UNCOVERED) {
     const UncoveredRows u = {{to}, rows, uncovered_mode(p->B, p->max_seqlen, rows)};
     a.zero_uncovered = u.mode;
-    if (const int e = zero_outside_rows(u, p->B, p->H, p->D, p->cu_seqlens, stream)) return cuda_fail(static_cast<cudaError_t>(e));
+    if (const int e = zero_outside_rows(u, p->B, p->H, p->D, p->cu_seqlens, stream, p->lse)) return cuda_fail(static_cast<cudaError_t>(e));
   }
   a.o_ptr = to.ptr; a.o_ss = to.stride_s; a.o_sh = to.stride_h; a.o_sb = to.stride_b;
   a.B = p->B; a.H = p->H; a.S_q = a.S_k = p->max_seqlen;

@@ -129,9 +129,10 @@ __device__ __forceinline__ int64_t packed_tile(int row_base, int b, int tile) { 
 // rows than its own.  (One caller per head for all of them took three to four times as long as the fill of whole tensors that this
 // replaces where a buffer was far from full.)  Offsets outside the tensor, which the host cannot see, are cut to its rows.
 // Only callers with r1 > len or len > max_len can have a share.
+// lse: the tensor's [H, total_rows] logsumexp, which such rows get as -infinity, or null.
 __device__ __forceinline__ void zero_uncovered_rows(void* base, int64_t stride_s, int64_t stride_h, int h, int b, int B,
                                                     const int* cu, int max_len, int total_rows, int D, int r0, int r1, bool outside,
-                                                    int tid, int nthreads) {
+                                                    int tid, int nthreads, float* lse = nullptr) {
   const int lo = cu[b], hi = cu[b + 1], len = hi - lo;
   r1 = min(r1, max_len);
   auto zero = [&](int64_t from, int64_t to) {
@@ -141,6 +142,8 @@ __device__ __forceinline__ void zero_uncovered_rows(void* base, int64_t stride_s
     for (int64_t i = tid; i < (to - from) * per_row; i += nthreads)
       *reinterpret_cast<uint4*>(static_cast<unsigned short*>(base) + (from + i / per_row) * stride_s + h * stride_h +
                                 (i % per_row) * 8) = make_uint4(0u, 0u, 0u, 0u);
+    if (lse != nullptr)
+      for (int64_t i = from + tid; i < to; i += nthreads) lse[static_cast<int64_t>(h) * total_rows + i] = -INFINITY;
   };
   if (len > max_len) {
     const int64_t cut = len - max_len, at = static_cast<int64_t>(lo) + max_len;

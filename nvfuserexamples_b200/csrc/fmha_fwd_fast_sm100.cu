@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(fast_threads<D>(), FastSmem<D, DROP>::kCtasPer
     if (q0 >= (CAUSAL ? q_limit : len)) {   // this sequence has no such query tile (whole CTA, before any barrier)
       if (a.zero_uncovered)
         zero_uncovered_rows(a.o_ptr, a.o_ss, a.o_sh, h, b, a.B, cu, a.S_q, a.total_rows, D, q0, q0 + kTileM,
-                            a.zero_uncovered == kUncoveredAll, threadIdx.x, blockDim.x);
+                            a.zero_uncovered == kUncoveredAll, threadIdx.x, blockDim.x, CAUSAL ? a.lse : nullptr);
       return;
     }
     if (threadIdx.x == 0) *uncovered = a.zero_uncovered && (q0 + kTileM > len || all > len);
@@ -502,7 +502,7 @@ __global__ void __launch_bounds__(fast_threads<D>(), FastSmem<D, DROP>::kCtasPer
   if constexpr (PACKED) {   // last, so that no start of a CTA waits for the offsets
     if (*uncovered)
       zero_uncovered_rows(a.o_ptr, a.o_ss, a.o_sh, h, b, a.B, reinterpret_cast<const int*>(a.mask), a.S_q, a.total_rows, D, q0,
-                          q0 + kTileM, a.zero_uncovered == kUncoveredAll, threadIdx.x, blockDim.x);
+                          q0 + kTileM, a.zero_uncovered == kUncoveredAll, threadIdx.x, blockDim.x, CAUSAL ? a.lse : nullptr);
   }
   tc_fence_before_sync();
   __syncthreads();

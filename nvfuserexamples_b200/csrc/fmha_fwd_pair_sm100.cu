@@ -534,7 +534,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) fmha_fwd_pair_kernel(const __
           const int q0 = it.q0 + g * kTileM;
           if (q0 < a.S_q && (q0 + kTileM > it.q_limit || cu[it.b + 1] - it.row_base > it.q_limit))
             zero_uncovered_rows(a.o_ptr, a.o_ss, a.o_sh, it.h, it.b, a.B, cu, a.S_q, a.total_rows, D, q0, q0 + kTileM,
-                                a.zero_uncovered == kUncoveredAll, row, 128);
+                                a.zero_uncovered == kUncoveredAll, row, 128, CAUSAL ? a.lse : nullptr);
         }
       }
       item_done(n);

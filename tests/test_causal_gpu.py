@@ -297,3 +297,22 @@ def test_replays_start_from_clear_sums(cuda_device, D):
         ref = ref64.causal(q, k, v, lens, d_o)
         for name, x in zip(("o", "dq", "dk", "dv"), got):
             ref64.check(x, ref[name], name)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lens,max_len,before,behind", [([200, 77], 200, 37, 90), ([900, 40, 1300, 650] * 3, 1300, 5, 2000), ([300, 120], 200, 0, 0), ([0], 5, 0, 300),
+                                                        ([30, 0, 20], 30, 400, 500), ([2000, 700], 600, 3, 1)], ids=str)
+def test_logsumexp_of_rows_outside_the_sequences(cuda_device, D, lens, max_len, before, behind):
+    """-infinity, as their zeros are an empty sum: before the first and behind the last sequence, and past max_seqlen of one."""
+    H, H_kv = (4, 2) if len(lens) < 5 else (16, 4)
+    q, k, v, _, cu = batch(lens, H, H_kv, D, torch.bfloat16, cuda_device, before=before, behind=behind)
+    for fill in (float("nan"), 3.0):
+        torch.full((H, q.shape[0]), fill, device=cuda_device)   # (freed at once: what lies where the next tensors of this size are put)
+        o, lse = ops.fmha_causal_varlen_fwd(q, k, v, cu, max_len)
+        ops.check_status()
+        live, at = torch.zeros(q.shape[0], dtype=torch.bool, device=cuda_device), before
+        for n in lens:
+            live[at:at + min(n, max_len)] = True
+            at += n
+        assert torch.isneginf(lse[:, ~live]).all() and torch.isfinite(lse[:, live]).all()
+        assert (o[~live] == 0).all() and torch.isfinite(o).all()
