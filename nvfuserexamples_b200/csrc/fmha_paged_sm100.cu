@@ -266,10 +266,10 @@ __device__ __forceinline__ bool way_begin(const PagedArgs& a, PgWay& w) {
   }
   w.b = w.tiles == 1 ? w.g : w.g / w.tiles;
   w.tile = w.g - w.b * w.tiles;
-  const int within = static_cast<int>(w0 - before * a.H_kv);
-  w.hk = within / w.u.weight;
+  const long long within = w0 - before * a.H_kv;   // (a group's key heads together may have 2^31 steps and more: 2^31 rows of 64 heads)
+  w.hk = static_cast<int>(within < (1ll << 31) ? static_cast<unsigned>(within) / static_cast<unsigned>(w.u.weight) : within / w.u.weight);
   w.n = 0;
-  way_part<KEYS>(a, w, within - w.hk * w.u.weight);
+  way_part<KEYS>(a, w, static_cast<int>(within - static_cast<long long>(w.hk) * w.u.weight));
   return true;
 }
 template <int KEYS>

@@ -119,3 +119,18 @@ def test_queries_of_all_sizes(cuda_device, D, dtype, sizes):
         check(o[:, live], (want_o[0][:, live], want_o[1][:, live]), f"o at {size}")
         check(lse[live], (want_lse[0][live], want_lse[1][live]), f"lse at {size}")
     ops.check_status()
+
+
+def test_a_line_of_more_than_32_bits(cuda_device):
+    """A sequence at the documented limit of rows, with so many key heads that their steps together pass 2^31.  Its pages do not exist (rows of
+    zeros), so there is nothing to bring in: every key counts the same."""
+    H, page, D = 66, 1 << 16, 64
+    width = ((1 << 31) - page) // page
+    k_cache = torch.zeros(1, H, page, D, dtype=torch.float16, device=cuda_device)
+    table = torch.full((1, width), -1, dtype=torch.int32, device=cuda_device)
+    q = randn(1, H, D, dtype=torch.float16, device=cuda_device, seed=1)
+    n = width * page
+    o, lse = ops.fmha_paged_fwd(q, k_cache, k_cache, table, ints([n], cuda_device))
+    ops.check_status()
+    assert (o == 0).all()
+    assert (lse - torch.tensor(float(n)).log().item()).abs().max() < 2.0 ** -12 * 2
