@@ -687,14 +687,16 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> fmha_causal_varlen_bwd(const at::
 // ---------------------------------------------------------------------------------------
 // paged caches: [pages, H_kv, page rows, D] in 16 bits, or [.., D/2] bytes of 4-bit codes with [.., D/32, 2] fp16 scales and bases
 // ---------------------------------------------------------------------------------------
+// A size that a traced call may not leave open (its other sizes stay as they are: Tensor::size would fix them all).
+int64_t fixed_size(const at::Tensor& x, int64_t dim) { return x.sym_size(dim).guard_int(__FILE__, __LINE__); }
 void check_pages(const at::Tensor& x, const char* name, const at::Tensor& like, int64_t last) {
-  TORCH_CHECK(x.dim() == 4 && x.size(3) == last && x.sizes() == like.sizes(), "mha_manual: ", name, " must be [pages, H_kv, page rows, ",
+  TORCH_CHECK(x.dim() == 4 && fixed_size(x, 3) == last && x.sym_sizes() == like.sym_sizes(), "mha_manual: ", name, " must be [pages, H_kv, page rows, ",
               last, "], as the other cache");
 }
 void check_params(const OptTensor& x, const char* name, const at::Tensor& cache, int64_t D) {
   TORCH_CHECK(x.has_value(), "mha_manual: a 4-bit cache has ", name);
-  TORCH_CHECK(x->dim() == 5 && x->size(0) == cache.size(0) && x->size(1) == cache.size(1) && x->size(2) == cache.size(2) && x->size(3) == D / 32 &&
-                  x->size(4) == 2 && x->scalar_type() == at::kHalf,
+  TORCH_CHECK(x->dim() == 5 && x->sym_size(0) == cache.sym_size(0) && fixed_size(*x, 1) == fixed_size(cache, 1) &&
+                  fixed_size(*x, 2) == fixed_size(cache, 2) && fixed_size(*x, 3) == D / 32 && fixed_size(*x, 4) == 2 && x->scalar_type() == at::kHalf,
               "mha_manual: ", name, " must be float16 [pages, H_kv, page rows, D/32, 2]");
 }
 // What the shapes say, without looking at memory: the head dimension.
@@ -705,12 +707,12 @@ int64_t check_cache_shapes(const at::Tensor& k_cache, const at::Tensor& v_cache,
               "mha_manual: k_cache must be float16, bfloat16 or uint8 (4-bit codes)");
   TORCH_CHECK(v_cache.scalar_type() == k_cache.scalar_type(), "mha_manual: v_cache has a different dtype");
   TORCH_CHECK(k_cache.dim() == 4, "mha_manual: k_cache must be [pages, H_kv, page rows, D]");
-  const int64_t D = k_cache.size(3) * (four ? 2 : 1);
+  const int64_t D = fixed_size(k_cache, 3) * (four ? 2 : 1);
   TORCH_CHECK(D == 64 || D == 128, "mha_manual: head dimension must be 64 or 128, got ", D);
-  check_pages(v_cache, "v_cache", k_cache, k_cache.size(3));
-  TORCH_CHECK(k_cache.size(2) > 0 && k_cache.size(2) % 16 == 0, "mha_manual: pages must have a multiple of 16 rows");
-  TORCH_CHECK(k_cache.size(1) > 0, "mha_manual: k_cache has no heads");
-  TORCH_CHECK(k_cache.size(0) <= INT32_MAX && k_cache.size(2) <= (1 << 16), "mha_manual: cache too large");
+  check_pages(v_cache, "v_cache", k_cache, fixed_size(k_cache, 3));
+  TORCH_CHECK(fixed_size(k_cache, 2) > 0 && fixed_size(k_cache, 2) % 16 == 0, "mha_manual: pages must have a multiple of 16 rows");
+  TORCH_CHECK(fixed_size(k_cache, 1) > 0, "mha_manual: k_cache has no heads");
+  TORCH_CHECK(k_cache.sym_size(0) <= INT32_MAX && fixed_size(k_cache, 2) <= (1 << 16), "mha_manual: cache too large");
   if (four) {
     check_params(k_params, "k_params", k_cache, D);
     check_params(v_params, "v_params", k_cache, D);
@@ -753,12 +755,12 @@ void fill_cache(fmha_kv_cache& c, const at::Tensor& on, const at::Tensor& k_cach
   c.table_width = static_cast<int32_t>(table.size(1));
   c.table_stride = table.size(0) > 1 ? table.stride(0) : 0;
 }
-// Lengths and offsets, by shape; then as the kernels read them.
-void check_lens_shapes(const at::Tensor& table, const OptTensor& seqlens, const OptTensor& cu, int64_t rows) {
-  const int64_t B = table.size(0);
-  if (seqlens.has_value()) TORCH_CHECK(seqlens->dim() == 1 && seqlens->numel() == B, "mha_manual: seqlens must be [B], B lines of block_table");
+// Lengths and offsets, by shape; then as the kernels read them.  (The numbers of rows, sequences and pages may be symbols here, in a traced call.)
+void check_lens_shapes(const at::Tensor& table, const OptTensor& seqlens, const OptTensor& cu, const c10::SymInt& rows) {
+  const c10::SymInt B = table.sym_size(0);
+  if (seqlens.has_value()) TORCH_CHECK(seqlens->dim() == 1 && seqlens->sym_size(0) == B, "mha_manual: seqlens must be [B], B lines of block_table");
   if (cu.has_value()) {
-    TORCH_CHECK(cu->dim() == 1 && cu->numel() == B + 1 && B > 0, "mha_manual: cu_seqlens must be [B+1], B lines of block_table");
+    TORCH_CHECK(cu->dim() == 1 && cu->sym_size(0) == B + 1 && B > 0, "mha_manual: cu_seqlens must be [B+1], B lines of block_table");
   } else {
     TORCH_CHECK(rows == 0 || (B > 0 && rows % B == 0), "mha_manual: without cu_seqlens every sequence has the same number of rows");
   }
@@ -770,16 +772,17 @@ at::Tensor as_ints(const at::Tensor& x, const at::Tensor& on, const char* name) 
 }
 
 void check_append_shapes(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_cache, int64_t D, const OptTensor& q, const OptTensor& inv_freq) {
-  TORCH_CHECK(k.dim() == 3 && k.sizes() == v.sizes() && k.size(1) == k_cache.size(1) && k.size(2) == D, "mha_manual: k and v must be [total_rows, H_kv, D]");
+  TORCH_CHECK(k.dim() == 3 && k.sym_sizes() == v.sym_sizes() && fixed_size(k, 1) == fixed_size(k_cache, 1) && fixed_size(k, 2) == D,
+              "mha_manual: k and v must be [total_rows, H_kv, D]");
   TORCH_CHECK(k.scalar_type() == at::kHalf || k.scalar_type() == at::kBFloat16, "mha_manual: k must be float16 or bfloat16");
   TORCH_CHECK(v.scalar_type() == k.scalar_type() && (k_cache.scalar_type() == at::kByte || k_cache.scalar_type() == k.scalar_type()),
               "mha_manual: k, v and a 16-bit cache must have the same dtype");
   if (q.has_value())
-    TORCH_CHECK(q->dim() == 3 && q->size(0) == k.size(0) && q->size(2) == D && q->scalar_type() == k.scalar_type(),
+    TORCH_CHECK(q->dim() == 3 && q->sym_size(0) == k.sym_size(0) && fixed_size(*q, 2) == D && q->scalar_type() == k.scalar_type(),
                 "mha_manual: q must be [total_rows, H, D] of the dtype of k");
   if (inv_freq.has_value()) {
-    const int64_t n = inv_freq->numel(), step = k_cache.scalar_type() == at::kByte ? 32 : 8;
     TORCH_CHECK(inv_freq->dim() == 1 && inv_freq->scalar_type() == at::kFloat, "mha_manual: inv_freq must be float32 [pairs]");
+    const int64_t n = fixed_size(*inv_freq, 0), step = k_cache.scalar_type() == at::kByte ? 32 : 8;
     TORCH_CHECK(2 * n <= D && n % step == 0, "mha_manual: inv_freq must have a multiple of ", step, " pairs, at most D/2, got ", n);
   }
 }
@@ -878,12 +881,12 @@ Pair kv_read(const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Ten
 }
 
 void check_paged_shapes(const at::Tensor& q, const at::Tensor& k_cache, int64_t D, bool with_cu, int64_t max_rows) {
-  TORCH_CHECK(q.dim() == 3 && q.size(2) == D && q.size(1) > 0 && q.size(1) % k_cache.size(1) == 0,
+  TORCH_CHECK(q.dim() == 3 && fixed_size(q, 2) == D && fixed_size(q, 1) > 0 && fixed_size(q, 1) % fixed_size(k_cache, 1) == 0,
               "mha_manual: q must be [total_rows, H, D], H a multiple of the heads of the cache");
   TORCH_CHECK(q.scalar_type() == at::kHalf || q.scalar_type() == at::kBFloat16, "mha_manual: q must be float16 or bfloat16");
   TORCH_CHECK(k_cache.scalar_type() == at::kByte || k_cache.scalar_type() == q.scalar_type(), "mha_manual: q and a 16-bit cache must have the same dtype");
   TORCH_CHECK(!with_cu || max_rows > 0, "mha_manual: with cu_seqlens, max_seqlen_q must be positive");
-  TORCH_CHECK(k_cache.size(0) > 0, "mha_manual: k_cache has no pages");
+  TORCH_CHECK(k_cache.sym_size(0) > 0, "mha_manual: k_cache has no pages");
 }
 std::tuple<at::Tensor, at::Tensor> fmha_paged_fwd(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& block_table,
                                                   const at::Tensor& seqlens, const OptTensor& cu_seqlens, int64_t max_seqlen_q,
@@ -1417,36 +1420,37 @@ at::Tensor fmha_varlen_qkvpacked_bwd_meta(const at::Tensor& d_o, const at::Tenso
 void meta_check_causal(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& cu, int64_t max_seqlen) {
   TORCH_CHECK(q.dim() == 3 && k.dim() == 3, "mha_manual: q and k must be [total_rows, H, D]");
   TORCH_CHECK(q.scalar_type() == at::kHalf || q.scalar_type() == at::kBFloat16, "mha_manual: q must be float16 or bfloat16");
-  TORCH_CHECK(v.sizes() == k.sizes() && k.size(0) == q.size(0) && k.size(2) == q.size(2) && k.size(1) > 0 && q.size(1) % k.size(1) == 0 &&
+  TORCH_CHECK(v.sym_sizes() == k.sym_sizes() && k.sym_size(0) == q.sym_size(0) && fixed_size(k, 2) == fixed_size(q, 2) && fixed_size(k, 1) > 0 &&
+                  fixed_size(q, 1) % fixed_size(k, 1) == 0 &&
                   k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(),
               "mha_manual: packed q, k, v must have the same rows, head dimension and dtype, and q a multiple of the heads of k and v");
-  TORCH_CHECK(q.size(2) == 64 || q.size(2) == 128, "mha_manual: head dimension must be 64 or 128, got ", q.size(2));
-  TORCH_CHECK(cu.dim() == 1 && cu.numel() >= 2, "mha_manual: cu_seqlens must be [B+1]");
+  TORCH_CHECK(fixed_size(q, 2) == 64 || fixed_size(q, 2) == 128, "mha_manual: head dimension must be 64 or 128, got ", fixed_size(q, 2));
+  TORCH_CHECK(cu.dim() == 1 && cu.sym_size(0) >= 2, "mha_manual: cu_seqlens must be [B+1]");
   TORCH_CHECK(max_seqlen > 0, "mha_manual: max_seqlen must be positive");
 }
 std::tuple<at::Tensor, at::Tensor> fmha_causal_varlen_fwd_meta(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                                                                const at::Tensor& cu_seqlens, int64_t max_seqlen, c10::optional<double>) {
   meta_check_causal(q, k, v, cu_seqlens, max_seqlen);
-  return {at::empty(q.sizes(), q.options()), at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat))};
+  return {at::empty_symint(q.sym_sizes(), q.options()), at::empty_symint({q.sym_size(1), q.sym_size(0)}, q.options().dtype(at::kFloat))};
 }
 std::tuple<at::Tensor, at::Tensor, at::Tensor> fmha_causal_varlen_bwd_meta(const at::Tensor& d_o, const at::Tensor& q, const at::Tensor& k,
                                                                            const at::Tensor& v, const at::Tensor& o, const at::Tensor& lse,
                                                                            const at::Tensor& cu_seqlens, int64_t max_seqlen,
                                                                            c10::optional<double>) {
   meta_check_causal(q, k, v, cu_seqlens, max_seqlen);
-  TORCH_CHECK(o.sizes() == q.sizes() && d_o.sizes() == q.sizes(), "mha_manual: o and d_o must have the shape of q");
-  TORCH_CHECK(lse.scalar_type() == at::kFloat && lse.numel() == q.size(0) * q.size(1), "mha_manual: lse must be float32 [H, total_rows]");
-  return {at::empty(q.sizes(), q.options()), at::empty(k.sizes(), k.options()), at::empty(v.sizes(), v.options())};
+  TORCH_CHECK(o.sym_sizes() == q.sym_sizes() && d_o.sym_sizes() == q.sym_sizes(), "mha_manual: o and d_o must have the shape of q");
+  TORCH_CHECK(lse.scalar_type() == at::kFloat && lse.sym_numel() == q.sym_size(0) * q.sym_size(1), "mha_manual: lse must be float32 [H, total_rows]");
+  return {at::empty_symint(q.sym_sizes(), q.options()), at::empty_symint(k.sym_sizes(), k.options()), at::empty_symint(v.sym_sizes(), v.options())};
 }
 
 OptTensor kv_append_meta(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& block_table,
                          const at::Tensor& seqlens, const OptTensor& cu_seqlens, const OptTensor& q, const OptTensor& inv_freq, bool,
                          const OptTensor& k_params, const OptTensor& v_params) {
   check_append_shapes(k, v, k_cache, check_cache_shapes(k_cache, v_cache, block_table, k_params, v_params), q, inv_freq);
-  check_lens_shapes(block_table, seqlens, cu_seqlens, k.size(0));
+  check_lens_shapes(block_table, seqlens, cu_seqlens, k.sym_size(0));
   check_written(k_cache, v_cache, k_params, v_params);
   count_writes(k_cache, v_cache, k_params, v_params);
-  return q.has_value() ? OptTensor(at::empty(q->sizes(), q->options())) : OptTensor();
+  return q.has_value() ? OptTensor(at::empty_symint(q->sym_sizes(), q->options())) : OptTensor();
 }
 void kv_append_kv_meta(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& block_table,
                        const at::Tensor& seqlens, const OptTensor& cu_seqlens, const OptTensor& inv_freq, bool interleaved, const OptTensor& k_params,
@@ -1463,15 +1467,15 @@ Pair kv_read_meta(const at::Tensor& k_cache, const at::Tensor& v_cache, const at
   const int64_t D = check_cache_shapes(k_cache, v_cache, block_table, k_params, v_params);
   check_lens_shapes(block_table, OptTensor(), cu_seqlens, total_rows);
   const auto options = k_cache.options().dtype(read_type(k_cache, bf16));
-  return {at::empty({total_rows, k_cache.size(1), D}, options), at::empty({total_rows, k_cache.size(1), D}, options)};
+  return {at::empty({total_rows, fixed_size(k_cache, 1), D}, options), at::empty({total_rows, fixed_size(k_cache, 1), D}, options)};
 }
 std::tuple<at::Tensor, at::Tensor> fmha_paged_fwd_meta(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
                                                        const at::Tensor& block_table, const at::Tensor& seqlens, const OptTensor& cu_seqlens,
                                                        int64_t max_seqlen_q, c10::optional<double>, const OptTensor& k_params,
                                                        const OptTensor& v_params) {
   check_paged_shapes(q, k_cache, check_cache_shapes(k_cache, v_cache, block_table, k_params, v_params), cu_seqlens.has_value(), max_seqlen_q);
-  check_lens_shapes(block_table, seqlens, cu_seqlens, q.size(0));
-  return {at::empty(q.sizes(), q.options()), at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat))};
+  check_lens_shapes(block_table, seqlens, cu_seqlens, q.sym_size(0));
+  return {at::empty_symint(q.sym_sizes(), q.options()), at::empty_symint({q.sym_size(1), q.sym_size(0)}, q.options().dtype(at::kFloat))};
 }
 
 }  // namespace

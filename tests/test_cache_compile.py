@@ -60,6 +60,35 @@ def test_causal_attention_compiles_with_its_gradients():
     assert o.shape == q.shape and lse.shape == (8, 40)
 
 
+def test_changing_batches_compile_once_more():
+    """Numbers of rows, sequences and pages that change from call to call are symbols after the second: no compilation for each."""
+    from torch._dynamo.testing import CompileCounterWithBackend
+
+    def step(q, k, k_cache, v_cache, table, lens):
+        turned = ops.kv_append(k, k, k_cache, v_cache, table, lens, q=q)
+        return ops.fmha_paged_fwd(turned, k_cache, v_cache, table, lens)[0]
+
+    def train(q, k, cu):
+        return ops.fmha_causal_varlen(q, k, k, cu, 20)
+
+    torch._dynamo.reset()
+    counter = CompileCounterWithBackend("aot_eager")
+    f = torch.compile(step, fullgraph=True, backend=counter)
+    with torch.no_grad():
+        for B, pages, width in ((3, 10, 4), (5, 20, 6), (7, 35, 9), (11, 50, 10), (6, 31, 7)):
+            cache = meta(pages, 2, 32, 128)
+            assert f(meta(B, 6, 128), meta(B, 2, 128), cache, cache.clone(), meta(B, width, **INT), meta(B, **INT)).shape == (B, 6, 128)
+    assert counter.frame_count == 2
+    torch._dynamo.reset()
+    counter = CompileCounterWithBackend("aot_eager")
+    f = torch.compile(train, fullgraph=True, backend=counter)
+    for B, rows in ((2, 40), (3, 50), (7, 90), (9, 33)):
+        q, k = meta(rows, 8, 64).requires_grad_(), meta(rows, 2, 64).requires_grad_()
+        f(q, k, meta(B + 1, **INT)).sum().backward()
+        assert q.grad.shape == q.shape and k.grad.shape == k.shape
+    assert counter.frame_count == 2
+
+
 @pytest.mark.parametrize("bits", [16, 4])
 def test_append_counts_as_a_write(bits):
     """The version counters of what is written move, so that autograd notices; of what is not, they do not."""
