@@ -8,7 +8,8 @@
 // type of k; a 4-bit cache codes those.
 //
 // Measured (device time): appending 9 389 rows of 32/8 heads of 128, 16 bits, 42 us, 5.5 TB/s of what is read and written; one row of 64 sequences 3.0 us, little
-// more than an empty launch; 5 321 rows of 16/4 heads of 64 in 4 bits 9.8 us, 2.9 TB/s, bound by instructions (some 30 a code); reading back 9 600 rows of 8 heads of
+// more than an empty launch, 3.4 in 4 bits; 5 321 rows of 16/4 heads of 64 in 4 bits 9.8 us, 2.9 TB/s: 7.05 million warp instructions, which take 6.2 us at one a
+// cycle of each scheduler (4.4 by bytes), the rest latency: 1.4 of 4.8 warps of a scheduler can issue, 59 % of the cycles do (24 warps an SM at 80 registers); reading back 9 600 rows of 8 heads of
 // 128 14.2 us, 5.6 TB/s, and 8 100 of 4 heads of 64 from 4 bits 5.0 us, 2.2 TB/s (few loads a warp: its row's place, then its heads).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

@@ -25,10 +25,12 @@
 // and below 2^-7 or from 32 on the scales are multiplied by a power of two (p_top, v_factor).  (Without that, o was off by 2 % for values of 1e-4, and by more than itself
 // where the largest probability, 2^24 times the others, had a value of zero; it costs 3 %, a load and some ten instructions a step.)
 //
-// Measured (device time, 32/8 heads of 128; bytes of the cache once).  16 bits: 32 sequences of 8000 rows, one new row: 157 us, 6.7 TB/s; 16 of 200-4000, four new
+// Measured (device time, 32/8 heads of 128; bytes of the cache once).  16 bits: 32 sequences of 8000 rows, one new row: 157 to 162 us, 6.7 to 6.5 TB/s, of 1000-8192 98 us, 6.2 TB/s; 16 of 200-4000, four new
 // rows: 34.6 us, 4.0 TB/s.  4 bits: two of 90 001-131 072: 63.5 us, 4.5 TB/s; 32 of 1000-8192: 48.5 us, 3.9 TB/s.  Of a short run some 4.5 us pass before the
-// first keys have landed and 3 at the join; in 4 bits the steady state is bound by issue and latency (1.8 instructions a cycle and SM; ALU 43 %, tensor
-// pipe 24 %, DRAM 50 %).  Before: tiles of 16 query rows and a grid of splits 39 / 107 / 122 us (four new rows / batch / long), a line of work 46 / 86 / 117,
+// first keys have landed and 3 at the join; in 4 bits the steady state is bound by issue and latency (1.6 to 1.8 instructions a cycle and SM; ALU 37-43 %, tensor
+// pipe 24 %, DRAM 44-50 %).  More than 8 query rows of a key head in 4 bits (two columns; at D = 128 in 168 registers with 224 bytes of spill stores, 280 of loads): 32 of
+// 500-4000, 64/4 heads 32.8 us, D = 64 21.9; 16 of 200-4000, four new rows, 32/8 heads 32.6.  Not meant for new rows by the hundred: every 16 query rows read the whole
+// cache again (256 new rows of 4 sequences of 4000, 32/8 heads: 366 us, 476 in 4 bits, where the products would take 41).  Before: tiles of 16 query rows and a grid of splits 39 / 107 / 122 us (four new rows / batch / long), a line of work 46 / 86 / 117,
 // the cache as the operand of 16 rows 48 / 55 / 71, shares in the accumulators' order 45 / 54 / 69, starts counted in the line 35 / 47 / 61.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
