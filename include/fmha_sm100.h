@@ -254,7 +254,7 @@ typedef struct {
    -infinity, as do rows outside the sequences and past max_rows of theirs.  What the cache holds behind a sequence's last row does not matter; an infinite or
    NaN value in V of a LATER new row can reach the earlier ones.  Scores count up to 2^24 in absolute value; the exponentials of larger ones are not to be told apart.
    From a 4-bit cache products are formed in fp16: q is rounded to it, a row with values of 1024 and more divided by a power of two before; probabilities, in a scaled
-   form, and their products with the scales of V as well, each once.  Relative to a row's largest probability, one of 2^-25 still has 11 bits, and from 2^-36 on they end. */
+   form, and their products with the scales of V as well, each once (a scale itself to 2^-30 of the largest, where that is 32 or more).  Relative to a row's largest probability, one of 2^-25 still has 11 bits, and from 2^-36 on they end. */
 typedef struct {
   int32_t struct_bytes; /* sizeof(fmha_paged_params) */
   int32_t dtype;        /* of q, o and a 16-bit cache */

@@ -138,7 +138,8 @@ __device__ __forceinline__ void code_pairs(uint32_t w, uint32_t (&v)[4]) {
 }
 
 // 4 bits, by the exponent field of V's largest scale (which is 2^(field - 15) to twice that; an infinity counts as the largest number): P is taken
-// 2^p_top-fold and the scales 2^v_factor-fold, so that P times a scale stays below 2^16.  Scales from 2^-7 to 32 are left as they are.
+// 2^p_top-fold and the scales 2^v_factor-fold, so that P times a scale stays below 2^16.  Scales from 2^-7 to 32 are left as they are; next to larger ones
+// a scale is rounded to 2^-30 of the largest, which only shows where a key with nearly all of the probability has values a millionth of another's.
 __device__ __forceinline__ int p_top(int field) { return 15 - min(max(field - 15, 0), 4); }
 __device__ __forceinline__ int v_factor(int field) { return field >= 20 ? 19 - min(field, 30) : field >= 8 ? 0 : 15 - field; }
 // 2^k as a half, -14 <= k <= 15, twice
